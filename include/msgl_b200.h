@@ -483,6 +483,74 @@ int msgl_prefill_layer_pages(const msgl_new_rows* rows, void* q, void* k_cache, 
                              int is_cross_attention, int sliding_window_size, int page_size, int64_t total,
                              void* stream);
 
+/*
+ * A K/V pool held in 4 bits.  Sixteen slots are a block; a pool (K or V) is (num_slots / 16, num_kv_heads,
+ * 9 * head_dim / 2) elements of the 16-bit data type, contiguous and 16-byte aligned: per block and KV head the
+ * codes of its sixteen rows, head_dim / 2 bytes each, then sixteen rows of (scale, bias) pairs, one pair for every
+ * 64 elements of a row.  An element is scale * code + bias; in a group of 64, bias = min,
+ * scale = T((max - min) / 15) (0 where that is below 2^-100) and code = min(15, rint((x - bias) / scale)).  The
+ * 32-bit word r * (head_dim / 64) + g of a row holds elements 64 g + 8 r to 64 g + 8 r + 7, element e of them in
+ * nibble e / 2 + 4 * (e % 2).  A pool of zero bytes reads as zeros.  Magnitudes above 2^15 and
+ * infinities are stored as 2^15, NaN as 0, and reported: a status word gets 4 added.  Slots and page ids outside the pool get 2 added.
+ * Operators over the pool take pages of page_size tokens, a multiple of 16 (slot = page * page_size + offset),
+ * and head_dim 128 or 256.  No operator of the reference has such a pool.
+ */
+
+/*
+ * k_cache[indices[r]] = k[r], v_cache[indices[r]] = v[r] for r < length, quantised.  k and v: (length,
+ * num_kv_heads, head_dim), dense heads, token strides in elements, rows 8-byte aligned.  A row whose index is
+ * outside [0, num_slots) is dropped.  The indices of a call are distinct: of two rows with one index each group
+ * of 64 elements, and its pair, is one or the other's.
+ */
+int msgl_store_kv_cache_q4(void* k_cache, void* v_cache, const int32_t* indices, const void* k, const void* v,
+                           int length, int num_kv_heads, int head_dim, int64_t num_slots, int64_t k_token_stride,
+                           int64_t v_token_stride, int dtype, void* status_word, void* stream);
+
+/* The other way round: k[r], v[r] (contiguous) = the values of slot indices[r], rounded once; zeros for an index
+ * outside the pool. */
+int msgl_load_kv_cache_q4(const void* k_cache, const void* v_cache, const int32_t* indices, void* k, void* v,
+                          int length, int num_kv_heads, int head_dim, int64_t num_slots, int dtype,
+                          void* status_word, void* stream);
+
+/*
+ * msgl_qk_norm_rope_store for this pool: the rotated, rounded keys and the values are quantised into it.  q is
+ * read (any token stride) and its result goes to q_out (n_tokens, num_q_heads, head_dim), contiguous.  Positions
+ * below 2^24; the angle is good to 1e-6 turns whatever the position.
+ */
+int msgl_qk_norm_rope_store_q4(const void* q, const void* k, const void* v, const void* q_weight,
+                               const void* k_weight, const int32_t* positions, const int32_t* out_loc, void* q_out,
+                               void* k_cache, void* v_cache, int n_tokens, int num_q_heads, int num_kv_heads,
+                               int head_dim, int rotary_dim, double rope_base, float eps, int64_t num_slots,
+                               int64_t q_token_stride, int64_t k_token_stride, int64_t v_token_stride, int dtype,
+                               void* status_word, void* stream);
+
+/* Scratch of the decode op below (total_pages: length of page_indices). */
+size_t msgl_decode_workspace_bytes_q4(int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                      int64_t total_pages, int page_size);
+
+/*
+ * msgl_paged_decode_attention_p16 over this pool: arguments, clamps, gate and zeros of empty sequences as there.
+ * Codes go to the tensor cores as they are, scales and biases are applied in fp32; the softmax weight times the
+ * value's scale is rounded to the data type.
+ */
+int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const void* v_cache,
+                                   const int32_t* page_indptr, const int32_t* page_indices, const int32_t* kv_lens,
+                                   const void* gate, void* out, void* workspace, size_t workspace_bytes, int batch,
+                                   int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots, int dtype,
+                                   float sm_scale, int page_size, int64_t total_pages, void* stream);
+
+/*
+ * msgl_paged_prefill_attention_p16 over this pool: masks, arguments and zeros of rows without a key as there.
+ * Scratch: msgl_prefill_workspace_bytes with total_kv = total_pages * page_size.
+ */
+int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const void* v_cache,
+                                    const int32_t* qo_indptr, const int32_t* page_indptr,
+                                    const int32_t* page_indices, const int32_t* kv_lens, const int32_t* prefix_lens,
+                                    const void* gate, void* out, void* workspace, size_t workspace_bytes, int batch,
+                                    int total_q, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
+                                    int dtype, float sm_scale, int max_len_extend, int is_cross_attention,
+                                    int sliding_window_size, int page_size, int64_t total_pages, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,12 @@ from .kernel import (  # noqa: F401
     paged_prefill_attention,
     paged_prefill_attention_p16,
     store_kv_cache,
+    kv_cache_q4_shape,
+    load_kv_cache_q4,
+    paged_decode_attention_q4,
+    paged_prefill_attention_q4,
+    qk_norm_rope_store_q4,
+    store_kv_cache_q4,
 )
 
 __all__ = [
@@ -25,4 +31,10 @@ __all__ = [
     "gather_kv_indices",
     "fast_compare_key",
     "qk_norm_rope_store",
+    "kv_cache_q4_shape",
+    "load_kv_cache_q4",
+    "paged_decode_attention_q4",
+    "paged_prefill_attention_q4",
+    "qk_norm_rope_store_q4",
+    "store_kv_cache_q4",
 ]

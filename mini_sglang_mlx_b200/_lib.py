@@ -71,6 +71,17 @@ SIGNATURES = {
              _i64, _i, _f, _i, _i, _i, _i, _i64, _vp]),
     "msgl_store_kv_cache": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i, _vp, _vp]),
     "msgl_gather_kv_indices": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i64, _i64, _i64, _vp, _vp]),
+    "msgl_store_kv_cache_q4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i, _vp, _vp]),
+    "msgl_load_kv_cache_q4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i, _vp, _vp]),
+    "msgl_qk_norm_rope_store_q4": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, C.c_double, _f, _i64, _i64, _i64, _i64,
+             _i, _vp, _vp]),
+    "msgl_decode_workspace_bytes_q4": (_sz, [_i, _i, _i, _i, _i64, _i]),
+    "msgl_paged_decode_attention_q4": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i64, _i, _f, _i, _i64, _vp]),
+    "msgl_paged_prefill_attention_q4": (
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i64, _i, _f, _i, _i, _i, _i,
+             _i64, _vp]),
     "msgl_fast_compare_key": (_i64, [_vp, _vp, _i64, _i64, _i]),
     "msgl_qk_norm_rope_store": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _f, _i64, _i64,

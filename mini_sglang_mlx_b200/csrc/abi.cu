@@ -14,28 +14,25 @@
 
 #include "../../include/msgl_b200.h"
 #include "decode_splitkv.cuh"
+#include "host_common.cuh"
 #include "prefill_pair.cuh"
 #include "prefill_tc.cuh"
 #include "qk_norm_rope.cuh"
 
-namespace {
+using namespace msgl_host;
 
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
-int fail(int code, const std::string& msg) {
+int msgl_host::fail(int code, const std::string& msg) {
   g_last_error = msg;
   return code;
 }
 
-int cuda_fail(const char* op, cudaError_t e) {
+int msgl_host::cuda_fail(const char* op, cudaError_t e) {
   return fail(MSGL_CUDA_ERROR, std::string(op) + ": CUDA error: " + cudaGetErrorString(e));
 }
 
-// Head of every workspace: the device status word (first 256 bytes), then kTicketSlots arrival
-// counters of split-KV pieces at a fixed place, so that a buffer re-used by calls of different
-// shapes never finds anything but the zeros the kernels leave there.
-constexpr size_t kTicketSlots = 16384;
-constexpr size_t kStatusBytes = 256 + kTicketSlots * sizeof(int);
+namespace {
 
 // Scratch of msgl_paged_decode_attention_static: lives in the library's image,
 // so every GPU that loads the library holds these bytes until the process exits.
@@ -70,7 +67,9 @@ int static_scratch_for_current_device(void** out) {
 constexpr int kDecWarps = 4;
 constexpr int kDecStages = 3;
 
-int sm_count_cached() {
+}  // namespace
+
+int msgl_host::sm_count_cached() {
   static thread_local int cached_dev = -1;
   static thread_local int cached_sms = 0;
   int dev = 0;
@@ -84,25 +83,7 @@ int sm_count_cached() {
   return cached_sms;
 }
 
-// Dynamic shared memory of a kernel, set once per kernel, device and thread (the runtime call takes
-// longer than the rest of a launch's preparation).
-template <typename K>
-cudaError_t allow_smem(K kernel, int bytes) {
-  struct Done {
-    const void* fn;
-    int dev, bytes;
-  };
-  static thread_local Done done[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const void* fn = reinterpret_cast<const void*>(kernel);
-  Done& d = done[((reinterpret_cast<uintptr_t>(fn) >> 4) ^ dev) % 64];
-  if (d.fn == fn && d.dev == dev && d.bytes == bytes) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) d = Done{fn, dev, bytes};
-  return e;
-}
+namespace {
 
 // ---- TMA tensor maps over a K or V pool (page-granular entries)
 // The encoder is a driver-API function; it is looked up through the runtime, so the library
@@ -173,10 +154,12 @@ bool make_pool_map(CUtensorMap* out, PoolBox form, const void* base, int64_t num
   return true;
 }
 
+}  // namespace
+
 // 3-D map over the query tensor (tokens, query heads, head_dim): a box is 64 elements x the
 // `group` heads of one KV head x 128 / group tokens, i.e. the 128 packed rows of a query
 // sub-tile in the order the kernel numbers them.  Needs a group that divides 128.
-bool make_query_tensor_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int group,
+bool msgl_host::make_query_tensor_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int group,
                            int head_dim, int dtype) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (!enc || total_q <= 0 || group <= 0 || 128 % group != 0 || num_q_heads % group != 0 ||
@@ -196,6 +179,8 @@ bool make_query_tensor_map(CUtensorMap* out, const void* q, int total_q, int num
   return r == CUDA_SUCCESS;
 }
 
+namespace {
+
 // 2-D map over the query rows (tokens x heads, head_dim) for tile::gather4: a box is one row x 64 elements.
 bool make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int head_dim, int dtype) {
   EncodeTiledFn enc = tensor_map_encoder();
@@ -211,49 +196,17 @@ bool make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launches `kernel` so that its CTAs may be scheduled while the previous kernel of the
-// stream drains (programmatic dependent launch); the kernel itself waits for the previous
-// kernel's memory with griddepcontrol.wait before it touches global memory.
-template <typename... P, typename... A>
-cudaError_t launch_clusters(int cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                            const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                             const A&... args) {
-  return launch_clusters(1, kernel, grid, block, smem, s, args...);
-}
-
-// ---- prefill scheduling decision (shared by the workspace query and the launch)
-struct PrefillPlan {
-  int kv_chunk;        // 0 = no kv split
-  int64_t items;       // grid.x
-  size_t part_o_bytes, part_ml_bytes, plan_bytes;
-  bool fused_merge;    // the CTA that arrives last at a unit merges it (else: a second launch)
-};
-
+}  // namespace
 
 // Query blocks that fill at most one 128-row sub-tile (verify, draft blocks) run the
 // one-sub-tile shape (64-token key tiles, two CTAs per SM); longer chunks the two-sub-tile
 // shape with 128-token key tiles.  head_dim 256 always runs the one-sub-tile shape (its
 // output accumulator alone takes 256 of the 512 TMEM columns), one CTA per SM.
-bool prefill_short_q(int max_len_extend, int group, int head_dim) {
+bool msgl_host::prefill_short_q(int max_len_extend, int group, int head_dim) {
   return head_dim == 256 || static_cast<int64_t>(max_len_extend) * group <= msgl::kTcSub;
 }
+
+namespace {
 
 // Pairs of CTAs (prefill_pair.cuh) serve query blocks of more than one 128-row tile whose key range is
 // not split: head_dim 256 always, head_dim 128 where they are the faster of two forms.  A pair takes
@@ -288,7 +241,9 @@ bool prefill_pairs(int batch, int total_q, int64_t total_kv, int group, int num_
   return waves(sms / 2) * (17. + 1.9 * key_tiles) < waves(sms) * (20. + 4. * key_tiles);
 }
 
-PrefillPlan plan_prefill(int batch, int total_q, int64_t total_kv, int hq, int hkv, int head_dim,
+}  // namespace
+
+PrefillPlan msgl_host::plan_prefill(int batch, int total_q, int64_t total_kv, int hq, int hkv, int head_dim,
                          int max_len_extend, int window, int sms) {
   // The key range is split only when the query tiles alone cannot give every CTA slot of the
   // GPU a CTA; then about two CTAs per slot are made.
@@ -351,6 +306,8 @@ PrefillPlan plan_prefill(int batch, int total_q, int64_t total_kv, int hq, int h
   }
   return pl;
 }
+
+namespace {
 
 // The waiting pattern of the attention kernels on a barrier that nothing completes: two warps wait
 // (bounded), the first to run out raises the CTA's abort flag, the other sees it and leaves too,
@@ -841,8 +798,6 @@ struct PageIndex {
 };
 
 }  // namespace
-
-static bool aligned16(const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; }
 
 // Arrival counters of the decode op: one per (sequence, query head).  They sit in the workspace header when there
 // are at most kTicketSlots of them; a larger batch gets a region of its own behind the header, cleared by every call.

@@ -458,6 +458,190 @@ PyObject* qk_norm_rope_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+// ------------------------------------------------------------------ the pool held in 4 bits
+// A pair of pools (num_blocks, num_kv_heads, 9 * head_dim / 2) of a 16-bit type, on the current device.
+struct Pool4 {
+  int hkv, d, dtype, device;
+  int64_t num_slots;
+};
+bool pool4(const Tensor& kc, const Tensor& vc, Pool4* s) {
+  if (kc.dim() != 3 || !kc.is_cuda() || kc.sizes() != vc.sizes() || kc.size(2) == 0 || kc.size(2) % 9 != 0) return false;
+  s->dtype = dtype_code(kc);
+  if (s->dtype < 0 || vc.scalar_type() != kc.scalar_type() || vc.device() != kc.device() || !kc.is_contiguous() ||
+      !vc.is_contiguous())
+    return false;
+  s->num_slots = kc.size(0) * 16;
+  s->hkv = static_cast<int>(kc.size(1));
+  s->d = static_cast<int>(kc.size(2) / 9 * 2);
+  s->device = kc.device().index();
+  return c10::cuda::current_device() == s->device;
+}
+// Rows (n, heads, head_dim) for such a pool: dense heads, any token stride.
+bool rows4(const Tensor& t, const Tensor& pool, const Pool4& s, int64_t n, int64_t heads) {
+  return t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == s.d && t.scalar_type() == pool.scalar_type() &&
+         t.device() == pool.device() && rows_dense(t, s.d);
+}
+
+// (k_cache, v_cache, indices, k, v, stream)
+PyObject* store_kv_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "store_kv_q4 takes 6 arguments");
+  ALL_TENSORS(a, 5);
+  const Tensor &kc = THPVariable_Unpack(a[0]), &vc = THPVariable_Unpack(a[1]), &idx = THPVariable_Unpack(a[2]),
+               &k = THPVariable_Unpack(a[3]), &v = THPVariable_Unpack(a[4]);
+  Pool4 s;
+  if (!pool4(kc, vc, &s) || !index_ok(idx, kc.device()) || !rows4(k, kc, s, idx.numel(), s.hkv) ||
+      !rows4(v, kc, s, idx.numel(), s.hkv))
+    Py_RETURN_NONE;
+  int64_t stream;
+  Scratch ws;
+  if (!stream_of(a[5], s.device, &stream) || !scratch_for(s.device, stream, kDecode, 256, &ws)) return nullptr;
+  const int rc = unlocked([&] {
+    return msgl_store_kv_cache_q4(kc.data_ptr(), vc.data_ptr(), i32(idx), k.data_ptr(), v.data_ptr(),
+                                  static_cast<int>(idx.numel()), s.hkv, s.d, s.num_slots, k.stride(0), v.stride(0), s.dtype,
+                                  ws.ptr, reinterpret_cast<void*>(stream));
+  });
+  if (rc) return raise_status(rc);
+  Py_RETURN_TRUE;
+}
+
+// (k_cache, v_cache, indices, stream) -> (k, v)
+PyObject* load_kv_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) return PyErr_Format(PyExc_TypeError, "load_kv_q4 takes 4 arguments");
+  ALL_TENSORS(a, 3);
+  const Tensor &kc = THPVariable_Unpack(a[0]), &vc = THPVariable_Unpack(a[1]), &idx = THPVariable_Unpack(a[2]);
+  Pool4 s;
+  if (!pool4(kc, vc, &s) || !index_ok(idx, kc.device())) Py_RETURN_NONE;
+  int64_t stream;
+  Scratch ws;
+  if (!stream_of(a[3], s.device, &stream) || !scratch_for(s.device, stream, kDecode, 256, &ws)) return nullptr;
+  Tensor rows[2];
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    for (Tensor& t : rows)
+      t = at::empty({idx.numel(), s.hkv, s.d}, at::TensorOptions().dtype(kc.scalar_type()).device(kc.device()));
+  }
+  const int rc = unlocked([&] {
+    return msgl_load_kv_cache_q4(kc.data_ptr(), vc.data_ptr(), i32(idx), rows[0].data_ptr(), rows[1].data_ptr(),
+                                 static_cast<int>(idx.numel()), s.hkv, s.d, s.num_slots, s.dtype, ws.ptr,
+                                 reinterpret_cast<void*>(stream));
+  });
+  if (rc) return raise_status(rc);
+  THPObjectPtr k(THPVariable_Wrap(std::move(rows[0]))), v(THPVariable_Wrap(std::move(rows[1])));
+  if (!k || !v) return nullptr;
+  return PyTuple_Pack(2, k.get(), v.get());
+}
+
+// (q, k, v, q_weight, k_weight, positions, out_loc, k_cache, v_cache, rope_base, eps, rotary_dim, stream) -> q
+PyObject* qk_norm_rope_store_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 13) return PyErr_Format(PyExc_TypeError, "qk_norm_rope_store_q4 takes 13 arguments");
+  for (int i = 0; i < 9; ++i)
+    if (!is_tensor(a[i]) && !((i == 3 || i == 4) && a[i] == Py_None)) Py_RETURN_NONE;
+  const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &v = THPVariable_Unpack(a[2]),
+               &pos = THPVariable_Unpack(a[5]), &loc = THPVariable_Unpack(a[6]), &kc = THPVariable_Unpack(a[7]),
+               &vc = THPVariable_Unpack(a[8]);
+  Pool4 s;
+  if (!pool4(kc, vc, &s) || q.dim() != 3) Py_RETURN_NONE;
+  const c10::Device dev = kc.device();
+  const int64_t nt = q.size(0), hq = q.size(1);
+  if (!rows4(q, kc, s, nt, hq) || !rows4(k, kc, s, nt, s.hkv) || !rows4(v, kc, s, nt, s.hkv) || !index_ok(pos, dev) ||
+      !index_ok(loc, dev) || pos.numel() != nt || loc.numel() != nt)
+    Py_RETURN_NONE;
+  const void* wt[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i) {
+    if (a[3 + i] == Py_None) continue;
+    const Tensor& w = THPVariable_Unpack(a[3 + i]);
+    if (w.scalar_type() != q.scalar_type() || w.device() != dev || w.dim() != 1 || w.size(0) != s.d || !w.is_contiguous())
+      Py_RETURN_NONE;
+    wt[i] = w.data_ptr();
+  }
+  ARG_FLOAT(base, a[9]);
+  ARG_FLOAT(eps, a[10]);
+  const long long rd = a[11] == Py_None ? s.d : PyLong_AsLongLong(a[11]);
+  if (rd == -1 && PyErr_Occurred()) return nullptr;
+  int64_t stream;
+  Scratch ws;
+  if (!stream_of(a[12], s.device, &stream) || !scratch_for(s.device, stream, kDecode, 256, &ws)) return nullptr;
+  Tensor out = empty_like_rows(q);
+  const int rc = unlocked([&] {
+    return msgl_qk_norm_rope_store_q4(q.data_ptr(), k.data_ptr(), v.data_ptr(), wt[0], wt[1], i32(pos), i32(loc),
+                                      out.data_ptr(), kc.data_ptr(), vc.data_ptr(), static_cast<int>(nt),
+                                      static_cast<int>(hq), s.hkv, s.d, static_cast<int>(rd), base, static_cast<float>(eps),
+                                      s.num_slots, q.stride(0), k.stride(0), v.stride(0), s.dtype, ws.ptr,
+                                      reinterpret_cast<void*>(stream));
+  });
+  return rc ? raise_status(rc) : THPVariable_Wrap(std::move(out));
+}
+
+// (q, k_cache, v_cache, page_indptr, page_indices, kv_lens, sm_scale, page_size, gate, stream)
+PyObject* decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) return PyErr_Format(PyExc_TypeError, "decode_q4 takes 10 arguments");
+  ALL_TENSORS(a, 6);
+  const Tensor &q = THPVariable_Unpack(a[0]), &kc = THPVariable_Unpack(a[1]), &vc = THPVariable_Unpack(a[2]),
+               &indptr = THPVariable_Unpack(a[3]), &pages = THPVariable_Unpack(a[4]), &lens = THPVariable_Unpack(a[5]);
+  Pool4 s;
+  const void* gate;
+  if (!pool4(kc, vc, &s) || q.dim() != 3 || !q.is_contiguous() || !rows4(q, kc, s, q.size(0), q.size(1)) ||
+      !index_ok(indptr, q.device()) || !index_ok(pages, q.device()) || !index_ok(lens, q.device()) ||
+      indptr.numel() != q.size(0) + 1 || lens.numel() != q.size(0) || !gate_ptr(a[8], q, &gate))
+    Py_RETURN_NONE;
+  ARG_FLOAT(scale, a[6]);
+  ARG_INT(page_size, a[7]);
+  const int batch = static_cast<int>(q.size(0)), hq = static_cast<int>(q.size(1)), ps = static_cast<int>(page_size);
+  int64_t stream;
+  Scratch ws;
+  if (!stream_of(a[9], s.device, &stream) ||
+      !scratch_for(s.device, stream, kDecode, msgl_decode_workspace_bytes_q4(batch, hq, s.hkv, s.d, pages.numel(), ps), &ws))
+    return nullptr;
+  Tensor out = empty_like_rows(q);
+  const int rc = in_turn(ws, [&] {
+    return msgl_paged_decode_attention_q4(q.data_ptr(), kc.data_ptr(), vc.data_ptr(), i32(indptr), i32(pages), i32(lens),
+                                          gate, out.data_ptr(), ws.ptr, ws.bytes, batch, hq, s.hkv, s.d, s.num_slots, s.dtype,
+                                          static_cast<float>(scale), ps, pages.numel(), reinterpret_cast<void*>(stream));
+  });
+  return rc ? raise_status(rc) : THPVariable_Wrap(std::move(out));
+}
+
+// (q, k_cache, v_cache, qo_indptr, page_indptr, page_indices, kv_lens, prefix_lens, sm_scale, max_len_extend, page_size,
+//  is_cross_attention, sliding_window_size, gate, stream)
+PyObject* prefill_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 15) return PyErr_Format(PyExc_TypeError, "prefill_q4 takes 15 arguments");
+  ALL_TENSORS(a, 8);
+  const Tensor &q = THPVariable_Unpack(a[0]), &kc = THPVariable_Unpack(a[1]), &vc = THPVariable_Unpack(a[2]),
+               &qo = THPVariable_Unpack(a[3]), &indptr = THPVariable_Unpack(a[4]), &pages = THPVariable_Unpack(a[5]),
+               &lens = THPVariable_Unpack(a[6]), &prefix = THPVariable_Unpack(a[7]);
+  Pool4 s;
+  const void* gate;
+  if (!pool4(kc, vc, &s) || q.dim() != 3 || !q.is_contiguous() || !rows4(q, kc, s, q.size(0), q.size(1)) ||
+      !index_ok(qo, q.device()) || !index_ok(indptr, q.device()) || !index_ok(pages, q.device()) ||
+      !index_ok(lens, q.device()) || !index_ok(prefix, q.device()) || qo.numel() < 2 || indptr.numel() != qo.numel() ||
+      lens.numel() + 1 != qo.numel() || prefix.numel() + 1 != qo.numel() || !gate_ptr(a[13], q, &gate))
+    Py_RETURN_NONE;
+  ARG_FLOAT(scale, a[8]);
+  ARG_INT(max_ext, a[9]);
+  ARG_INT(page_size, a[10]);
+  ARG_INT(window, a[12]);
+  const int cross = PyObject_IsTrue(a[11]);
+  if (cross < 0) return nullptr;
+  const int batch = static_cast<int>(prefix.numel()), total_q = static_cast<int>(q.size(0)), hq = static_cast<int>(q.size(1)),
+            ps = static_cast<int>(page_size);
+  int64_t stream;
+  Scratch ws;
+  if (!stream_of(a[14], s.device, &stream) ||
+      !scratch_for(s.device, stream, kPrefill,
+                   msgl_prefill_workspace_bytes(batch, total_q, pages.numel() * page_size, hq, s.hkv, s.d,
+                                                static_cast<int>(max_ext), static_cast<int>(window)),
+                   &ws))
+    return nullptr;
+  Tensor out = empty_like_rows(q);
+  const int rc = in_turn(ws, [&] {
+    return msgl_paged_prefill_attention_q4(
+      q.data_ptr(), kc.data_ptr(), vc.data_ptr(), i32(qo), i32(indptr), i32(pages), i32(lens), i32(prefix), gate,
+      out.data_ptr(), ws.ptr, ws.bytes, batch, total_q, hq, s.hkv, s.d, s.num_slots, s.dtype, static_cast<float>(scale),
+      static_cast<int>(max_ext), cross, static_cast<int>(window), ps, pages.numel(), reinterpret_cast<void*>(stream));
+  });
+  return rc ? raise_status(rc) : THPVariable_Wrap(std::move(out));
+}
+
 // ------------------------------------------------------------------ a layer's new tokens, store and attention
 // k, v, out_loc and projection (None, or (q_weight, k_weight, positions, rope_base, eps, rotary_dim or
 // None)) of a layer call -> *rows.  1: fine, 0: not what the native call takes, -1: a Python error.
@@ -775,7 +959,8 @@ PyObject* set_maker(PyObject*, PyObject* fn) {
 PyMethodDef kMethods[] = {FAST(decode),       FAST(decode_paged),       FAST(prefill),
                           FAST(prefill_paged), FAST(store_kv),          FAST(qk_norm_rope_store),
                           FAST(decode_layer), FAST(prefill_layer),     FAST(collect_lens),
-                          FAST(index_arrays),
+                          FAST(index_arrays), FAST(store_kv_q4),        FAST(load_kv_q4),
+                          FAST(qk_norm_rope_store_q4), FAST(decode_q4), FAST(prefill_q4),
                           {"set_workspace_maker", set_maker<&g_make_workspace>, METH_O, nullptr},
                           {"set_pages_maker", set_maker<&g_make_pages>, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

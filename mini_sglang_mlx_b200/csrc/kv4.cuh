@@ -1,0 +1,290 @@
+// The K/V pool held in 4 bits: its format, and the kernels that put rows into it and read them back.
+//
+// Sixteen slots are a block.  A pool is (num_blocks, hkv) pieces of 9 * head_dim bytes, one per block and KV head: the codes of
+// its sixteen rows (head_dim / 2 bytes each), then sixteen rows of (scale, bias) pairs of the 16-bit type T, a pair for every 64
+// elements of a row.  So all that one KV head of a 16-token page takes is contiguous (1152 or 2304 bytes): one bulk copy.
+// An element is scale * code + bias with, in a group of 64,
+//
+//   bias = min,   scale = T((max - min) / 15)   (0 below 2^-100),   code = min(15, rint((x - bias) / scale)),
+//
+// so min itself is held exactly, and an element is off by half a scale, and by 15 half units in the last place of the scale.
+// Word r * (head_dim / 64) + g of a row holds elements 64 g + 8 r .. + 7: a lane that takes consecutive words gets the same
+// share of every group, which is what keeps the fragments of the attention kernels inside one group's scale.
+// Element e of a word sits in nibble e / 2 + 4 (e % 2): shifted by 4 i and masked, a word gives elements 2 i and 2 i + 1 in
+// its halves, two neighbours of a 16-bit row.
+#pragma once
+
+#include "common.cuh"
+
+namespace msgl {
+
+constexpr int kKv4Rows = 16;     // slots of a block
+constexpr int kKv4Group = 64;    // elements that share a scale and a bias
+__host__ __device__ constexpr int kv4_block_bytes(int hd) { return 9 * hd; }
+__host__ __device__ constexpr int kv4_pairs_at(int hd) { return 8 * hd; }   // byte offset of the pairs in a block
+// What is held lies within +-2^15 (so that scale * code + bias is finite in either type, whichever way the scale was rounded):
+// larger numbers and infinities are stored as that, NaN as 0, and the status word says so.
+constexpr float kKv4Max = 32768.f;
+constexpr int kKv4Reported = 4;
+
+template <typename T>
+struct Pack2;
+template <>
+struct Pack2<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+};
+template <>
+struct Pack2<__half> {
+  using V = __half2;
+};
+template <typename T>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  using V = typename Pack2<T>::V;
+  const V r = __hmax2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  using V = typename Pack2<T>::V;
+  const V r = __hmin2_nan(*reinterpret_cast<V*>(&a), *reinterpret_cast<V*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The 16-bit numbers OFF + n of nibble i of both halves of a word, and OFF.
+template <typename T>
+struct Nibble;
+template <>
+struct Nibble<__nv_bfloat16> {    // seven bits of fraction: a nibble in the lowest four counts from 128, one at bit 3 from 16
+  __host__ __device__ static constexpr float off(int i) { return i == 0 ? 128.f : 16.f; }
+  static constexpr float kSlack = 8.f;
+  __device__ __forceinline__ static uint32_t make(uint32_t w, int i) {
+    return i == 0 ? ((w & 0x000f000fu) | 0x43004300u) : (((w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u);
+  }
+};
+template <>
+struct Nibble<__half> {           // ten bits of fraction: at bit 4, 4, 2 and 6
+  __host__ __device__ static constexpr float off(int i) { return i < 2 ? 64.f : i == 2 ? 256.f : 16.f; }
+  static constexpr float kSlack = 2.f;    // (2^2 of the largest scale, 8734, is a half)
+  __device__ __forceinline__ static uint32_t make(uint32_t w, int i) {
+    return i == 0   ? (((w << 4) & 0x00f000f0u) | 0x54005400u)
+           : i == 1 ? ((w & 0x00f000f0u) | 0x54005400u)
+           : i == 2 ? (((w >> 6) & 0x003c003cu) | 0x5c005c00u)
+                    : (((w >> 6) & 0x03c003c0u) | 0x4c004c00u);
+  }
+};
+// A constant in both halves.
+template <typename T>
+__device__ __forceinline__ uint32_t both(float x) { return MmaOp<T>::pack(x, x); }
+
+// BYTES at an aligned address, four to a word.
+template <int BYTES>
+__device__ __forceinline__ void read_words(uint32_t (&r)[BYTES / 4], const unsigned char* at) {
+  if constexpr (BYTES == 8) {
+    const uint2 x = *reinterpret_cast<const uint2*>(at);
+    r[0] = x.x;
+    r[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(at)[i];
+      r[4 * i] = x.x;
+      r[4 * i + 1] = x.y;
+      r[4 * i + 2] = x.z;
+      r[4 * i + 3] = x.w;
+    }
+  }
+}
+
+// The eight elements of a word under a pair, in order: scale * code + bias, rounded once.
+__device__ __forceinline__ uint32_t fma_pair(__nv_bfloat16, uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_pair(__half, uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint4 kv4_values(uint32_t word, uint32_t pair) {
+  const uint32_t scale = __byte_perm(pair, pair, 0x1010), bias = __byte_perm(pair, pair, 0x3232);
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t n = fma_pair(T{}, Nibble<T>::make(word, i), both<T>(1.f), both<T>(-Nibble<T>::off(i)));   // exact
+    v[i] = fma_pair(T{}, n, scale, bias);
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Codes of the 2 W elements that a lane holds of a group of 64, LANES = 32 / W lanes of `mask` together, and the group's pair
+// (scale in the low half).  Element e comes back in nibble e / 2 + 4 (e % 2) of the result (W = 2: of its four lowest
+// nibbles of each half, to be shifted by 8 for the upper half of a word).
+// The quotient is that of an IEEE division (an approximate one, then its exact remainder): x - bias and scale are short
+// numbers whose quotient is often half-way between two codes, where a unit in the last place decides.
+template <typename T, int W>
+__device__ __forceinline__ uint32_t kv4_quantise(uint32_t (&x)[W], uint32_t mask, uint32_t& pair, int* status) {
+  constexpr int LANES = 32 / W;
+  float lo, hi;
+#pragma unroll 1
+  for (int again = 0;; ++again) {
+    uint32_t mx = x[0], mn = x[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      mx = max2_nan<T>(mx, x[w]);
+      mn = min2_nan<T>(mn, x[w]);
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+      mx = max2_nan<T>(mx, __shfl_xor_sync(mask, mx, o));
+      mn = min2_nan<T>(mn, __shfl_xor_sync(mask, mn, o));
+    }
+    const float2 a = unpack_pair(T{}, mx), b = unpack_pair(T{}, mn);
+    hi = fmaxf(a.x, a.y);
+    lo = fminf(b.x, b.y);
+    // (fmaxf would drop a NaN of one half)
+    if ((fabsf(a.x) <= kKv4Max && fabsf(a.y) <= kKv4Max && fabsf(b.x) <= kKv4Max &&
+         fabsf(b.y) <= kKv4Max) ||
+        again)
+      break;
+    if (status) atomicOr(status, kKv4Reported);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      float2 v = unpack_pair(T{}, x[w]);
+      v.x = v.x != v.x ? 0.f : fminf(fmaxf(v.x, -kKv4Max), kKv4Max);
+      v.y = v.y != v.y ? 0.f : fminf(fmaxf(v.y, -kKv4Max), kKv4Max);
+      x[w] = MmaOp<T>::pack(v.x, v.y);
+    }
+  }
+  const T s16 = MmaOp<T>::from_float((hi - lo) / 15.f);
+  const float scale = to_f32(s16);
+  const bool flat = !(scale >= 7.888609052210118e-31f);   // 2^-100
+  pair = MmaOp<T>::pack(flat ? 0.f : scale, lo);
+  const float inv = flat ? 0.f : __frcp_rn(scale);
+  const uint64_t lo2 = pack_f32x2(-lo, -lo), inv2 = pack_f32x2(inv, inv), scale2 = pack_f32x2(-scale, -scale);
+  uint32_t out = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float2 v = unpack_pair(T{}, x[w]);
+    const uint64_t a = add_f32x2(pack_f32x2(v.x, v.y), lo2);
+    uint64_t q = mul_f32x2(a, inv2);
+    q = fma_f32x2(fma_f32x2(q, scale2, a), inv2, q);
+    float q0, q1;
+    unpack_f32x2(q, q0, q1);
+    // (rint by the addition of 1.5 * 2^23; what is over 15 comes from a scale that was rounded down)
+    const uint32_t n0 = __float_as_uint(fminf(q0, 15.f) + 12582912.f) & 15u;
+    const uint32_t n1 = __float_as_uint(fminf(q1, 15.f) + 12582912.f) & 15u;
+    out |= (n0 | n1 << 16) << (4 * w);
+  }
+  return out;
+}
+
+// ---------------------------------------------------------------- rows into the pool
+struct Kv4StoreParams {
+  unsigned char *k_pool, *v_pool;
+  const void *k, *v;          // (n, hkv, head_dim), dense heads
+  const int32_t* slots;
+  int64_t k_stride, v_stride; // elements between tokens
+  int64_t num_slots;
+  int n, hkv;
+  int wide;                   // rows are 16-byte aligned
+  int* status;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreParams p) {
+  constexpr int CH = HD / 8, G = HD / kKv4Group;
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int32_t* slots = after_wait(p.slots);
+  const T* k = after_wait(static_cast<const T*>(p.k));
+  const T* v = after_wait(static_cast<const T*>(p.v));
+  const int lane = threadIdx.x & 31;
+  const uint32_t mask = 0xffu << (lane & 24);       // the eight lanes of a group
+  const int64_t total = static_cast<int64_t>(p.n) * p.hkv * CH;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t row = i / CH;
+    const int c = static_cast<int>(i - row * CH);   // elements 8 c .. 8 c + 7
+    const int t = static_cast<int>(row / p.hkv), h = static_cast<int>(row - static_cast<int64_t>(t) * p.hkv);
+    const int slot = slots[t];
+    if (slot < 0 || slot >= p.num_slots) {
+      if (p.status) atomicOr(p.status, 2);
+      continue;
+    }
+    const T* ks = k + t * p.k_stride + h * HD + c * 8;
+    const T* vs = v + t * p.v_stride + h * HD + c * 8;
+    uint32_t x[2][4];
+    if (p.wide) {
+      *reinterpret_cast<uint4*>(x[0]) = *reinterpret_cast<const uint4*>(ks);
+      *reinterpret_cast<uint4*>(x[1]) = *reinterpret_cast<const uint4*>(vs);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        reinterpret_cast<uint2*>(x[0])[j] = reinterpret_cast<const uint2*>(ks)[j];
+        reinterpret_cast<uint2*>(x[1])[j] = reinterpret_cast<const uint2*>(vs)[j];
+      }
+    }
+    const int64_t block = (static_cast<int64_t>(slot / kKv4Rows) * p.hkv + h) * kv4_block_bytes(HD);
+    const int r = slot % kKv4Rows, g = c / 8;
+    const int64_t code_at = block + r * (HD / 2) + ((c % 8) * G + g) * 4;
+    const int64_t pair_at = block + kv4_pairs_at(HD) + (r * G + g) * 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unsigned char* pool = j == 0 ? p.k_pool : p.v_pool;
+      uint32_t pair;
+      const uint32_t word = kv4_quantise<T, 4>(x[j], mask, pair, p.status);
+      *reinterpret_cast<uint32_t*>(pool + code_at) = word;
+      if (c % 8 == 0) *reinterpret_cast<uint32_t*>(pool + pair_at) = pair;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- rows out of the pool
+struct Kv4LoadParams {
+  const unsigned char *k_pool, *v_pool;
+  void *k, *v;                // (n, hkv, head_dim), contiguous
+  const int32_t* slots;
+  int64_t num_slots;
+  int n, hkv;
+  int* status;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
+  constexpr int CH = HD / 8, G = HD / kKv4Group;
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int32_t* slots = after_wait(p.slots);
+  const unsigned char* pools[2] = {after_wait(p.k_pool), after_wait(p.v_pool)};
+  const int64_t total = static_cast<int64_t>(p.n) * p.hkv * CH;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t row = i / CH;
+    const int c = static_cast<int>(i - row * CH);
+    const int t = static_cast<int>(row / p.hkv), h = static_cast<int>(row - static_cast<int64_t>(t) * p.hkv);
+    const int slot = slots[t];
+    const bool ok = slot >= 0 && slot < p.num_slots;
+    if (!ok && p.status) atomicOr(p.status, 2);
+    const int64_t block = (static_cast<int64_t>(ok ? slot / kKv4Rows : 0) * p.hkv + h) * kv4_block_bytes(HD);
+    const int r = slot % kKv4Rows, g = c / 8;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t word = 0, pair = 0;
+      if (ok) {
+        word = *reinterpret_cast<const uint32_t*>(pools[j] + block + r * (HD / 2) + ((c % 8) * G + g) * 4);
+        pair = *reinterpret_cast<const uint32_t*>(pools[j] + block + kv4_pairs_at(HD) + (r * G + g) * 4);
+      }
+      const float2 sb = unpack_pair(T{}, pair);
+      uint4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t n = word >> (4 * e);
+        reinterpret_cast<uint32_t*>(&o)[e] = MmaOp<T>::pack(fmaf(static_cast<float>(n & 15u), sb.x, sb.y),
+                                                            fmaf(static_cast<float>(n >> 16 & 15u), sb.x, sb.y));
+      }
+      reinterpret_cast<uint4*>(j == 0 ? p.k : p.v)[i] = o;
+    }
+  }
+}
+
+}  // namespace msgl

@@ -57,6 +57,7 @@
 
 #include <type_traits>
 
+#include "kv4.cuh"
 #include "prefill_tiles.cuh"
 
 namespace msgl {
@@ -464,7 +465,10 @@ __device__ __noinline__ void merge_kv_splits_cta(const MergeArgs p, int nsp, int
   }
 }
 
-template <typename T, int BN, int NSUB, int HD = 128, bool PAGED = false>
+// KV4: the pool is held in 4 bits (kv4.cuh) and addressed by pages; the copying warps read codes, scales and biases and write
+// the tiles' elements, each scale * code + bias rounded once to T (one fma of two elements; a 16-bit pool holds the same
+// rounding).  Everything behind the tiles is as it is.
+template <typename T, int BN, int NSUB, int HD = 128, bool PAGED = false, bool KV4 = false>
 __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
                                   TcShape<NSUB, HD, PAGED>::kMinCtasForRegs)
     prefill_tc_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap tm_k,
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   const int qt = it.qt, split = it.split;
   const int slot_item = it.base + qt * sq.nsplit + split;   // where this item's kv-split partial goes
   auto over_group = [&](int x) { return NSUB == 2 ? x / G : divide_by(x, p.group_recip); };
-  if (PAGED && it.first && tid == 0 && p.status) {
+  if ((PAGED || KV4) && it.first && tid == 0 && p.status) {
     // a length that is negative or exceeds the sequence's pages was clamped: report it
     const int64_t cap = static_cast<int64_t>(p.page_indptr[it.b + 1] - p.page_indptr[it.b]) * p.page_size;
     const int len = p.kv_lens[it.b];
@@ -797,6 +801,50 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
             }
           }
         }
+      }
+    } else if constexpr (KV4) {
+      constexpr int PPR = HD / 32;                     // 16-byte pieces (four words) of a row's codes
+      constexpr int G = HD / kKv4Group;
+      const int32_t* __restrict__ pages = p.page_indices + sq.kv_begin;
+      const int64_t num_blocks = p.num_slots / kKv4Rows;
+      const int page_blocks = p.page_size / kKv4Rows;
+      load_q();
+      auto produce = [&](int seq, const unsigned char* pool, int tile) {
+        const int bf = seq % kTcBufs;
+        alive = mbar_wait_warp(bar_empty(bf), ((seq / kTcBufs) & 1) ^ 1, abort_flag);
+        if (!alive) return;
+        unsigned char* dst = smem_raw + (ring - smem_u32(smem_raw)) + bf * kTcKvTileBytes;
+        for (int e = ptid; e < BN * PPR; e += NPROD) {
+          const int row = e / PPR, piece = e % PPR;
+          const int t = kv_lo + tile * BN + row;
+          uint32_t words[4] = {0u, 0u, 0u, 0u}, pairs[G];
+#pragma unroll
+          for (int g = 0; g < G; ++g) pairs[g] = 0u;
+          if (t < kv_hi_load) {
+            const int page = divide_by(t, p.page_recip);
+            const int64_t block = static_cast<int64_t>(__ldg(pages + page)) * page_blocks + (t - page * p.page_size) / kKv4Rows;
+            if (block >= 0 && block < num_blocks) {
+              const unsigned char* at = pool + (block * p.hkv + h) * kv4_block_bytes(HD);
+              read_words<16>(words, at + (t % kKv4Rows) * (HD / 2) + piece * 16);
+              read_words<G * 4>(pairs, at + kv4_pairs_at(HD) + (t % kKv4Rows) * (G * 4));
+            } else if (p.status) {
+              atomicOr(p.status, 2);
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int g = w % G, r8 = piece * (4 / G) + w / G;
+            *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(row, g * 8 + r8)) = kv4_values<T>(words[w], pairs[g]);
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar_full(bf));
+      };
+      for (int t = 0; t < LA && t < ntiles && alive; ++t) produce(ring_seq_k<LA>(t), kbase, t);
+#pragma unroll 1
+      for (int j = 0; j < ntiles && alive; ++j) {
+        produce(ring_seq_v<LA>(j), vbase, j);
+        if (alive && j + LA < ntiles) produce(ring_seq_k<LA>(j + LA), kbase, j + LA);
       }
     } else {
       constexpr int RPT = (BN + PROWS - 1) / PROWS;  // passes over a tile

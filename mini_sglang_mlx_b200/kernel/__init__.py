@@ -28,6 +28,12 @@ __all__ = [
     "qk_norm_rope_store",
     "build_attn_metadata",
     "device_status",
+    "kv_cache_q4_shape",
+    "store_kv_cache_q4",
+    "load_kv_cache_q4",
+    "qk_norm_rope_store_q4",
+    "paged_decode_attention_q4",
+    "paged_prefill_attention_q4",
 ]
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
@@ -412,6 +418,150 @@ def qk_norm_rope_store(q, k, v, q_weight, k_weight, positions, out_loc, k_cache,
              f"{op}: tensors must live on the same CUDA device")
     _again(op, _ops.qk_norm_rope_store, q.device, *args)
     return q
+
+
+# ---- a K/V pool held in 4 bits: no operator of the reference has one
+
+KV4_ROWS = 16     # slots of a block
+KV4_GROUP = 64    # elements that share a scale and a bias
+
+
+def kv_cache_q4_shape(num_slots: int, num_kv_heads: int, head_dim: int) -> Tuple[int, int, int]:
+    """Shape of a K or V pool of ``num_slots`` tokens held in 4 bits, in elements of the 16-bit data type:
+    ``(ceil(num_slots / 16), num_kv_heads, 9 * head_dim / 2)``.  Per block of sixteen slots and per head the codes of
+    sixteen rows (``head_dim / 2`` bytes each), then sixteen rows of (scale, bias) pairs, one for every 64 elements:
+    4.5 bits an element.  An element is ``scale * code + bias`` with, in its group of 64, ``bias`` = min, ``scale`` = (max - min) /
+    15 in the data type and ``code`` = min(15, rint((x - bias) / scale)).  A pool of zeros reads as zeros."""
+    _require(head_dim in (128, 256), "kv_cache_q4_shape: head_dim must be 128 or 256")
+    _require(num_slots >= 0 and num_kv_heads > 0, "kv_cache_q4_shape: negative num_slots or no num_kv_heads")
+    return (-(-int(num_slots) // KV4_ROWS), int(num_kv_heads), 9 * int(head_dim) // 2)
+
+
+def _check_pool_q4(op: str, k_cache, v_cache) -> Tuple[int, int]:
+    """(num_kv_heads, head_dim) of a pair of 4-bit pools."""
+    _require(k_cache.dim() == 3 and k_cache.shape[2] > 0 and k_cache.shape[2] % 9 == 0,
+             f"{op}: k_cache and v_cache must be (num_blocks, num_kv_heads, 9 * head_dim / 2)")
+    _require(k_cache.dtype in _DTYPES, f"{op}: unsupported dtype, must be float16 or bfloat16")
+    _require(v_cache.dtype == k_cache.dtype and v_cache.shape == k_cache.shape,
+             f"{op}: v_cache must match k_cache in shape and dtype")
+    _require(k_cache.is_contiguous() and v_cache.is_contiguous(), f"{op}: k_cache and v_cache must be contiguous")
+    _require(k_cache.is_cuda, f"{op}: tensors must live on a CUDA device")
+    _require(v_cache.device == k_cache.device, f"{op}: all tensors must be on the same device")
+    return k_cache.shape[1], k_cache.shape[2] // 9 * 2
+
+
+def _check_rows_q4(op: str, name: str, rows, k_cache, n: int, heads: int, d: int) -> None:
+    _require(rows.dim() == 3 and tuple(rows.shape) == (n, heads, d), f"{op}: {name} must be ({n}, {heads}, {d})")
+    _require(rows.dtype == k_cache.dtype, f"{op}: {name} must have the pools' dtype")
+    _require(rows.device == k_cache.device, f"{op}: all tensors must be on the same device")
+    _require(rows.stride(2) == 1 and rows.stride(1) == d, f"{op}: rows must be dense")
+
+
+def _check_ints_q4(op: str, device, **arrays) -> None:
+    for name, (t, n) in arrays.items():
+        _require(t.dim() == 1 and t.dtype == torch.int32 and t.is_contiguous(), f"{op}: {name} must be 1D, int32 and contiguous")
+        _require(n is None or t.numel() == n, f"{op}: {name} must have {n} entries")
+        _require(t.device == device, f"{op}: all tensors must be on the same device")
+
+
+def store_kv_cache_q4(k_cache, v_cache, indices, k, v, *, stream=None) -> None:
+    """``store_kv_cache`` into 4-bit pools (``kv_cache_q4_shape``): rows ``k[r]``, ``v[r]`` are quantised into slot
+    ``indices[r]``.  k and v ``(length, num_kv_heads, head_dim)`` of the pools' dtype, dense heads, any token stride.
+
+    A row whose index lies outside the pool is dropped and reported by ``device_status`` (2); the indices of a call
+    are distinct.  Magnitudes above 2**15 and infinities are stored as 2**15, NaN as 0, both reported (4)."""
+    args = (k_cache, v_cache, indices, k, v, None if stream is None else _handle(stream))
+    if _ops.store_kv_q4(*args) is not None:
+        return
+    op = "store_kv_cache_q4"
+    hkv, d = _check_pool_q4(op, k_cache, v_cache)
+    _check_ints_q4(op, k_cache.device, indices=(indices, None))
+    for name, t in (("k", k), ("v", v)):
+        _check_rows_q4(op, name, t, k_cache, indices.numel(), hkv, d)
+    _again(op, _ops.store_kv_q4, k_cache.device, *args)
+
+
+def load_kv_cache_q4(k_cache, v_cache, indices, *, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rows at ``indices`` of 4-bit pools as ``(len(indices), num_kv_heads, head_dim)`` of their dtype, keys and values:
+    ``scale * code + bias``, rounded once.  An index outside the pool gives zeros and is reported by ``device_status`` (2)."""
+    args = (k_cache, v_cache, indices, None if stream is None else _handle(stream))
+    out = _ops.load_kv_q4(*args)
+    if out is not None:
+        return out
+    op = "load_kv_cache_q4"
+    _check_pool_q4(op, k_cache, v_cache)
+    _check_ints_q4(op, k_cache.device, indices=(indices, None))
+    return _again(op, _ops.load_kv_q4, k_cache.device, *args)
+
+
+def qk_norm_rope_store_q4(q, k, v, q_weight, k_weight, positions, out_loc, k_cache, v_cache, *, rope_base: float,
+                          eps: float = 1e-6, rotary_dim: Optional[int] = None, stream=None) -> torch.Tensor:
+    """``qk_norm_rope_store`` for 4-bit pools: per-head RMSNorm of q and k, rotary embedding of both, and the new rows
+    quantised into slots ``out_loc`` (the rotated keys are rounded to the data type first, as a 16-bit pool would hold
+    them).  q is read, and what it becomes is returned as a new contiguous tensor.  q, k and v may be views into one fused projection
+    output.  Positions below 2**24.  What ``store_kv_cache_q4`` says of indices and of numbers that are not finite holds here too."""
+    args = (q, k, v, q_weight, k_weight, positions, out_loc, k_cache, v_cache, rope_base, eps, rotary_dim,
+            None if stream is None else _handle(stream))
+    out = _ops.qk_norm_rope_store_q4(*args)
+    if out is not None:
+        return out
+    op = "qk_norm_rope_store_q4"
+    hkv, d = _check_pool_q4(op, k_cache, v_cache)
+    _require(q.dim() == 3, f"{op}: q must be (n_tokens, num_q_heads, head_dim)")
+    n, hq = q.shape[:2]
+    for name, t, heads in (("q", q, hq), ("k", k, hkv), ("v", v, hkv)):
+        _check_rows_q4(op, name, t, k_cache, n, heads, d)
+    for wt in (q_weight, k_weight):
+        _require(wt is None or (wt.dtype == q.dtype and tuple(wt.shape) == (d,) and wt.is_contiguous()
+                                and wt.device == q.device),
+                 f"{op}: a norm weight must be (head_dim,) in the data dtype")
+    _check_ints_q4(op, q.device, positions=(positions, n), out_loc=(out_loc, n))
+    return _again(op, _ops.qk_norm_rope_store_q4, q.device, *args)
+
+
+def _check_attention_q4(op: str, q, k_cache, v_cache, gate) -> None:
+    _, d = _check_pool_q4(op, k_cache, v_cache)
+    _require(q.dim() == 3, f"{op}: q must be 3D (rows, num_q_heads, head_dim)")
+    _check_rows_q4(op, "q", q, k_cache, q.shape[0], q.shape[1], d)
+    _require(q.is_contiguous(), f"{op}: q must be contiguous")
+    if gate is not None:
+        _check_gate(op, gate, q)
+
+
+def paged_decode_attention_q4(q, k_cache, v_cache, page_indptr, page_indices, kv_lens, sm_scale: float, *,
+                              page_size: int = 16, gate=None, stream=None) -> torch.Tensor:
+    """``paged_decode_attention_p16`` over 4-bit pools.  ``page_size``: a multiple of 16 (slot = page * page_size +
+    offset).  Without the split hints of that operator, which it does not read either: the batch is cut into equal shares."""
+    args = (q, k_cache, v_cache, page_indptr, page_indices, kv_lens, sm_scale, page_size, gate,
+            None if stream is None else _handle(stream))
+    out = _ops.decode_q4(*args)
+    if out is not None:
+        return out
+    op = "paged_decode_attention_q4"
+    _check_attention_q4(op, q, k_cache, v_cache, gate)
+    _check_ints_q4(op, q.device, page_indptr=(page_indptr, q.shape[0] + 1), page_indices=(page_indices, None),
+                   kv_lens=(kv_lens, q.shape[0]))
+    return _again(op, _ops.decode_q4, q.device, *args)
+
+
+def paged_prefill_attention_q4(q, k_cache, v_cache, qo_indptr, page_indptr, page_indices, kv_lens, prefix_lens,
+                               sm_scale: float, max_len_extend: int, *, page_size: int = 16,
+                               is_cross_attention: bool = False, sliding_window_size: int = 0, gate=None,
+                               stream=None) -> torch.Tensor:
+    """``paged_prefill_attention_p16`` over 4-bit pools: ragged query blocks over prefix and new tokens, causal,
+    bidirectional or under a sliding window; rows without a visible key give zeros.  ``page_size``: a multiple of 16."""
+    args = (q, k_cache, v_cache, qo_indptr, page_indptr, page_indices, kv_lens, prefix_lens, sm_scale, max_len_extend,
+            page_size, is_cross_attention, sliding_window_size, gate, None if stream is None else _handle(stream))
+    out = _ops.prefill_q4(*args)
+    if out is not None:
+        return out
+    op = "paged_prefill_attention_q4"
+    _check_attention_q4(op, q, k_cache, v_cache, gate)
+    batch = prefix_lens.numel()
+    _require(batch > 0, f"{op}: batch must be > 0")
+    _check_ints_q4(op, q.device, qo_indptr=(qo_indptr, batch + 1), page_indptr=(page_indptr, batch + 1),
+                   page_indices=(page_indices, None), kv_lens=(kv_lens, batch), prefix_lens=(prefix_lens, batch))
+    return _again(op, _ops.prefill_q4, q.device, *args)
 
 
 def gather_kv_indices(page_table, table_idx, kv_indptr, total_kv: int, *, stream=None):
