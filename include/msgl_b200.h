@@ -541,8 +541,10 @@ int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const voi
 
 /*
  * msgl_paged_prefill_attention_p16 over this pool: masks, arguments and zeros of rows without a key as there.
- * Scratch: msgl_prefill_workspace_bytes with total_kv = total_pages * page_size.
+ * max_len_extend is the longest query block, or more (rows of a longer one may stay unwritten, and 2 is reported).
  */
+size_t msgl_prefill_workspace_bytes_q4(int batch, int total_q, int64_t total_pages, int page_size, int num_q_heads,
+                                       int num_kv_heads, int head_dim, int max_len_extend, int sliding_window_size);
 int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const void* v_cache,
                                     const int32_t* qo_indptr, const int32_t* page_indptr,
                                     const int32_t* page_indices, const int32_t* kv_lens, const int32_t* prefix_lens,

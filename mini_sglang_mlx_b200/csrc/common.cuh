@@ -122,6 +122,11 @@ __device__ __forceinline__ float fast_sqrt(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Packed two-float arithmetic (one instruction for two lanes of a register pair).
 __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
@@ -321,6 +326,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tma
       : "memory");
 }
 // Untiled bulk copies (16-byte aligned addresses, sizes a multiple of 16 bytes).
+// global -> shared, its bytes counted on `bar` as they land:
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
 // shared -> global, tracked by the thread's bulk async-group:
 __device__ __forceinline__ void bulk_store(void* gdst, uint32_t ssrc, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(ssrc),

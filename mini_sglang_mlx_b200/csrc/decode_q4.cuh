@@ -1,5 +1,9 @@
 // Paged attention for few query rows per sequence over the 4-bit pool (kv4.cuh): flash decoding over equal shares of a batch.
 //
+// Columns.  What shares a KV head of a sequence are its columns: the group of query heads of one token (decode), or of each of a
+// few new tokens (BLOCKS: a verify or draft block, under the masks of the prefill op).  A CTA takes 8 NT of them; with more
+// there are several CTAs for a share, side by side, and the second one's blocks come out of L2.
+//
 // Work split.  For every KV head the sequences' 16-token blocks are laid end to end and cut into equal shares; a CTA owns one
 // share of one head.  The part of a sequence that a share holds is a segment; a segment that is a whole sequence writes final
 // rows, any other an fp32 partial (weighted sum, maximum, sum of the weights), and the CTA that arrives last at the
@@ -8,19 +12,20 @@
 // A block of a head (codes, scales and biases of K: 9 head_dim bytes, and of V) comes with two bulk copies into a ring of the
 // warp's own; the warps of a CTA take the blocks of a segment in turn.
 //
-// Arithmetic.  The codes go to the tensor cores as they are: a nibble put under the right exponent is the 16-bit
-// number OFF + n, exactly, in one and-or, and what OFF adds is taken off in fp32:
-//   S = K q^T:    m16n8k16 with 16 tokens as rows and 8 query heads as columns.  k steps stay inside a group of 64 elements, so
-//                 s = sum_g scale_g (sum_d (OFF + n) q - sum_d OFF q) + bias_g sum_d q, with the middle term (per head and group,
-//                 from a product with OFF itself) as the accumulator's start.
+// Arithmetic.  The codes go to the tensor cores as they are, because small integers are f16 numbers already: the pattern n 2^k, inside
+// the fraction, is n 2^(k-24).  A word masked, shifted by eight and masked, gives its elements two by two.
+//   S = K q^T:    m16n8k16 with 16 tokens as rows and 8 columns.  k steps stay inside a group of 64 elements, so
+//                 s = sum_g scale_g (sum_d n q) + bias_g sum_d q, in fp32.  q is an f16 number times a power of two of its row
+//                 (exactly, but for what is below 2^-24 of the row's largest).
 //   O^T = V^T P^T: rows are head_dim, the 16 tokens the k dimension.  A group's scale belongs to the token, so it is multiplied
-//                 into the weight: P_g = T(p scale_g).  OFF sum(P_g) is taken off at the end (the sum by a product with ones),
-//                 and sum(p bias_g) is kept in fp32.  T(p scale) is the one rounding in front of the output's: a relative half
-//                 unit of T per weight, as a 16-bit pool's kernel rounds p.  It counts by the code, so codes are taken from their
-//                 middle: with v = scale (n - 8) + (bias + 8 scale) its effect is 2.5 times less than with v = scale n + bias.
-// (Heads as rows and tokens as columns, the usual way round, leaves half of each product's rows empty at eight heads; to
-// scale the codes to 16-bit values first takes twice the integer instructions and rounds every element.)
-// The weights' reference maximum moves only when a score passes it by more than 2^kSlack, so that the rows' maxima need not
+//                 into the weight: P_g = f16(p scale_g 2^-e), 2^e a power of two over all scales so far;
+//                 sum(p bias_g) is kept in fp32.  That rounding of P_g, half a unit of f16, is the only one in front of the
+//                 output's.
+// (Columns as rows and tokens as columns, the usual way round, leaves half of each product's rows empty at eight columns; to
+// scale the codes to 16-bit values first takes twice the integer instructions, and rounds every element.  The byte n is the e4m3 number
+// n 2^-9 and would take half the masks, but a product of e4m3 with an fp32 sum is made of two of f16, conversions and additions
+// here: 171 us for 32 requests of 4096 to 32768 tokens.)
+// The weights' reference maximum moves only when a score passes it by more than 2^8, so that the rows' maxima need not
 // be reduced in every step.
 #pragma once
 
@@ -32,18 +37,21 @@ struct Q4DecodeParams {
   const void* q;              // (rows, hq, D)
   const unsigned char *k_pool, *v_pool;
   const int32_t *page_indptr, *page_indices, *kv_lens;
+  const int32_t *qo_indptr, *prefix_lens;   // BLOCKS
   int page_blocks;            // blocks of 16 tokens per page
   int total_pages;            // entries of page_indices
   void* out;
   const void* gate;           // like q, or null
-  // (2 shares, hkv, group, D + 4) partials: weighted sums, maximum, sum of the weights.  Row 2 s of share s is the end or a
-  // middle part of a sequence that began in front of it, row 2 s + 1 the first part of one that goes on behind it.
+  // (2 shares, hkv, column tiles, 8 NT, D + 4) partials: weighted sums, maximum, sum of the weights.  Row 2 s of share s is the
+  // end or a middle part of a sequence that began in front of it, row 2 s + 1 the first part of one that goes on behind it.
   float* part;
-  int* tickets;               // (batch, hkv) arrival counters, zero before and after
+  int* tickets;               // (batch, hkv, column tiles) arrival counters, zero before and after
   int* status;
   int batch, hq, hkv, group;
+  int col_tiles;              // CTAs side by side
   int num_shares;             // per head
   int min_share, pad;         // blocks a share holds at least; blocks that the end of a segment counts for
+  int is_cross, window;       // BLOCKS
   int64_t num_blocks;
   float scale_log2;
 };
@@ -59,29 +67,50 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(bar)
-               : "memory");
-}
-template <typename T, int HD, int NT, int WARPS, int STAGES, int MINB>
+// U blocks a step and stage: with two, the next block's loads and products fill the first one's waits.
+template <typename T, int HD, int NT, bool BLOCKS, int U, int WARPS, int STAGES, int MINB>
 __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4DecodeParams p) {
   constexpr int G = HD / kKv4Group;          // groups of a row
   constexpr int BLK = kv4_block_bytes(HD);
   constexpr int ROW = HD / 2;                // code bytes of a row
   constexpr int PAIRS = kv4_pairs_at(HD);
   constexpr int MROW = q4_merge_row(HD), PROW = q4_partial_floats(HD);
-  using N = Nibble<T>;
+  constexpr int COLS = 8 * NT;
+  constexpr int WORDS = 2 * G;               // words of a K row per lane
+  constexpr float kSlack = 8.f;
+  constexpr float kNoScore = -1.5e38f;       // reference maximum of a column without a key (its sums are zero)
+  constexpr int kLeastExponent = -80;        // of the scales, as the reference counts it (sums stay below 2^128 then)
+  using Mma = MmaOp<__half>;
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ uint64_t s_bar[WARPS * STAGES];
   __shared__ int s_last;
+  struct Keys {
+    int page0, len;      // its first page, its tokens (clamped to what the pages hold)
+    int first, blocks;   // blocks with a key that some of its columns see
+    int tok0, new_tok;   // BLOCKS: first query token and how many
+    int prefix;
+  };
+  struct Segment {
+    Keys k;
+    int beg;             // position of the whole sequence
+    int lo, ng;          // first of its blocks in the share, and how many
+    int cols;            // columns of this CTA
+  };
+  // (what a warp needs now and then does not sit in its registers)
+  struct Ahead {
+    Segment s;
+    int b, step, more;
+  };
+  __shared__ Ahead s_ahead[WARPS];
+  __shared__ Segment s_current[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, c = lane & 3;
   const int h = static_cast<int>(blockIdx.x) % p.hkv;
-  const int share_id = static_cast<int>(blockIdx.x) / p.hkv;
-  unsigned char* const ring = smem_raw + warp * (STAGES * 2 * BLK);
-  float* const sm_o = reinterpret_cast<float*>(smem_raw + WARPS * STAGES * 2 * BLK);   // [WARPS][4][MROW]
+  const int ct = BLOCKS || COLS < 16 ? static_cast<int>(blockIdx.x) / p.hkv % p.col_tiles : 0;
+  const int share_id = static_cast<int>(blockIdx.x) / p.hkv / p.col_tiles;
+  unsigned char* const ring = smem_raw + warp * (STAGES * U * 2 * BLK);
+  float* const sm_o = reinterpret_cast<float*>(smem_raw + WARPS * STAGES * U * 2 * BLK);   // [WARPS][4][MROW]
   float* const sm_ml = sm_o + WARPS * 4 * MROW;                                       // [WARPS][4][2]
   if (lane < STAGES) mbar_init(smem_u32(&s_bar[warp * STAGES + lane]), 1);
   fence_mbar_init();
@@ -96,19 +125,32 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
   const unsigned char* const vp = after_wait(p.v_pool);
 
   // ---- positions: a sequence takes its blocks and `pad` more; this CTA has [r0, r1)
-  auto length = [&](int b, int& page0) -> int {      // tokens, clamped to what the sequence's pages hold
-    page0 = min(max(__ldg(indptr + b), 0), p.total_pages);
+  auto keys = [&](int b) -> Keys {
+    Keys k{};
+    k.page0 = min(max(__ldg(indptr + b), 0), p.total_pages);
     const int last = min(__ldg(indptr + b + 1), p.total_pages);
-    const int64_t cap = static_cast<int64_t>(max(last - page0, 0)) * p.page_blocks * kKv4Rows;
-    return static_cast<int>(min(static_cast<int64_t>(max(__ldg(lens + b), 0)), cap));
+    const int64_t cap = static_cast<int64_t>(max(last - k.page0, 0)) * p.page_blocks * kKv4Rows;
+    k.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(lens + b), 0)), cap));
+    k.first = 0;
+    if constexpr (BLOCKS) {
+      k.tok0 = __ldg(p.qo_indptr + b);
+      k.new_tok = max(__ldg(p.qo_indptr + b + 1) - k.tok0, 0);
+      k.prefix = __ldg(p.prefix_lens + b);
+      const int hi = p.is_cross ? k.len : static_cast<int>(min(static_cast<int64_t>(k.len), static_cast<int64_t>(k.prefix) + k.new_tok));
+      const int lo = p.window > 0 ? max(0, k.prefix - p.window + 1) : 0;
+      k.first = lo / kKv4Rows;
+      k.blocks = hi > lo && k.new_tok > 0 ? (hi + kKv4Rows - 1) / kKv4Rows - k.first : 0;
+    } else {
+      k.blocks = (k.len + kKv4Rows - 1) / kKv4Rows;
+    }
+    return k;
   };
-  auto room = [&](int len) -> int { return len == 0 ? 0 : (len + kKv4Rows - 1) / kKv4Rows + p.pad; };
+  auto room = [&](int blocks) -> int { return blocks == 0 ? 0 : blocks + p.pad; };
   const int run = (p.batch + 31) / 32;
   int sum = 0;
   for (int j = 0; j < run; ++j) {
     const int b = lane * run + j;
-    int page0;
-    if (b < p.batch) sum += room(length(b, page0));
+    if (b < p.batch) sum += room(keys(b).blocks);
   }
   int incl = sum;
 #pragma unroll
@@ -132,9 +174,8 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
       int pos = incl - sum;
       for (int j = 0; j < run; ++j) {
         const int b = l * run + j;
-        int page0;
         if (b >= p.batch) break;
-        const int n = room(length(b, page0));
+        const int n = room(keys(b).blocks);
         if (pos >= r0 || pos + n > r0) {
           found = b;
           at = pos;
@@ -147,75 +188,86 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
     beg0 = __shfl_sync(0xffffffffu, at, l);
   }
 
-  struct Segment {
-    int beg, ng_all;     // position and blocks of the whole sequence
-    int lo, ng;          // first of its blocks in the share, and how many
-    int page0, len;
-  };
   auto segment = [&](int b, int beg, Segment& s) -> bool {
     if (b >= p.batch || (beg >= r1 && !tail)) return false;
     s.beg = beg;
-    s.len = length(b, s.page0);
-    s.ng_all = (s.len + kKv4Rows - 1) / kKv4Rows;
-    const int lo = max(beg, r0), hi = min(beg + s.ng_all, r1);
+    s.k = keys(b);
+    const int lo = max(beg, r0), hi = min(beg + s.k.blocks, r1);
     s.lo = lo - beg;
-    s.ng = max(hi - lo, 0);
+    s.cols = min((BLOCKS ? s.k.new_tok : 1) * p.group - ct * COLS, COLS);
+    s.ng = s.cols > 0 ? max(hi - lo, 0) : 0;
     return true;
   };
-  auto behind = [&](const Segment& s) -> int { return s.beg + (s.ng_all == 0 ? 0 : s.ng_all + p.pad); };
+  auto behind = [&](const Segment& s) -> int { return s.beg + room(s.k.blocks); };
 
-  // ---- copies, ahead of the arithmetic: this warp's blocks of the share in order, 32 page ids at a time in the lanes
-  Segment ps;
-  int pb = b0, pg = warp;
-  bool more = segment(pb, beg0, ps);
-  int have = 0, at = 0;            // ids of this batch, next one
-  int my_block = -1;
-  uint32_t bad = 0;                // stages whose page is not in the pool
-  auto issue = [&](int stage) {
-    while (at == have) {
-      if (!more) return;
-      if (pg >= ps.ng) {
-        pg -= ps.ng;
-        more = segment(++pb, behind(ps), ps);
-        continue;
+  // ---- copies, ahead of the arithmetic: this warp's steps of the share in order.  The lanes hold the blocks of the next
+  // 32 / U steps, U lanes a step: -1 a page that is not in the pool, -2 none.
+  constexpr int BATCH = 32 / U;
+  constexpr uint32_t ALL = (1u << U) - 1;
+  if (lane == 0) {
+    Ahead a;
+    a.b = b0;
+    a.step = warp;
+    a.more = segment(b0, beg0, a.s);
+    s_ahead[warp] = a;
+  }
+  __syncwarp();
+  int have = 0, at = 0;            // steps of this batch, next one
+  int my_block = -2;
+  uint32_t bad = 0;                // blocks in the ring whose page is not in the pool
+  auto refill = [&]() {
+    Ahead a = s_ahead[warp];
+    while (true) {
+      if (!a.more) break;
+      const int steps = (a.s.ng + U - 1) / U;
+      if (a.step < steps) {
+        have = min(BATCH, (steps - a.step + WARPS - 1) / WARPS);
+        break;
       }
-      have = min(32, (ps.ng - pg + WARPS - 1) / WARPS);
+      a.step -= steps;
+      a.more = segment(++a.b, behind(a.s), a.s);
+    }
+    my_block = -2;
+    if (a.more) {
       at = 0;
-      my_block = -1;
-      if (lane < have) {
-        const int g = ps.lo + pg + lane * WARPS;
+      const int i = (a.step + lane / U * WARPS) * U + lane % U;
+      if (lane / U < have && i < a.s.ng) {
+        const int g = a.s.k.first + a.s.lo + i;
         const int page = p.page_blocks == 1 ? g : g / p.page_blocks;
-        const int64_t block = static_cast<int64_t>(__ldg(pages + ps.page0 + page)) * p.page_blocks + (g - page * p.page_blocks);
-        if (block >= 0 && block < p.num_blocks) my_block = static_cast<int>(block);
-        else if (p.status) atomicOr(p.status, 2);
+        const int64_t block = static_cast<int64_t>(__ldg(pages + a.s.k.page0 + page)) * p.page_blocks + (g - page * p.page_blocks);
+        my_block = block >= 0 && block < p.num_blocks ? static_cast<int>(block) : -1;
+        if (my_block < 0 && p.status) atomicOr(p.status, 2);
       }
-      pg += have * WARPS;
+      a.step += have * WARPS;
     }
-    const int block = __shfl_sync(0xffffffffu, my_block, at++);
-    bad = block < 0 ? bad | 1u << stage : bad & ~(1u << stage);
-    if (lane == 0) {
-      const uint32_t bar = smem_u32(&s_bar[warp * STAGES + stage]);
-      if (block >= 0) {
-        const int64_t off = (static_cast<int64_t>(block) * p.hkv + h) * BLK;
-        const uint32_t dst = smem_u32(ring + stage * (2 * BLK));
-        mbar_arrive_expect_tx(bar, 2 * BLK);
-        bulk_load(dst, kp + off, BLK, bar);
-        bulk_load(dst + BLK, vp + off, BLK, bar);
-      } else {
-        mbar_arrive(bar);
-      }
+    __syncwarp();
+    if (lane == 0) s_ahead[warp] = a;
+    __syncwarp();
+    return a.more != 0;
+  };
+  const int64_t block_bytes = static_cast<int64_t>(p.hkv) * BLK, head_at = static_cast<int64_t>(h) * BLK;
+  auto issue = [&](int stage) {    // this warp's next step into a stage, if it has one
+    if (at == have && !refill()) return;
+    const int block = __shfl_sync(0xffffffffu, my_block, at * U + lane % U);
+    ++at;
+    const uint32_t in = __ballot_sync(0xffffffffu, block >= 0) & ALL;
+    const uint32_t bar = smem_u32(&s_bar[warp * STAGES + stage]);
+    if (bad != 0 || in != ALL) {
+      const uint32_t out = __ballot_sync(0xffffffffu, block == -1) & ALL;
+      bad = (bad & ~(ALL << (stage * U))) | out << (stage * U);
+    }
+    if (lane == 0) mbar_arrive_expect_tx(bar, __popc(in) * (2 * BLK));
+    if (lane < U && block >= 0) {
+      const int64_t off = block * block_bytes + head_at;
+      const uint32_t dst = smem_u32(ring) + (stage * U + lane) * (2 * BLK);
+      bulk_load(dst, kp + off, BLK, bar);
+      bulk_load(dst + BLK, vp + off, BLK, bar);
     }
   };
-  int stage = 0, fill = 0, ahead = 0;
-  uint32_t parity = 0;
-  auto top_up = [&]() {
 #pragma unroll 1
-    for (; ahead < STAGES; ++ahead) {
-      issue(fill);
-      fill = fill + 1 == STAGES ? 0 : fill + 1;
-    }
-  };
-  top_up();
+  for (int i = 0; i < STAGES; ++i) issue(i);
+  int stage = 0;
+  uint32_t parity = 0;
 
   bool alive = true;
   int part_b[2] = {0, 0}, part_first[2] = {0, 0}, part_count[2] = {0, 0}, parts = 0;
@@ -225,49 +277,79 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
   int cg = warp;
   Segment cs;
   for (int b = b0, beg = beg0; segment(b, beg, cs); beg = behind(cs), ++b) {
-    if (h == 0 && tid == 0 && cs.beg >= r0 && p.status && __ldg(lens + b) != cs.len)
+    if (h == 0 && ct == 0 && tid == 0 && cs.beg >= r0 && p.status && __ldg(lens + b) != cs.k.len)
       atomicOr(p.status, 2);    // a length that is negative or beyond the sequence's pages: clamped, reported
-    if (cs.ng == 0 && cs.ng_all > 0) continue;
-    // ---- q: B fragments of a group's four k steps, and the group's sums of q and of OFF q for this lane's two columns
-    uint32_t qf[NT][G][8];
-    float qo[NT][G][2], qs[NT][G][2];
+    if (BLOCKS && h == 0 && ct == 0 && tid == 0 && cs.beg >= r0 && p.status &&
+        static_cast<int64_t>(cs.k.new_tok) * p.group > p.col_tiles * COLS)
+      atomicOr(p.status, 2);    // more new tokens than the call was told of: the rows behind are not written
+    if (cs.cols <= 0 || (cs.ng == 0 && cs.k.blocks > 0)) continue;
+    if (lane == 0) s_current[warp] = cs;
+    __syncwarp();
+    // query row of a column of this CTA
+    auto row_of = [&](int col) -> int64_t {
+      if constexpr (!BLOCKS) return static_cast<int64_t>(b) * p.hq + h * p.group + ct * COLS + col;
+      const int n = ct * COLS + col, t = n / p.group;
+      return static_cast<int64_t>(cs.k.tok0 + t) * p.hq + h * p.group + (n - t * p.group);
+    };
+    // ---- q: B fragments of the k steps (two of a word), 16 times q where the codes are the lowest bits of the fraction, and
+    // a group's sum of q (2^-20 of it, as the products have it) for this lane's two columns
+    uint32_t qf[NT][WORDS][4];
+    float qs[NT][G][2], cscale[NT][2];
+    int tok[NT][2];          // BLOCKS: token of this lane's columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int col = nt * 8 + r;
-      const T* qr = q + (static_cast<int64_t>(b) * p.hq + h * p.group + col) * HD + 16 * c;
+      const T* qr = q + (col < cs.cols ? row_of(col) : 0) * HD + 16 * c;
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {        // word (r8, g) = (2 c + w / G, w % G)
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (col < cs.cols) x = *reinterpret_cast<const uint4*>(qr + (w % G) * 64 + (w / G) * 8);
+        qf[nt][w][0] = x.x;
+        qf[nt][w][1] = x.y;
+        qf[nt][w][2] = x.z;
+        qf[nt][w][3] = x.w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(qf[nt][w][i] >> 16 & 0x7fffu, qf[nt][w][i] & 0x7fffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float power = row_power(T{}, top), inv = 1.f / power;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        cscale[nt][j] = p.scale_log2 * 1048576.f * __shfl_sync(0xffffffffu, power, (2 * c + j) * 4);
+        tok[nt][j] = BLOCKS ? (ct * COLS + nt * 8 + 2 * c + j) / p.group : 0;
+      }
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = unpack_pair(T{}, qf[nt][w][i]);
+          const float by = i & 1 ? inv : 16.f * inv;
+          qf[nt][w][i] = Mma::pack(x.x * by, x.y * by);
+        }
+      const uint32_t unit[4] = {0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u};
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
-        if (col < p.group) {
-          x = *reinterpret_cast<const uint4*>(qr + g * 64);
-          y = *reinterpret_cast<const uint4*>(qr + g * 64 + 8);
-        }
-        qf[nt][g][0] = x.x;
-        qf[nt][g][1] = x.y;
-        qf[nt][g][2] = x.z;
-        qf[nt][g][3] = x.w;
-        qf[nt][g][4] = y.x;
-        qf[nt][g][5] = y.y;
-        qf[nt][g][6] = y.z;
-        qf[nt][g][7] = y.w;
-        float one[4] = {0.f, 0.f, 0.f, 0.f}, off[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t a1[4] = {both<T>(1.f), both<T>(1.f), both<T>(1.f), both<T>(1.f)};
+        float one[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const int i = 2 * (ks & 1);
-          const uint32_t ao[4] = {both<T>(N::off(i)), both<T>(N::off(i)), both<T>(N::off(i + 1)), both<T>(N::off(i + 1))};
-          MmaOp<T>::run(one, a1, qf[nt][g][2 * ks], qf[nt][g][2 * ks + 1]);
-          MmaOp<T>::run(off, ao, qf[nt][g][2 * ks], qf[nt][g][2 * ks + 1]);
-        }
+        for (int w = g; w < WORDS; w += G)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) Mma::run(one, unit, qf[nt][w][i], qf[nt][w][i + 1]);
         qs[nt][g][0] = one[0];
         qs[nt][g][1] = one[1];
-        qo[nt][g][0] = -off[0];
-        qo[nt][g][1] = -off[1];
       }
     }
+    // tokens of the segment, and those that every column sees (BLOCKS: from the last token's window to the first token's position)
+    const int t_lo = (cs.k.first + cs.lo) * kKv4Rows;
+    const int t_hi = min(cs.k.len, (cs.k.first + cs.lo + cs.ng) * kKv4Rows);
+    const int all_lo = BLOCKS && p.window > 0 ? cs.k.prefix + cs.k.new_tok - p.window : 0;
+    const int all_hi = BLOCKS && !p.is_cross ? min(t_hi, cs.k.prefix + 1) : t_hi;
+    const int steps = (cs.ng + U - 1) / U, prefix = cs.k.prefix;
+    float vlim = 0.f;                             // the power of two over the scales so far (0: there was none)
+    float limit = kSlack - kLeastExponent;        // exponent over the reference that is not let pass
     float o[NT][G][4][4];        // [group][nibble]: elements 64 g + 8 r + 2 i, + 1 of columns 2 c, 2 c + 1
-    float ps4[NT][G][4];         // sums of P_g (elements 0 and 1)
-    float pbias[NT][G][2];       // sums of p (bias_g + 8 scale_g) over this lane's tokens
+    float pbias[NT][G][2];       // sums of p bias_g over this lane's tokens
     float m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -275,176 +357,218 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
       for (int g = 0; g < G; ++g) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          ps4[nt][g][e] = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][g][i][e] = 0.f;
         }
         pbias[nt][g][0] = pbias[nt][g][1] = 0.f;
       }
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = kNoScore;
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    for (; cg < cs.ng; cg += WARPS) {
-      {
-        const uint32_t bar = smem_u32(&s_bar[warp * STAGES + stage]);
-        bool ok = !alive || mbar_try_wait(bar, parity);
-        if (!ok) {
-          const long long t0 = clock64();
-          while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < kTcWaitCycles) {
-          }
+#pragma unroll 1
+    for (; cg < steps; cg += WARPS) {
+      const uint32_t bar = smem_u32(&s_bar[warp * STAGES + stage]);
+      if (__any_sync(0xffffffffu, !mbar_try_wait(bar, parity))) {
+        if (!alive) continue;
+        bool ok;
+        const long long t0 = clock64();
+        while (!(ok = mbar_try_wait(bar, parity)) && clock64() - t0 < kTcWaitCycles) {
         }
-        alive = __all_sync(0xffffffffu, alive && ok ? 1 : 0) != 0;
+        alive = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
         if (!alive) continue;
       }
-      const unsigned char* kb = ring + stage * (2 * BLK);
-      const unsigned char* vb = kb + BLK;
-      const int nvalid = cs.len - (cs.lo + cg) * kKv4Rows;       // >= 1
+      const unsigned char* const step_at = ring + stage * (U * 2 * BLK);
+      const int t0 = t_lo + cg * (U * kKv4Rows);
       // pairs of tokens rho and rho + 8
-      uint32_t kpair[2][G], vpair[2][G];
+      uint32_t kpair[U][2][G], vpair[U][2][G];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        read_words<G * 4>(kpair[t], kb + PAIRS + (rho + 8 * t) * (G * 4));
-        read_words<G * 4>(vpair[t], vb + PAIRS + (rho + 8 * t) * (G * 4));
-      }
-      if (nvalid < kKv4Rows || (bad >> stage & 1u)) {       // rows behind the end hold anything; a page outside the pool: zeros
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (rho + 8 * t >= nvalid || (bad >> stage & 1u)) {
+        for (int t = 0; t < 2; ++t) {
+          const unsigned char* at = step_at + u * (2 * BLK) + PAIRS + (rho + 8 * t) * (G * 4);
+          read_words<G * 4>(kpair[u][t], at);
+          read_words<G * 4>(vpair[u][t], at + BLK);
+        }
+      if (t0 + U * kKv4Rows > t_hi || bad != 0) {   // rows behind the end hold anything; a page outside the pool: zeros
 #pragma unroll
-            for (int g = 0; g < G; ++g) kpair[t][g] = vpair[t][g] = 0u;
-          }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (t0 + u * kKv4Rows + rho + 8 * t >= t_hi || (bad >> (stage * U + u) & 1u)) {
+#pragma unroll
+              for (int g = 0; g < G; ++g) kpair[u][t][g] = vpair[u][t][g] = 0u;
+            }
       }
       // ---- scores
-      float s[NT][4];
+      float s[U][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-      {
-        uint32_t w0[2 * G], w1[2 * G];       // words 2 c (groups 0 .. G - 1) and 2 c + 1 of tokens rho and rho + 8
-        read_words<8 * G>(w0, kb + rho * ROW + c * (8 * G));
-        read_words<8 * G>(w1, kb + (rho + 8) * ROW + c * (8 * G));
+      for (int u = 0; u < U; ++u) {
+        const unsigned char* const kb = step_at + u * (2 * BLK);
+        uint32_t w0[WORDS], w1[WORDS];       // words of tokens rho and rho + 8
+        read_words<4 * WORDS>(w0, kb + rho * ROW + c * (4 * WORDS));
+        read_words<4 * WORDS>(w1, kb + (rho + 8) * ROW + c * (4 * WORDS));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           float acc[NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            acc[nt][0] = acc[nt][2] = qo[nt][g][0];
-            acc[nt][1] = acc[nt][3] = qo[nt][g][1];
-          }
+          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint32_t x = w0[(ks >> 1) * G + g], y = w1[(ks >> 1) * G + g];
-            const int i = 2 * (ks & 1);
-            const uint32_t a[4] = {N::make(x, i), N::make(y, i), N::make(x, i + 1), N::make(y, i + 1)};
+          for (int w = g; w < WORDS; w += G) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(acc[nt], a, qf[nt][g][2 * ks], qf[nt][g][2 * ks + 1]);
+            for (int i = 0; i < 4; i += 2) {
+              const uint32_t x = w0[w] >> (4 * i), y = w1[w] >> (4 * i);
+              const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) Mma::run(acc[nt], a, qf[nt][w][i], qf[nt][w][i + 1]);
+            }
           }
-          const float2 p0 = unpack_pair(T{}, kpair[0][g]), p1 = unpack_pair(T{}, kpair[1][g]);
+          const float2 p0 = unpack_pair(T{}, kpair[u][0][g]), p1 = unpack_pair(T{}, kpair[u][1][g]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              s[nt][j] = fmaf(p0.y, qs[nt][g][j], fmaf(p0.x, acc[nt][j], s[nt][j]));
-              s[nt][2 + j] = fmaf(p1.y, qs[nt][g][j], fmaf(p1.x, acc[nt][2 + j], s[nt][2 + j]));
+              s[u][nt][j] = fmaf(p0.x, acc[nt][j], g == 0 ? p0.y * qs[nt][g][j] : fmaf(p0.y, qs[nt][g][j], s[u][nt][j]));
+              s[u][nt][2 + j] = fmaf(p1.x, acc[nt][2 + j], g == 0 ? p1.y * qs[nt][g][j] : fmaf(p1.y, qs[nt][g][j], s[u][nt][2 + j]));
             }
           }
         }
       }
-      bool up = false;
+      float smax = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[nt][j] *= p.scale_log2;
-          if (nvalid < kKv4Rows && rho + 8 * (j >> 1) >= nvalid) s[nt][j] = -INFINITY;
-          up |= s[nt][j] > m[nt][j & 1] + N::kSlack;
+        for (int g = 0; g < G; ++g)
+          smax = max3(smax, unpack_pair(T{}, vpair[u][0][g]).x, unpack_pair(T{}, vpair[u][1][g]).x);
+      // ---- exponents over the reference (one that is not there yet is far below every score)
+      float x[U][NT][4], over = -INFINITY;
+      auto seen = [&](int u, int nt, int j) -> bool {
+        const int t = t0 + u * kKv4Rows + rho + 8 * (j >> 1);
+        if constexpr (!BLOCKS) return t < t_hi;
+        const int pos = prefix + tok[nt][j & 1];
+        return t < t_hi && (p.is_cross || t <= pos) && (p.window == 0 || t > pos - p.window);
+      };
+      const bool edge = t0 + U * kKv4Rows > all_hi || t0 < all_lo;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[u][nt][j] *= cscale[nt][j & 1];
         }
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[u][nt][j] = seen(u, nt, j) ? s[u][nt][j] : -INFINITY;
       }
-      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[u][nt][j] = s[u][nt][j] - m[nt][j & 1];
+          over = max3(max3(over, x[u][nt][0], x[u][nt][1]), x[u][nt][2], x[u][nt][3]);
+        }
+      if (__any_sync(0xffffffffu, over > limit || smax > vlim)) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
+        if (smax > vlim) {
+          const uint32_t e = (__float_as_uint(smax) >> 23) + 1;
+          vlim = __uint_as_float(e << 23);
+          limit = kSlack - max(static_cast<int>(e) - 127, kLeastExponent);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float mx = fmaxf(s[nt][j], s[nt][2 + j]);
+            float mx = -INFINITY;
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            mx = fmaxf(mx, m[nt][j]);
-            const float a = mx == -INFINITY ? 1.f : fast_exp2(m[nt][j] - mx);
+            for (int u = 0; u < U; ++u) mx = max3(mx, s[u][nt][j], s[u][nt][2 + j]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mx = fmaxf(mx + (kSlack - limit), m[nt][j]);
+            const float a = fast_exp2(m[nt][j] - mx);
             m[nt][j] = mx;
             l[nt][j] *= a;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               pbias[nt][g][j] *= a;
-              ps4[nt][g][j] *= a;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 o[nt][g][i][j] *= a;
                 o[nt][g][i][2 + j] *= a;
               }
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              x[u][nt][j] = s[u][nt][j] - mx;
+              x[u][nt][2 + j] = s[u][nt][2 + j] - mx;
+            }
           }
         }
       }
-      uint32_t pf[NT][G][2];      // P_g as B fragments
+      uint32_t pf[U][NT][G][2];      // P_g as B fragments
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float mm = m[nt][j & 1];
-          s[nt][j] = fast_exp2(s[nt][j] - (mm == -INFINITY ? 0.f : mm));
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[u][nt][j] = fast_exp2(x[u][nt][j]);
+          l[nt][0] += x[u][nt][0] + x[u][nt][2];
+          l[nt][1] += x[u][nt][1] + x[u][nt][3];
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float2 p0 = unpack_pair(T{}, vpair[u][0][g]), p1 = unpack_pair(T{}, vpair[u][1][g]);
+            pbias[nt][g][0] = fmaf(x[u][nt][0], p0.y, fmaf(x[u][nt][2], p1.y, pbias[nt][g][0]));
+            pbias[nt][g][1] = fmaf(x[u][nt][1], p0.y, fmaf(x[u][nt][3], p1.y, pbias[nt][g][1]));
+            pf[u][nt][g][0] = transpose_8x8(Mma::pack(x[u][nt][0] * p0.x, x[u][nt][1] * p0.x));
+            pf[u][nt][g][1] = transpose_8x8(Mma::pack(x[u][nt][2] * p1.x, x[u][nt][3] * p1.x));
+          }
         }
-        l[nt][0] += s[nt][0] + s[nt][2];
-        l[nt][1] += s[nt][1] + s[nt][3];
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float2 p0 = unpack_pair(T{}, vpair[0][g]), p1 = unpack_pair(T{}, vpair[1][g]);
-          const float b0 = fmaf(8.f, p0.x, p0.y), b1 = fmaf(8.f, p1.x, p1.y);
-          pbias[nt][g][0] = fmaf(s[nt][0], b0, fmaf(s[nt][2], b1, pbias[nt][g][0]));
-          pbias[nt][g][1] = fmaf(s[nt][1], b0, fmaf(s[nt][3], b1, pbias[nt][g][1]));
-          pf[nt][g][0] = transpose_8x8(MmaOp<T>::pack(s[nt][0] * p0.x, s[nt][1] * p0.x));
-          pf[nt][g][1] = transpose_8x8(MmaOp<T>::pack(s[nt][2] * p1.x, s[nt][3] * p1.x));
-        }
-      }
       // ---- O^T += V^T P^T
-      {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const unsigned char* const vb = step_at + u * (2 * BLK) + BLK + r * (4 * G);
         uint32_t v0[G], v1[G], v2[G], v3[G];      // word r of tokens tv, tw, tv + 8, tw + 8
-        read_words<4 * G>(v0, vb + tv * ROW + r * (4 * G));
-        read_words<4 * G>(v1, vb + tw * ROW + r * (4 * G));
-        read_words<4 * G>(v2, vb + (tv + 8) * ROW + r * (4 * G));
-        read_words<4 * G>(v3, vb + (tw + 8) * ROW + r * (4 * G));
+        read_words<4 * G>(v0, vb + tv * ROW);
+        read_words<4 * G>(v1, vb + tw * ROW);
+        read_words<4 * G>(v2, vb + (tv + 8) * ROW);
+        read_words<4 * G>(v3, vb + (tw + 8) * ROW);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint32_t lo0 = __byte_perm(v0[g], v1[g], 0x5410), hi0 = __byte_perm(v0[g], v1[g], 0x7632);
           const uint32_t lo1 = __byte_perm(v2[g], v3[g], 0x5410), hi1 = __byte_perm(v2[g], v3[g], 0x7632);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t a[4] = {N::make(lo0, i), N::make(hi0, i), N::make(lo1, i), N::make(hi1, i)};
+            const uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu;
+            const uint32_t a[4] = {lo0 >> (8 * (i >> 1)) & mask, hi0 >> (8 * (i >> 1)) & mask, lo1 >> (8 * (i >> 1)) & mask,
+                                   hi1 >> (8 * (i >> 1)) & mask};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(o[nt][g][i], a, pf[nt][g][0], pf[nt][g][1]);
+            for (int nt = 0; nt < NT; ++nt) Mma::run(o[nt][g][i], a, pf[u][nt][g][0], pf[u][nt][g][1]);
           }
-          const uint32_t a1[4] = {both<T>(1.f), both<T>(1.f), both<T>(1.f), both<T>(1.f)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) MmaOp<T>::run(ps4[nt][g], a1, pf[nt][g][0], pf[nt][g][1]);
         }
       }
-      __syncwarp();                 // every lane has read the stage
-      --ahead;
+      __syncwarp();                 // every lane has read the stage: it is free
+      issue(stage);
       if (++stage == STAGES) {
         stage = 0;
         parity ^= 1;
       }
-      top_up();
     }
-    cg -= cs.ng;
+    cg -= steps;
+    cs = s_current[warp];
 
     // ---- end of the segment: the warps' sums are merged, four columns (those of one j) at a time
-    const bool whole = cs.ng == cs.ng_all;
-    const int64_t slot = ((2ll * share_id + (cs.beg >= r0 ? 1 : 0)) * p.hkv + h) * p.group;
+    const bool whole = cs.ng == cs.k.blocks;
+    const int64_t slot = (((2ll * share_id + (cs.beg >= r0 ? 1 : 0)) * p.hkv + h) * p.col_tiles + ct) * COLS;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (nt * 8 + j >= p.group) continue;         // (none of the columns 8 nt + j, + 2, + 4, + 6)
+        if (nt * 8 + j >= cs.cols) continue;         // (none of the columns 8 nt + j, + 2, + 4, + 6)
         float lj = l[nt][j];
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) lj += __shfl_xor_sync(0xffffffffu, lj, x);
@@ -457,9 +581,9 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
           float x[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float d = fmaf(-8.f - N::off(i), ps4[nt][g][j], bj);
-            x[2 * i] = o[nt][g][i][j] + d;
-            x[2 * i + 1] = o[nt][g][i][2 + j] + d;
+            const float unit = i & 1 ? 1048576.f : 16777216.f;
+            x[2 * i] = fmaf(o[nt][g][i][j], unit, bj);
+            x[2 * i + 1] = fmaf(o[nt][g][i][2 + j], unit, bj);
           }
           *reinterpret_cast<float4*>(row + g * 64) = make_float4(x[0], x[1], x[2], x[3]);
           *reinterpret_cast<float4*>(row + g * 64 + 4) = make_float4(x[4], x[5], x[6], x[7]);
@@ -469,7 +593,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
         for (int e = tid; e < HD; e += WARPS * 32) {      // float4 pieces of the four columns
           const int cc = e / (HD / 4), d = e % (HD / 4) * 4;
           const int col = nt * 8 + 2 * cc + j;
-          if (col >= p.group) continue;
+          if (col >= cs.cols) continue;
           float M = -INFINITY, den = 0.f;
 #pragma unroll
           for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_ml[(w * 4 + cc) * 2]);
@@ -487,7 +611,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
           }
           if (whole) {
             const float inv = den == 0.f ? 0.f : 1.f / den;
-            const int64_t at = (static_cast<int64_t>(b) * p.hq + h * p.group + col) * HD + d;
+            const int64_t at = row_of(col) * HD + d;
             alignas(8) T y[4] = {MmaOp<T>::from_float(x.x * inv), MmaOp<T>::from_float(x.y * inv),
                                  MmaOp<T>::from_float(x.z * inv), MmaOp<T>::from_float(x.w * inv)};
             if (p.gate != nullptr) {
@@ -508,43 +632,64 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
       const int i = parts++ & 1;
       part_b[i] = b;
       part_first[i] = cs.beg / share;
-      part_count[i] = (cs.beg + cs.ng_all - 1) / share - part_first[i] + 1;
+      part_count[i] = (cs.beg + cs.k.blocks - 1) / share - part_first[i] + 1;
     }
   }
 
   // ---- the CTA that arrives last at a (sequence, head) merges its pieces
   for (int i = 0; i < parts; ++i) {
     if (tid == 0) {
-      int* ticket = p.tickets + static_cast<int64_t>(part_b[i]) * p.hkv + h;
+      int* ticket = p.tickets + (static_cast<int64_t>(part_b[i]) * p.hkv + h) * p.col_tiles + ct;
       s_last = atomic_add_acq_rel(ticket, 1) == part_count[i] - 1;   // (the others' rows: behind the CTA barrier above)
       if (s_last) *ticket = 0;
     }
     __syncthreads();
     if (s_last) {
-      const int64_t pitch = 2ll * p.hkv * p.group * PROW;          // from share to share
-      const float* rows = p.part + part_first[i] * pitch + static_cast<int64_t>(h) * p.group * PROW;
+      const int64_t pitch = 2ll * p.hkv * p.col_tiles * COLS * PROW;          // from share to share
+      const float* rows = p.part + part_first[i] * pitch + (static_cast<int64_t>(h) * p.col_tiles + ct) * COLS * PROW;
       const int n = part_count[i];
-      for (int e = tid; e < p.group * (HD / 4); e += WARPS * 32) {
+      const Keys k = keys(part_b[i]);
+      const int cols = min((BLOCKS ? k.new_tok : 1) * p.group - ct * COLS, COLS);
+      for (int e = tid; e < cols * (HD / 4); e += WARPS * 32) {
         const int col = e / (HD / 4), d = e % (HD / 4) * 4;
         const float* row = rows + col * PROW;
         auto piece = [&](int k) { return row + k * pitch + (k == 0 ? pitch / 2 : 0); };
         float M = -INFINITY, den = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < n; ++k) M = fmaxf(M, __ldcg(piece(k) + HD));
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int k = 0; k < n; ++k) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(k) + HD));
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(piece(k) + d));
-          const float wgt = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-          den = fmaf(wgt, ml.y, den);
-          x.x = fmaf(wgt, y.x, x.x);
-          x.y = fmaf(wgt, y.y, x.y);
-          x.z = fmaf(wgt, y.z, x.z);
-          x.w = fmaf(wgt, y.w, x.w);
+        constexpr int FLY = 8;                      // pieces in flight
+#pragma unroll 1
+        for (int k0 = 0; k0 < n; k0 += FLY) {
+          float2 ml[FLY];
+          float4 y[FLY];
+#pragma unroll
+          for (int k = 0; k < FLY; ++k) {
+            const float* at = piece(min(k0 + k, n - 1));
+            ml[k] = __ldcg(reinterpret_cast<const float2*>(at + HD));
+            y[k] = __ldcg(reinterpret_cast<const float4*>(at + d));
+          }
+          float mx = M;
+#pragma unroll
+          for (int k = 0; k < FLY; ++k) mx = fmaxf(mx, ml[k].x);
+          const float old = M == -INFINITY ? 0.f : fast_exp2(M - mx);
+          M = mx;
+          den *= old;
+          x.x *= old;
+          x.y *= old;
+          x.z *= old;
+          x.w *= old;
+#pragma unroll
+          for (int k = 0; k < FLY; ++k) {
+            const float wgt = k0 + k >= n || ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - mx);
+            den = fmaf(wgt, ml[k].y, den);
+            x.x = fmaf(wgt, y[k].x, x.x);
+            x.y = fmaf(wgt, y[k].y, x.y);
+            x.z = fmaf(wgt, y[k].z, x.z);
+            x.w = fmaf(wgt, y[k].w, x.w);
+          }
         }
         const float inv = den == 0.f ? 0.f : 1.f / den;
-        const int64_t at = (static_cast<int64_t>(part_b[i]) * p.hq + h * p.group + col) * HD + d;
+        const int head = BLOCKS ? (ct * COLS + col) % p.group : ct * COLS + col;
+        const int64_t at = ((BLOCKS ? k.tok0 + (ct * COLS + col) / p.group : static_cast<int64_t>(part_b[i])) * p.hq + h * p.group + head) * HD + d;
         alignas(8) T y[4] = {MmaOp<T>::from_float(x.x * inv), MmaOp<T>::from_float(x.y * inv),
                              MmaOp<T>::from_float(x.z * inv), MmaOp<T>::from_float(x.w * inv)};
         if (p.gate != nullptr) {
@@ -559,7 +704,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
   if (!alive) {       // gave up: what is still on its way lands before the shared memory goes away; bounded
     if (p.status && lane == 0) atomicOr(p.status, 1);
     const long long t0 = clock64();
-    for (; ahead > 0; --ahead) {
+    for (int i = 0; i < STAGES; ++i) {
       while (!mbar_try_wait(smem_u32(&s_bar[warp * STAGES + stage]), parity) && clock64() - t0 < 2000000LL) {
       }
       if (++stage == STAGES) {

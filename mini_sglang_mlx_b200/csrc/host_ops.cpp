@@ -628,8 +628,8 @@ PyObject* prefill_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Scratch ws;
   if (!stream_of(a[14], s.device, &stream) ||
       !scratch_for(s.device, stream, kPrefill,
-                   msgl_prefill_workspace_bytes(batch, total_q, pages.numel() * page_size, hq, s.hkv, s.d,
-                                                static_cast<int>(max_ext), static_cast<int>(window)),
+                   msgl_prefill_workspace_bytes_q4(batch, total_q, pages.numel(), ps, hq, s.hkv, s.d,
+                                                   static_cast<int>(max_ext), static_cast<int>(window)),
                    &ws))
     return nullptr;
   Tensor out = empty_like_rows(q);

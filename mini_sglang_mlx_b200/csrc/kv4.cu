@@ -35,35 +35,82 @@ unsigned grid_of(int64_t threads, int per_sm) {
 }
 
 // ---- decode scheduling, in blocks of 16 tokens
-constexpr int kQ4Warps = 8;
 constexpr int kQ4MinShare = 8;
 constexpr int kQ4MaxShare = 1024;
 constexpr int kQ4Pad = 12;
 
 struct Q4Plan {
-  int ctas_per_sm;
+  int col_tiles, cols;       // CTAs side by side, columns of each
   int64_t shares;
   size_t ticket_bytes, part_bytes;
 };
-Q4Plan plan_q4_decode(int batch, int hq, int hkv, int head_dim, int64_t total_tokens, int sms) {
+// `columns` of a sequence at most, `blocks` of all sequences at most.
+Q4Plan plan_q4(int batch, int columns, int hkv, int head_dim, int64_t blocks, int sms) {
   Q4Plan pl{};
-  pl.ctas_per_sm = head_dim == 128 && hq / hkv <= 8 ? 2 : 1;
-  const int64_t wave = std::max(1, sms * pl.ctas_per_sm / hkv);
-  const int64_t blocks = total_tokens / msgl::kKv4Rows + static_cast<int64_t>(batch) * kQ4Pad;
+  pl.cols = head_dim == 128 && columns > 8 ? 16 : 8;
+  pl.col_tiles = (columns + pl.cols - 1) / pl.cols;
+  constexpr int ctas_per_sm = 1;
+  const int64_t wave = std::max(1, sms * ctas_per_sm / (hkv * pl.col_tiles));
+  blocks += static_cast<int64_t>(batch) * kQ4Pad;
   pl.shares = wave * std::max<int64_t>(1, (blocks + wave * kQ4MaxShare - 1) / (wave * kQ4MaxShare));
-  const size_t tickets = static_cast<size_t>(batch) * hkv;
+  const size_t tickets = static_cast<size_t>(batch) * hkv * pl.col_tiles;
   pl.ticket_bytes = tickets <= kTicketSlots ? 0 : (tickets * sizeof(int) + 255) / 256 * 256;
-  pl.part_bytes = static_cast<size_t>(pl.shares) * 2 * hq * msgl::q4_partial_floats(head_dim) * sizeof(float);
+  pl.part_bytes = static_cast<size_t>(pl.shares) * 2 * hkv * pl.col_tiles * pl.cols * msgl::q4_partial_floats(head_dim) * sizeof(float);
   return pl;
 }
 
-template <typename T, int HD, int NT, int STAGES, int MINB>
-cudaError_t launch_q4_decode(const msgl::Q4DecodeParams& p, cudaStream_t s) {
-  auto* kernel = msgl::q4_decode_kernel<T, HD, NT, kQ4Warps, STAGES, MINB>;
-  constexpr int smem = msgl::q4_decode_smem(HD, kQ4Warps, STAGES);
+template <typename T, int HD, int NT, bool BLOCKS, int U, int WARPS, int STAGES, int MINB>
+cudaError_t launch_q4(const msgl::Q4DecodeParams& p, cudaStream_t s) {
+  auto* kernel = msgl::q4_decode_kernel<T, HD, NT, BLOCKS, U, WARPS, STAGES, MINB>;
+  constexpr int smem = msgl::q4_decode_smem(HD, WARPS, STAGES * U);
   const cudaError_t e = allow_smem(kernel, smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(p.num_shares * p.hkv)), dim3(kQ4Warps * 32), smem, s, p);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(p.num_shares * p.col_tiles * p.hkv)), dim3(WARPS * 32), smem, s, p);
+}
+template <bool BLOCKS>
+cudaError_t launch_q4_any(const msgl::Q4DecodeParams& p, int head_dim, int cols, int dtype, cudaStream_t s) {
+  auto go = [&](auto tag) -> cudaError_t {
+    using T = decltype(tag);
+    if (head_dim == 256) return launch_q4<T, 256, 1, BLOCKS, 1, 12, 3, 1>(p, s);
+    return cols == 8 ? launch_q4<T, 128, 1, BLOCKS, 2, 12, 3, 1>(p, s) : launch_q4<T, 128, 2, BLOCKS, 1, 12, 6, 1>(p, s);
+  };
+  return dtype == MSGL_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+}
+
+// The rest of a call's parameters, and its launch.
+template <bool BLOCKS>
+int run_q4(const char* op, msgl::Q4DecodeParams& p, const Q4Plan& pl, void* workspace, size_t workspace_bytes, int head_dim,
+           int dtype, void* stream) {
+  if (!workspace || workspace_bytes < kStatusBytes + pl.ticket_bytes + pl.part_bytes)
+    return fail(MSGL_BAD_ARG, std::string(op) + ": workspace too small");
+  if (pl.shares * pl.col_tiles * p.hkv > 0x7fffffffLL)
+    return fail(MSGL_BAD_SHAPE, std::string(op) + ": problem too large for one launch");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  p.status = reinterpret_cast<int*>(ws);
+  p.tickets = reinterpret_cast<int*>(ws + (pl.ticket_bytes == 0 ? 256 : kStatusBytes));
+  p.part = reinterpret_cast<float*>(ws + kStatusBytes + pl.ticket_bytes);
+  if (pl.ticket_bytes != 0) {
+    const cudaError_t e = cudaMemsetAsync(p.tickets, 0, pl.ticket_bytes, s);
+    if (e != cudaSuccess) return cuda_fail(op, e);
+  }
+  p.col_tiles = pl.col_tiles;
+  p.num_shares = static_cast<int>(pl.shares);
+  p.min_share = kQ4MinShare;
+  p.pad = kQ4Pad;
+  const cudaError_t e = launch_q4_any<BLOCKS>(p, head_dim, pl.cols, dtype, s);
+  return e == cudaSuccess ? MSGL_OK : cuda_fail(op, e);
+}
+
+// Query blocks of few columns per KV head run the decode kernel (decode_q4.cuh), others the one-CTA tcgen05 kernel.
+constexpr int kQ4BlockColumns = 16;
+bool q4_block_form(int max_len_extend, int group) {
+  return static_cast<int64_t>(max_len_extend) * group <= kQ4BlockColumns;
+}
+// Blocks of a call at most: what the pages hold, or what a window leaves.
+int64_t q4_block_bound(int batch, int64_t total_pages, int page_size, int max_len_extend, int window) {
+  const int64_t all = total_pages * page_size / msgl::kKv4Rows;
+  return window > 0 ? std::min<int64_t>(all, batch * ((static_cast<int64_t>(window) + max_len_extend) / msgl::kKv4Rows + 2)) : all;
 }
 
 }  // namespace
@@ -200,7 +247,8 @@ size_t msgl_decode_workspace_bytes_q4(int batch, int num_q_heads, int num_kv_hea
   if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || total_pages < 0 || page_size <= 0)
     return kStatusBytes;
   const int sms = sm_count_cached();
-  const Q4Plan pl = plan_q4_decode(batch, num_q_heads, num_kv_heads, head_dim, total_pages * page_size, sms > 0 ? sms : 148);
+  const Q4Plan pl = plan_q4(batch, std::max(1, num_q_heads / num_kv_heads), num_kv_heads, head_dim,
+                            total_pages * page_size / msgl::kKv4Rows, sms > 0 ? sms : 148);
   return kStatusBytes + pl.ticket_bytes + pl.part_bytes;
 }
 
@@ -230,13 +278,8 @@ int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const voi
     return fail(MSGL_BAD_ARG, std::string(op) + "q, the pools, out, gate and the workspace must be 16-byte aligned");
   const int sms = sm_count_cached();
   if (sms <= 0) return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot query the device");
-  const Q4Plan pl = plan_q4_decode(batch, num_q_heads, num_kv_heads, head_dim, total_pages * page_size, sms);
-  if (!workspace || workspace_bytes < kStatusBytes + pl.ticket_bytes + pl.part_bytes)
-    return fail(MSGL_BAD_ARG, std::string(op) + "workspace too small");
-  if (pl.shares * num_kv_heads > 0x7fffffffLL)
-    return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  const Q4Plan pl = plan_q4(batch, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
+                            total_pages * page_size / msgl::kKv4Rows, sms);
   msgl::Q4DecodeParams p{};
   p.q = q;
   p.k_pool = static_cast<const unsigned char*>(k_cache);
@@ -248,30 +291,28 @@ int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const voi
   p.total_pages = static_cast<int>(total_pages);
   p.out = out;
   p.gate = gate;
-  p.status = reinterpret_cast<int*>(ws);
-  p.tickets = reinterpret_cast<int*>(ws + (pl.ticket_bytes == 0 ? 256 : kStatusBytes));
-  p.part = reinterpret_cast<float*>(ws + kStatusBytes + pl.ticket_bytes);
-  if (pl.ticket_bytes != 0) {
-    const cudaError_t e = cudaMemsetAsync(p.tickets, 0, pl.ticket_bytes, s);
-    if (e != cudaSuccess) return cuda_fail("paged_decode_attention_q4", e);
-  }
   p.batch = batch;
   p.hq = num_q_heads;
   p.hkv = num_kv_heads;
   p.group = num_q_heads / num_kv_heads;
-  p.num_shares = static_cast<int>(pl.shares);
-  p.min_share = kQ4MinShare;
-  p.pad = kQ4Pad;
   p.num_blocks = num_slots / msgl::kKv4Rows;
   p.scale_log2 = sm_scale * msgl::kLog2e;
-  auto go = [&](auto tag) -> cudaError_t {
-    using T = decltype(tag);
-    if (head_dim == 128)
-      return p.group <= 8 ? launch_q4_decode<T, 128, 1, 5, 2>(p, s) : launch_q4_decode<T, 128, 2, 8, 1>(p, s);
-    return p.group <= 8 ? launch_q4_decode<T, 256, 1, 4, 1>(p, s) : launch_q4_decode<T, 256, 2, 4, 1>(p, s);
-  };
-  const cudaError_t e = dtype == MSGL_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(__half{});
-  return e == cudaSuccess ? MSGL_OK : cuda_fail("paged_decode_attention_q4", e);
+  return run_q4<false>("paged_decode_attention_q4", p, pl, workspace, workspace_bytes, head_dim, dtype, stream);
+}
+
+size_t msgl_prefill_workspace_bytes_q4(int batch, int total_q, int64_t total_pages, int page_size, int num_q_heads,
+                                       int num_kv_heads, int head_dim, int max_len_extend, int sliding_window_size) {
+  if (batch <= 0 || total_q <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || total_pages < 0 || page_size <= 0)
+    return kStatusBytes;
+  max_len_extend = std::max(1, max_len_extend);
+  const int group = std::max(1, num_q_heads / num_kv_heads);
+  if (!q4_block_form(max_len_extend, group))
+    return msgl_prefill_workspace_bytes(batch, total_q, total_pages * page_size, num_q_heads, num_kv_heads, head_dim,
+                                        max_len_extend, sliding_window_size);
+  const int sms = sm_count_cached();
+  const Q4Plan pl = plan_q4(batch, max_len_extend * group, num_kv_heads, head_dim,
+                            q4_block_bound(batch, total_pages, page_size, max_len_extend, sliding_window_size), sms > 0 ? sms : 148);
+  return kStatusBytes + pl.ticket_bytes + pl.part_bytes;
 }
 
 int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const void* v_cache, const int32_t* qo_indptr,
@@ -304,6 +345,32 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     return fail(MSGL_BAD_ARG, std::string(op) + "q, the pools, out, gate and the workspace must be 16-byte aligned");
   const int sms = sm_count_cached();
   if (sms <= 0) return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot query the device");
+  if (batch <= 65535 && q4_block_form(max_len_extend, num_q_heads / num_kv_heads)) {
+    const Q4Plan blocks = plan_q4(batch, max_len_extend * (num_q_heads / num_kv_heads), num_kv_heads, head_dim,
+                                  q4_block_bound(batch, total_pages, page_size, max_len_extend, sliding_window_size), sms);
+    msgl::Q4DecodeParams p{};
+    p.q = q;
+    p.k_pool = static_cast<const unsigned char*>(k_cache);
+    p.v_pool = static_cast<const unsigned char*>(v_cache);
+    p.page_indptr = page_indptr;
+    p.page_indices = page_indices;
+    p.kv_lens = kv_lens;
+    p.qo_indptr = qo_indptr;
+    p.prefix_lens = prefix_lens;
+    p.page_blocks = page_size / msgl::kKv4Rows;
+    p.total_pages = static_cast<int>(total_pages);
+    p.out = out;
+    p.gate = gate;
+    p.batch = batch;
+    p.hq = num_q_heads;
+    p.hkv = num_kv_heads;
+    p.group = num_q_heads / num_kv_heads;
+    p.is_cross = is_cross_attention ? 1 : 0;
+    p.window = sliding_window_size;
+    p.num_blocks = num_slots / msgl::kKv4Rows;
+    p.scale_log2 = sm_scale * msgl::kLog2e;
+    return run_q4<true>("paged_prefill_attention_q4", p, blocks, workspace, workspace_bytes, head_dim, dtype, stream);
+  }
   const PrefillPlan pl = plan_prefill(batch, total_q, total_pages * page_size, num_q_heads, num_kv_heads, head_dim,
                                       max_len_extend, sliding_window_size, sms);
   if (!workspace || workspace_bytes < kStatusBytes + pl.plan_bytes + pl.part_ml_bytes + pl.part_o_bytes)
@@ -343,13 +410,15 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
   p.page_recip = msgl::reciprocal(page_size);
   p.chunk_recip = msgl::reciprocal(p.kv_chunk);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  CUtensorMap none;
+  CUtensorMap none, tm_q;
   std::memset(&none, 0, sizeof(none));
+  std::memset(&tm_q, 0, sizeof(tm_q));
+  p.q_tma = make_query_tensor_map(&tm_q, q, total_q, num_q_heads, p.group, head_dim, dtype) ? 1 : 0;
   const dim3 grid(static_cast<unsigned>(pl.items * num_kv_heads));
   auto launch = [&](auto kernel, auto merge, int threads, int smem) -> cudaError_t {
     cudaError_t err = allow_smem(kernel, smem);
     if (err != cudaSuccess) return err;
-    err = launch_dependent(kernel, grid, dim3(threads), smem, s, p, none, none, none);
+    err = launch_dependent(kernel, grid, dim3(threads), smem, s, p, none, none, tm_q);
     if (err != cudaSuccess) return err;
     if (pl.kv_chunk > 0 && !pl.fused_merge)
       return launch_dependent(merge, dim3(grid.x, msgl::kMergeSlices), dim3(msgl::kMergeWarps * 32), 0, s, p);
@@ -362,12 +431,12 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     using S1w = msgl::TcShape<1, 256>;
     if (head_dim == 256)
       return launch(msgl::prefill_tc_kernel<T, 64, 1, 256, false, true>, msgl::prefill_merge_kernel<T, 256, S1w::kBM>,
-                    S1w::kThreads, S1w::kSmemBytes);
+                    S1w::kThreads, msgl::Kv4Shape<1, 256>::kSmemBytes);
     if (prefill_short_q(max_len_extend, p.group, head_dim))
       return launch(msgl::prefill_tc_kernel<T, 64, 1, 128, false, true>, msgl::prefill_merge_kernel<T, 128, S1::kBM>,
-                    S1::kThreads, S1::kSmemBytes);
+                    S1::kThreads, msgl::Kv4Shape<1, 128>::kSmemBytes);
     return launch(msgl::prefill_tc_kernel<T, 128, 2, 128, false, true>, msgl::prefill_merge_kernel<T, 128, S2::kBM>,
-                  S2::kThreads, S2::kSmemBytes);
+                  S2::kThreads, msgl::Kv4Shape<2, 128>::kSmemBytes);
   };
   const cudaError_t e = dtype == MSGL_DTYPE_BF16 ? dispatch(__nv_bfloat16{}) : dispatch(__half{});
   return e == cudaSuccess ? MSGL_OK : cuda_fail("paged_prefill_attention_q4", e);

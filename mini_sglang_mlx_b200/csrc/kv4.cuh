@@ -56,7 +56,6 @@ struct Nibble;
 template <>
 struct Nibble<__nv_bfloat16> {    // seven bits of fraction: a nibble in the lowest four counts from 128, one at bit 3 from 16
   __host__ __device__ static constexpr float off(int i) { return i == 0 ? 128.f : 16.f; }
-  static constexpr float kSlack = 8.f;
   __device__ __forceinline__ static uint32_t make(uint32_t w, int i) {
     return i == 0 ? ((w & 0x000f000fu) | 0x43004300u) : (((w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u);
   }
@@ -64,7 +63,6 @@ struct Nibble<__nv_bfloat16> {    // seven bits of fraction: a nibble in the low
 template <>
 struct Nibble<__half> {           // ten bits of fraction: at bit 4, 4, 2 and 6
   __host__ __device__ static constexpr float off(int i) { return i < 2 ? 64.f : i == 2 ? 256.f : 16.f; }
-  static constexpr float kSlack = 2.f;    // (2^2 of the largest scale, 8734, is a half)
   __device__ __forceinline__ static uint32_t make(uint32_t w, int i) {
     return i == 0   ? (((w << 4) & 0x00f000f0u) | 0x54005400u)
            : i == 1 ? ((w & 0x00f000f0u) | 0x54005400u)
@@ -116,6 +114,23 @@ __device__ __forceinline__ uint4 kv4_values(uint32_t word, uint32_t pair) {
     v[i] = fma_pair(T{}, n, scale, bias);
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// A row's power of two, from its largest magnitude (the bits of a T): what is divided by it is below 2^11.
+__device__ __forceinline__ float row_power(__half, uint32_t top) {
+  const float x = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
+  return __uint_as_float((max(__float_as_uint(x) >> 23, 12u) - 10u) << 23);
+}
+__device__ __forceinline__ float row_power(__nv_bfloat16, uint32_t top) {
+  return __uint_as_float((max(top >> 7, 12u) - 10u) << 23);
+}
+
+// A pair of type T as one of another type.
+template <typename T>
+__device__ __forceinline__ uint32_t same_pair(T, T, uint32_t pair) { return pair; }
+__device__ __forceinline__ uint32_t same_pair(__nv_bfloat16, __half, uint32_t pair) {
+  const float2 x = unpack_pair(__nv_bfloat16{}, pair);
+  return MmaOp<__half>::pack(x.x, x.y);
 }
 
 // Codes of the 2 W elements that a lane holds of a group of 64, LANES = 32 / W lanes of `mask` together, and the group's pair

@@ -96,6 +96,17 @@ struct TcShape {
   static constexpr bool kRebalanceRegs = !(PAGED && NSUB == 1) && !(HD == 256 && !PAGED);
 };
 
+// The same over a pool held in 4 bits (kv4.cuh).  The first copying warp fetches blocks (16 tokens of the head, one bulk copy)
+// into a ring of their own; the others, a block each in turn, write its elements into the tiles, scale * code + bias
+// rounded once (K to T, V to f16, see below); the tiles' ring is shorter for it.
+template <int NSUB, int HD>
+struct Kv4Shape {
+  // (three buffers and twice the blocks: 512 tokens of four over 4096 115 us for 104, short blocks the same)
+  static constexpr int kRingBytes = 4 * (NSUB == 2 ? 128 : 64) * HD * 2;
+  static constexpr int kRawSlots = NSUB == 2 ? 24 : 12;
+  static constexpr int kSmemBytes = NSUB * TcShape<NSUB, HD>::kQTileBytes + kRingBytes + kRawSlots * kv4_block_bytes(HD) + 1024;
+};
+
 // ---------------------------------------------------------------- PTX wrappers
 __device__ __forceinline__ void tc_fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -194,11 +205,6 @@ template <int N>
 __device__ __forceinline__ void reg_fence(uint32_t (&r)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) asm volatile("" : "+r"(r[e])::"memory");
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 // 32 columns of this thread's TMEM lane into r[OFF .. OFF+32)
 template <int OFF, int N>
@@ -465,9 +471,10 @@ __device__ __noinline__ void merge_kv_splits_cta(const MergeArgs p, int nsp, int
   }
 }
 
-// KV4: the pool is held in 4 bits (kv4.cuh) and addressed by pages; the copying warps read codes, scales and biases and write
-// the tiles' elements, each scale * code + bias rounded once to T (one fma of two elements; a 16-bit pool holds the same
-// rounding).  Everything behind the tiles is as it is.
+// KV4: the pool is held in 4 bits and addressed by pages (Kv4Shape).  Every operand is f16 there whatever T is: three bits of
+// fraction more than bf16 where elements of K and V and the weights are rounded (in bf16, results are 0.0035 off 64 bits as a
+// norm; the rounding of the output alone is 0.0017).  What the pool holds lies within +-2^15, so f16 takes it (below 2^-14 to
+// 2^-25); a row of q is divided by a power of two, which comes back in the row's scale.
 template <typename T, int BN, int NSUB, int HD = 128, bool PAGED = false, bool KV4 = false>
 __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
                                   TcShape<NSUB, HD, PAGED>::kMinCtasForRegs)
@@ -477,6 +484,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   static_assert(BN == 64 || BN == 128, "key tile of 64 or 128 tokens");
   static_assert(NSUB == 2 || BN == 64, "the one-sub-tile shape has TMEM for 64-column score tiles only");
   using Shape = TcShape<NSUB, HD, PAGED>;
+  using M = typename std::conditional<KV4, __half, T>::type;       // type of the operands
+  constexpr bool CONVERT = !std::is_same<M, T>::value;
   constexpr int kTcQTileBytes = Shape::kQTileBytes;
   constexpr int CPR = HD / 8;                          // 16-byte chunks of a token row
   constexpr int BM = Shape::kBM, SUB = kTcSub;
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   constexpr int PROWS = NPROD / CPR;                    // token rows covered by one pass of the producers
   constexpr int LA = BN == 64 ? 2 : 1;        // key tiles S runs ahead of PV (= S buffers per sub-tile)
   constexpr int kTcKvTileBytes = BN * Shape::kRowBytes;
-  constexpr int kTcBufs = Shape::kRingBytes / kTcKvTileBytes;
+  constexpr int kTcBufs = (KV4 ? Kv4Shape<NSUB, HD>::kRingBytes : Shape::kRingBytes) / kTcKvTileBytes;
   constexpr uint32_t kOCol = NSUB * 128;      // first TMEM column of the O accumulators
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -495,7 +504,11 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
   __shared__ FoundItem found;
-  __shared__ int s_slots[(LA + 1) * BN];  // slot ids of the key tiles being copied / next to copy
+  constexpr int kRaw = KV4 ? Kv4Shape<NSUB, HD>::kRawSlots : 1;
+  __shared__ uint64_t s_raw_full[kRaw], s_raw_empty[kRaw];   // KV4: fetched blocks
+  __shared__ int s_raw_bad[kRaw];                             // their page is not in the pool
+  __shared__ float s_row_power[CONVERT ? BM : 1];             // what a row of q was divided by
+  __shared__ int s_slots[KV4 ? 1 : (LA + 1) * BN];  // slot ids of the key tiles being copied / next to copy
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5, lane = tid & 31;
@@ -517,7 +530,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   auto bar_pv = [&](int i, int sb) { return smem_u32(&bars.pv_done[i][sb]); };
   // Q arrives as TMA boxes when the caller could describe it (query heads per KV head a power
   // of two), else as 16-byte copies by the producer threads
-  const bool q_tma = PAGED && p.q_tma != 0;
+  const bool q_tma = (PAGED || KV4) && !CONVERT && p.q_tma != 0;
 
   if (warp == 1) {
     // a barrier per lane.  (PAGED: per copying warp its 32 lanes, their cp.async arrivals, and the arrival that
@@ -525,9 +538,13 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     auto init = [&](uint64_t* first, int n, int count) {
       if (lane < n) mbar_init(smem_u32(first + lane), count);
     };
-    init(&bars.q_full, 1, q_tma ? 1 : NPROD);
+    init(&bars.q_full, 1, q_tma ? 1 : CONVERT ? NSUB * SUB / 32 : NPROD);
     init(&bars.idx_sync, 1, NPROD);
-    init(bars.full, kTcBufs, PAGED ? (NPROD / 32) * 33 : NPROD);
+    init(bars.full, kTcBufs, PAGED ? (NPROD / 32) * 33 : KV4 ? BN / kKv4Rows : NPROD);
+    if constexpr (KV4) {
+      init(s_raw_full, kRaw, 1);
+      init(s_raw_empty, kRaw, 1);
+    }
     init(bars.empty, kTcBufs, 1);
     init(bars.stage, NSUB, SUB / 32);                  // one arrival per warp of the group
     init(&bars.s_full[0][0], 2 * NSUB, 1);
@@ -548,7 +565,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   } else {
     ItemCoord at;
     const bool have = find_item<kTcThreads>(p, static_cast<int>(blockIdx.x), BM, reinterpret_cast<int*>(smem_raw), at);
-    if (PAGED) fence_proxy_async_smem();   // (Q comes by bulk copies to where the item search had its counts)
+    if (PAGED || KV4) fence_proxy_async_smem();   // (Q comes by bulk copies to where the item search had its counts)
     if (tid == 0) {
       found.have = have;
       if (have) {
@@ -642,6 +659,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     auto load_q = [&]() {
     if (p.early) grid_dependency_wait();
     if (NSUB == 1 && ntiles == 0) return;      // (the epilogue's zeros are staged where Q would land)
+    if constexpr (CONVERT) return;             // (Q is the softmax warps')
     if (q_tma) {
       // Q: one box per sub-tile and 64-element column block.  The tensor map is
       // (head_dim, query heads, tokens) with a box of 64 x G x 128/G, so the rows land in
@@ -803,48 +821,119 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
         }
       }
     } else if constexpr (KV4) {
-      constexpr int PPR = HD / 32;                     // 16-byte pieces (four words) of a row's codes
-      constexpr int G = HD / kKv4Group;
-      const int32_t* __restrict__ pages = p.page_indices + sq.kv_begin;
-      const int64_t num_blocks = p.num_slots / kKv4Rows;
-      const int page_blocks = p.page_size / kKv4Rows;
+      constexpr int PPT = BN / kKv4Rows;               // blocks of a tile
+      constexpr int BLK = kv4_block_bytes(HD), G = HD / kKv4Group;
+      constexpr int DW = Shape::kWarps - kTcProducerWarp0 - 1;     // warps that write tiles
+      const uint32_t raw = ring + kTcBufs * kTcKvTileBytes;
+      unsigned char* const raw_at = smem_raw + (raw - smem_u32(smem_raw));
       load_q();
-      auto produce = [&](int seq, const unsigned char* pool, int tile) {
-        const int bf = seq % kTcBufs;
-        alive = mbar_wait_warp(bar_empty(bf), ((seq / kTcBufs) & 1) ^ 1, abort_flag);
-        if (!alive) return;
-        unsigned char* dst = smem_raw + (ring - smem_u32(smem_raw)) + bf * kTcKvTileBytes;
-        for (int e = ptid; e < BN * PPR; e += NPROD) {
-          const int row = e / PPR, piece = e % PPR;
-          const int t = kv_lo + tile * BN + row;
-          uint32_t words[4] = {0u, 0u, 0u, 0u}, pairs[G];
+      // Tiles in the order of the ring: `seq`, K or V, tile; their blocks are numbered through (`at`).
+      auto each_tile = [&](auto&& f) {
+        int at = 0;
+        for (int t = 0; t < LA && t < ntiles && alive; ++t, at += PPT) f(ring_seq_k<LA>(t), false, t, at);
+#pragma unroll 1
+        for (int j = 0; j < ntiles && alive; ++j) {
+          f(ring_seq_v<LA>(j), true, j, at);
+          at += PPT;
+          if (!alive || j + LA >= ntiles) continue;
+          f(ring_seq_k<LA>(j + LA), false, j + LA, at);
+          at += PPT;
+        }
+        return at;
+      };
+      if (warp == kTcProducerWarp0) {
+        // ---- the fetching warp: lane i has block i of a tile: its place in the pool, -1: a page that is not in it, -2: behind the keys
+        const int32_t* __restrict__ pages = p.page_indices + sq.kv_begin;
+        const int num_blocks = static_cast<int>(p.num_slots / kKv4Rows), page_blocks = p.page_size / kKv4Rows;
+        auto block_of = [&](int tile) -> int {
+          const int t = kv_lo + tile * BN + lane * kKv4Rows;
+          if (lane >= PPT || tile >= ntiles || t >= kv_hi_load) return -2;
+          const int page = divide_by(t, p.page_recip);
+          const int64_t block = static_cast<int64_t>(__ldg(pages + page)) * page_blocks + (t - page * p.page_size) / kKv4Rows;
+          if (block >= 0 && block < num_blocks) return static_cast<int>(block);
+          if (p.status) atomicOr(p.status, 2);
+          return -1;
+        };
+        int window[LA + 2];        // blocks of tiles j .. j + LA + 1
 #pragma unroll
-          for (int g = 0; g < G; ++g) pairs[g] = 0u;
-          if (t < kv_hi_load) {
-            const int page = divide_by(t, p.page_recip);
-            const int64_t block = static_cast<int64_t>(__ldg(pages + page)) * page_blocks + (t - page * p.page_size) / kKv4Rows;
-            if (block >= 0 && block < num_blocks) {
-              const unsigned char* at = pool + (block * p.hkv + h) * kv4_block_bytes(HD);
-              read_words<16>(words, at + (t % kKv4Rows) * (HD / 2) + piece * 16);
-              read_words<G * 4>(pairs, at + kv4_pairs_at(HD) + (t % kKv4Rows) * (G * 4));
-            } else if (p.status) {
-              atomicOr(p.status, 2);
+        for (int t = 0; t <= LA + 1; ++t) window[t] = block_of(t);
+        const int at_end = each_tile([&](int, bool is_v, int tile, int at) {
+          // (K runs LA tiles ahead of V, but for the first LA of them)
+          int block = window[is_v ? 0 : LA];
+          if (!is_v && at < LA * PPT) block = tile == 0 ? window[0] : window[1];
+          bool ok = true;
+          if (lane < PPT) {
+            const int n = at + lane, slot = n % kRaw;
+            ok = mbar_wait(smem_u32(&s_raw_empty[slot]), ((n / kRaw) & 1) ^ 1, abort_flag);
+            if (ok) {
+              const uint32_t bar = smem_u32(&s_raw_full[slot]);
+              s_raw_bad[slot] = block == -1;
+              if (block >= 0) {
+                mbar_arrive_expect_tx(bar, BLK);
+                bulk_load(raw + slot * BLK, (is_v ? vbase : kbase) + (static_cast<int64_t>(block) * p.hkv + h) * BLK, BLK, bar);
+              } else {
+                mbar_arrive(bar);
+              }
             }
           }
+          alive = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+          if (!is_v && at < LA * PPT) return;
+          if (is_v && tile + LA < ntiles) return;       // (its K comes next, with this window)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int g = w % G, r8 = piece * (4 / G) + w / G;
-            *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(row, g * 8 + r8)) = kv4_values<T>(words[w], pairs[g]);
-          }
+          for (int t = 0; t <= LA; ++t) window[t] = window[t + 1];
+          window[LA + 1] = block_of(tile + (is_v ? 0 : -LA) + LA + 2);
+        });
+        if (!alive) {
+          // gave up: the copies still in flight land before the CTA's shared memory goes away; bounded
+          const long long t0 = clock64();
+          for (int n = max(0, at_end - kRaw); n < at_end + PPT; ++n)
+            while (!mbar_try_wait(smem_u32(&s_raw_full[n % kRaw]), (n / kRaw) & 1) && clock64() - t0 < 2000000LL) {
+            }
         }
-        fence_proxy_async_smem();
-        mbar_arrive(bar_full(bf));
-      };
-      for (int t = 0; t < LA && t < ntiles && alive; ++t) produce(ring_seq_k<LA>(t), kbase, t);
+      } else {
+        // ---- the writing warps: lane l takes piece l % PPR (16 bytes, four words) of rows l / PPR, ...
+        constexpr int PPR = HD / 32, RPP = 32 / PPR;   // rows a pass
+        const int dw = warp - kTcProducerWarp0 - 1;
+        const int piece = lane % PPR, rsub = lane / PPR;
+        each_tile([&](int seq, bool is_v, int tile, int at) {
+          const int bf = seq % kTcBufs;
+          int blk = (dw - at % DW + DW) % DW;
+          if (blk >= PPT) return;
+          alive = mbar_wait_warp(bar_empty(bf), ((seq / kTcBufs) & 1) ^ 1, abort_flag);
+          unsigned char* const dst = smem_raw + (ring - smem_u32(smem_raw)) + bf * kTcKvTileBytes;
 #pragma unroll 1
-      for (int j = 0; j < ntiles && alive; ++j) {
-        produce(ring_seq_v<LA>(j), vbase, j);
-        if (alive && j + LA < ntiles) produce(ring_seq_k<LA>(j + LA), kbase, j + LA);
+          for (; blk < PPT && alive; blk += DW) {
+            const int n = at + blk, slot = n % kRaw;
+            alive = mbar_wait_warp(smem_u32(&s_raw_full[slot]), (n / kRaw) & 1, abort_flag);
+            if (!alive) break;
+            const unsigned char* const src = raw_at + slot * BLK;
+            const int left = s_raw_bad[slot] ? 0 : kv_hi_load - (kv_lo + tile * BN + blk * kKv4Rows);   // rows with a key
+            uint32_t words[kKv4Rows / RPP][4], pairs[kKv4Rows / RPP][G];
+#pragma unroll
+            for (int i = 0; i < kKv4Rows / RPP; ++i) {
+              const int row = i * RPP + rsub;
+              read_words<16>(words[i], src + row * (HD / 2) + piece * 16);
+              read_words<G * 4>(pairs[i], src + kv4_pairs_at(HD) + row * (G * 4));
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_raw_empty[slot]));
+#pragma unroll
+            for (int i = 0; i < kKv4Rows / RPP; ++i) {
+              const int row = i * RPP + rsub;
+              const bool in = row < left;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const int g = w % G, r8 = piece * (4 / G) + w / G;
+                uint4 x = kv4_values<M>(words[i][w], same_pair(T{}, M{}, pairs[i][g]));
+                if (!in) x = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(blk * kKv4Rows + row, g * 8 + r8)) = x;
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_full(bf));
+          }
+        });
       }
     } else {
       constexpr int RPT = (BN + PROWS - 1) / PROWS;  // passes over a tile
@@ -916,8 +1005,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   } else if (warp == kMmaWarp) {
     // =========================================================== MMA issuer
     {
-    const uint32_t idesc_s = idesc_m128<T>(BN, 0);
-    const uint32_t idesc_pv = idesc_m128<T>(HD, 1);
+    const uint32_t idesc_s = idesc_m128<M>(BN, 0);
+    const uint32_t idesc_pv = idesc_m128<M>(HD, 1);
     bool alive = true;
     // Descriptors are computed by the whole (converged) warp so that they stay
     // warp-uniform values; only the elected lane issues the instructions.
@@ -1031,13 +1120,67 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     float m_ref = -INFINITY, l = 0.f;
     bool alive = true;
     const bool sc_neg = !(p.scale_log2 > 0.f);
-    const float sc = sc_neg ? 1.f : p.scale_log2;
+    float row_scale = p.scale_log2;
+    if constexpr (CONVERT) {
+      // Q as f16, a warp its own 32 rows, CPR lanes a row, RU rows in flight a lane.  (By the copying warps, in front of their
+      // first tile: four chunks of 300 to 512 tokens over up to 4096 132 us for 104.)
+      constexpr int RP = 32 / CPR, RU = 8;              // rows a pass; passes in flight
+      const uint32_t mask = CPR == 32 ? 0xffffffffu : (lane & 16) ? 0xffff0000u : 0x0000ffffu;
+      const int chunk = lane % CPR;
+      unsigned char* const q_at = smem_raw + (q_smem - smem_u32(smem_raw)) + i * kTcQTileBytes;
+      if (ntiles > 0) {
+#pragma unroll 1
+        for (int b = 0; b < 32; b += RP * RU) {
+          uint4 x[RU];
+#pragma unroll
+          for (int u = 0; u < RU; ++u) {
+            const int at = i * SUB + (warp & 3) * 32 + b + u * RP + lane / CPR;
+            x[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (at < rows_valid) {
+              const int t = over_group(pk0 + at), g = pk0 + at - t * G;
+              x[u] = *reinterpret_cast<const uint4*>(
+                  static_cast<const T*>(p.q) +
+                  (static_cast<int64_t>(sq.q_begin + t) * p.hq + static_cast<int64_t>(h) * G + g) * HD + chunk * 8);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < RU; ++u) {
+            const int at = (warp & 3) * 32 + b + u * RP + lane / CPR;
+            uint32_t* const w = reinterpret_cast<uint32_t*>(&x[u]);
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, max(w[e] >> 16 & 0x7fffu, w[e] & 0x7fffu));
+#pragma unroll
+            for (int o = 1; o < CPR; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+            const float power = row_power(T{}, top), inv = 1.f / power;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack_pair(T{}, w[e]);
+              w[e] = MmaOp<M>::pack(f.x * inv, f.y * inv);
+            }
+            *reinterpret_cast<uint4*>(q_at + tc_tile_offset<128>(at, chunk)) = x[u];
+            if (chunk == 0) s_row_power[i * SUB + at] = power;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        row_scale *= s_row_power[row];
+      }
+      if (lane == 0) mbar_arrive(bar_q);
+    }
+    const float sc = sc_neg ? 1.f : row_scale;
 
 #pragma unroll 1
     for (int j = 0; j < my_tiles; ++j) {
       const int sb = j % LA;
       alive = mbar_wait_warp(bar_sf(i, sb), (j / LA) & 1, abort_flag);
       if (!alive) break;
+      if constexpr (KV4) {
+        if (i * SUB + (warp & 3) * 32 >= rows_valid) {     // (a warp whose rows are nobody's: what stands there as P stays there)
+          if (lane == 0) mbar_arrive(bar_pf(i, sb));
+          continue;
+        }
+      }
       tc_fence_after();
 #ifdef MSGL_TRACE
       if (tid == 0 && j == 0) MSGL_TR(5, clock64());   // first scores ready
@@ -1057,7 +1200,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       reg_fence(v);
       if (sc_neg) {  // a non-positive scale: fold it into the scores so that max() commutes
 #pragma unroll
-        for (int e = 0; e < BN; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * p.scale_log2);
+        for (int e = 0; e < BN; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * row_scale);
       }
       if (need_mask) {
 #pragma unroll
@@ -1119,7 +1262,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
           const float p1 = fast_exp2(x1);
           if (e & 2) lb = add_f32x2(lb, pack_f32x2(p0, p1));
           else la = add_f32x2(la, pack_f32x2(p0, p1));
-          pk16[e >> 1] = MmaOp<T>::pack(p0, p1);
+          pk16[e >> 1] = MmaOp<M>::pack(p0, p1);
         }
         tmem_st16(s_tm + sb * BN + c * 16, pk16);  // P columns [16c, 16c+16) of this S buffer
       }
@@ -1327,7 +1470,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       const MergeArgs ma{p.part_o, p.part_ml, p.out, p.gate, p.hq, p.group, p.group_recip};
       // (rows x 2 splits in flight per lane: what the register cap of the main kernel holds)
       constexpr int kMergeRows = (!Shape::kRebalanceRegs && HD == 128) ? 4 : 2;
-      constexpr int kFree = Shape::kSmemBytes - 1024;       // Q and the ring
+      constexpr int kFree = (KV4 ? Kv4Shape<NSUB, HD>::kSmemBytes : Shape::kSmemBytes) - 1024;       // Q and the rings
       if (nsp * (HD * 4 + 8) * 16 <= kFree)    // (else: less than 16 rows at a time)
         merge_kv_splits_cta<T, HD, kMergers, BM>(ma, nsp, slot0, p.hkv, rows_valid, pk0, sq.q_begin, h,
                                                  smem_raw + (smem0 - smem_u32(smem_raw)), kFree);
