@@ -542,15 +542,21 @@ int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const voi
 /*
  * msgl_paged_prefill_attention_p16 over this pool: masks, arguments and zeros of rows without a key as there.
  * max_len_extend is the longest query block, or more (rows of a longer one may stay unwritten, and 2 is reported).
+ * Long prefills expand their pages into f16 first, into `expanded`, memory of the call's own of
+ * msgl_prefill_expanded_bytes_q4 bytes (0 where a call does not), which can go elsewhere once its launches are queued
+ * (of a captured call: once its graph is replayed no more); without it (NULL) the attention kernel expands as it goes.
  */
+size_t msgl_prefill_expanded_bytes_q4(int batch, int total_q, int64_t total_pages, int page_size, int num_q_heads,
+                                      int num_kv_heads, int head_dim, int dtype, int max_len_extend,
+                                      int is_cross_attention, int sliding_window_size);
 size_t msgl_prefill_workspace_bytes_q4(int batch, int total_q, int64_t total_pages, int page_size, int num_q_heads,
                                        int num_kv_heads, int head_dim, int max_len_extend, int sliding_window_size);
 int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const void* v_cache,
                                     const int32_t* qo_indptr, const int32_t* page_indptr,
                                     const int32_t* page_indices, const int32_t* kv_lens, const int32_t* prefix_lens,
-                                    const void* gate, void* out, void* workspace, size_t workspace_bytes, int batch,
-                                    int total_q, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_slots,
-                                    int dtype, float sm_scale, int max_len_extend, int is_cross_attention,
+                                    const void* gate, void* out, void* workspace, size_t workspace_bytes,
+                                    void* expanded, size_t expanded_bytes, int batch, int total_q, int num_q_heads,
+                                    int num_kv_heads, int head_dim, int64_t num_slots, int dtype, float sm_scale, int max_len_extend, int is_cross_attention,
                                     int sliding_window_size, int page_size, int64_t total_pages, void* stream);
 
 #ifdef __cplusplus

@@ -80,8 +80,9 @@ SIGNATURES = {
     "msgl_paged_decode_attention_q4": (
         _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i64, _i, _f, _i, _i64, _vp]),
     "msgl_prefill_workspace_bytes_q4": (_sz, [_i, _i, _i64, _i, _i, _i, _i, _i, _i]),
+    "msgl_prefill_expanded_bytes_q4": (_sz, [_i, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _i]),
     "msgl_paged_prefill_attention_q4": (
-        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i64, _i, _f, _i, _i, _i, _i,
+        _i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _i, _i, _i, _i, _i, _i64, _i, _f, _i, _i, _i, _i,
              _i64, _vp]),
     "msgl_fast_compare_key": (_i64, [_vp, _vp, _i64, _i64, _i]),
     "msgl_qk_norm_rope_store": (

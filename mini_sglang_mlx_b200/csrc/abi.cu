@@ -105,18 +105,13 @@ EncodeTiledFn tensor_map_encoder() {
   return fn;
 }
 
+}  // namespace
+
 // Maps over a pool (num_slots rows of num_kv_heads * head_dim 16-bit elements).  A copy lands in shared memory with the
 // 128-byte swizzle, i.e. in the layout the tensor-core descriptors of the kernels expect; rows outside the pool read as
 // zeros.  The maps are kept per thread, one per hash of the pool's address and the form: a model's layers each have two
 // pools and go through them in turn.
-enum class PoolBox {
-  kPage,   // 2-D, 16 token rows x 64 elements (128 bytes) of one head
-  kRow,    // 2-D, one row of those, for tile::gather4
-  kHead,   // 3-D (64 elements, slots, blocks of 64 elements of a row): 16 token rows x all head_dim elements of one head, a block
-           // of columns after the other, as the decode kernel's tiles lie in shared memory.  (A copy instruction costs
-           // its warp 67 cycles whatever its size: one per tile instead of two or four.)
-};
-bool make_pool_map(CUtensorMap* out, PoolBox form, const void* base, int64_t num_slots, int num_kv_heads, int head_dim,
+bool msgl_host::make_pool_map(CUtensorMap* out, PoolBox form, const void* base, int64_t num_slots, int num_kv_heads, int head_dim,
                    int dtype) {
   struct Cached {
     const void* base;
@@ -154,8 +149,6 @@ bool make_pool_map(CUtensorMap* out, PoolBox form, const void* base, int64_t num
   return true;
 }
 
-}  // namespace
-
 // 3-D map over the query tensor (tokens, query heads, head_dim): a box is 64 elements x the
 // `group` heads of one KV head x 128 / group tokens, i.e. the 128 packed rows of a query
 // sub-tile in the order the kernel numbers them.  Needs a group that divides 128.
@@ -179,10 +172,8 @@ bool msgl_host::make_query_tensor_map(CUtensorMap* out, const void* q, int total
   return r == CUDA_SUCCESS;
 }
 
-namespace {
-
 // 2-D map over the query rows (tokens x heads, head_dim) for tile::gather4: a box is one row x 64 elements.
-bool make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int head_dim, int dtype) {
+bool msgl_host::make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int head_dim, int dtype) {
   EncodeTiledFn enc = tensor_map_encoder();
   const int64_t rows = static_cast<int64_t>(total_q) * num_q_heads;
   if (!enc || rows <= 0 || rows >= (1ll << 31) || reinterpret_cast<uintptr_t>(q) % 16 != 0) return false;
@@ -196,8 +187,6 @@ bool make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-}  // namespace
-
 // Query blocks that fill at most one 128-row sub-tile (verify, draft blocks) run the
 // one-sub-tile shape (64-token key tiles, two CTAs per SM); longer chunks the two-sub-tile
 // shape with 128-token key tiles.  head_dim 256 always runs the one-sub-tile shape (its
@@ -205,8 +194,6 @@ bool make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_
 bool msgl_host::prefill_short_q(int max_len_extend, int group, int head_dim) {
   return head_dim == 256 || static_cast<int64_t>(max_len_extend) * group <= msgl::kTcSub;
 }
-
-namespace {
 
 // Pairs of CTAs (prefill_pair.cuh) serve query blocks of more than one 128-row tile whose key range is
 // not split: head_dim 256 always, head_dim 128 where they are the faster of two forms.  A pair takes
@@ -222,7 +209,7 @@ namespace {
 // copy of its own, and the pair has four copying warps and gathers of four rows against seven copying
 // warps (two layers of 2000-token prompts over 8000 cached tokens: 1168 us against 1109; with gathers for
 // K and V alike 1450).
-bool prefill_pairs(int batch, int total_q, int64_t total_kv, int group, int num_kv_heads, int head_dim,
+bool msgl_host::prefill_pairs(int batch, int total_q, int64_t total_kv, int group, int num_kv_heads, int head_dim,
                    int max_len_extend, bool cross, int window, int kv_chunk, bool paged, int sms) {
   if (kv_chunk != 0 || static_cast<int64_t>(max_len_extend) * group <= msgl::kTcSub) return false;
   if (head_dim == 256) return true;
@@ -240,8 +227,6 @@ bool prefill_pairs(int batch, int total_q, int64_t total_kv, int group, int num_
   };
   return waves(sms / 2) * (17. + 1.9 * key_tiles) < waves(sms) * (20. + 4. * key_tiles);
 }
-
-}  // namespace
 
 PrefillPlan msgl_host::plan_prefill(int batch, int total_q, int64_t total_kv, int hq, int hkv, int head_dim,
                          int max_len_extend, int window, int sms) {

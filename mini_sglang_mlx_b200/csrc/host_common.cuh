@@ -74,6 +74,18 @@ cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t
   return launch_clusters(1, kernel, grid, block, smem, s, args...);
 }
 
+// Tensor maps over a pool, see make_pool_map.
+enum class PoolBox {
+  kPage,   // 2-D, 16 token rows x 64 elements (128 bytes) of one head
+  kRow,    // 2-D, one row of those, for tile::gather4
+  kHead,   // 3-D (64 elements, slots, blocks of 64 elements of a row): 16 token rows x all head_dim elements of one head, a block
+           // of columns after the other, as the decode kernel's tiles lie in shared memory.  (A copy instruction costs
+           // its warp 67 cycles whatever its size: one per tile instead of two or four.)
+};
+bool make_pool_map(CUtensorMap* out, PoolBox form, const void* base, int64_t num_slots, int num_kv_heads, int head_dim,
+                   int dtype);
+// Tensor map over the query rows for tile::gather4.
+bool make_query_row_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int head_dim, int dtype);
 // Tensor map over the query tensor whose box is the 128 packed rows of a query sub-tile; false where
 // the group does not divide 128.
 bool make_query_tensor_map(CUtensorMap* out, const void* q, int total_q, int num_q_heads, int group,
@@ -86,6 +98,8 @@ struct PrefillPlan {
   size_t part_o_bytes, part_ml_bytes, plan_bytes;
   bool fused_merge;    // the CTA that arrives last at a unit merges it (else: a second launch)
 };
+bool prefill_pairs(int batch, int total_q, int64_t total_kv, int group, int num_kv_heads, int head_dim,
+                   int max_len_extend, bool cross, int window, int kv_chunk, bool paged, int sms);
 bool prefill_short_q(int max_len_extend, int group, int head_dim);
 PrefillPlan plan_prefill(int batch, int total_q, int64_t total_kv, int hq, int hkv, int head_dim,
                          int max_len_extend, int window, int sms);

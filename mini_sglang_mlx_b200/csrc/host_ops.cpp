@@ -626,6 +626,7 @@ PyObject* prefill_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
             ps = static_cast<int>(page_size);
   int64_t stream;
   Scratch ws;
+  Pages expanded;
   if (!stream_of(a[14], s.device, &stream) ||
       !scratch_for(s.device, stream, kPrefill,
                    msgl_prefill_workspace_bytes_q4(batch, total_q, pages.numel(), ps, hq, s.hkv, s.d,
@@ -633,10 +634,15 @@ PyObject* prefill_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    &ws))
     return nullptr;
   Tensor out = empty_like_rows(q);
+  if (!pages_for(s.device, stream,
+                 msgl_prefill_expanded_bytes_q4(batch, total_q, pages.numel(), ps, hq, s.hkv, s.d, s.dtype,
+                                                static_cast<int>(max_ext), cross, static_cast<int>(window)),
+                 &expanded))
+    return nullptr;
   const int rc = in_turn(ws, [&] {
     return msgl_paged_prefill_attention_q4(
       q.data_ptr(), kc.data_ptr(), vc.data_ptr(), i32(qo), i32(indptr), i32(pages), i32(lens), i32(prefix), gate,
-      out.data_ptr(), ws.ptr, ws.bytes, batch, total_q, hq, s.hkv, s.d, s.num_slots, s.dtype, static_cast<float>(scale),
+      out.data_ptr(), ws.ptr, ws.bytes, expanded.ptr, expanded.bytes, batch, total_q, hq, s.hkv, s.d, s.num_slots, s.dtype, static_cast<float>(scale),
       static_cast<int>(max_ext), cross, static_cast<int>(window), ps, pages.numel(), reinterpret_cast<void*>(stream));
   });
   return rc ? raise_status(rc) : THPVariable_Wrap(std::move(out));

@@ -8,6 +8,7 @@
 #include "decode_q4.cuh"
 #include "host_common.cuh"
 #include "kv4_project.cuh"
+#include "prefill_pair.cuh"
 #include "prefill_tc.cuh"
 
 using namespace msgl_host;
@@ -111,6 +112,35 @@ bool q4_block_form(int max_len_extend, int group) {
 int64_t q4_block_bound(int batch, int64_t total_pages, int page_size, int max_len_extend, int window) {
   const int64_t all = total_pages * page_size / msgl::kKv4Rows;
   return window > 0 ? std::min<int64_t>(all, batch * ((static_cast<int64_t>(window) + max_len_extend) / msgl::kKv4Rows + 2)) : all;
+}
+
+// Long prefills lay their pages out first (kv4_expand_kernel) and run the pairs of CTAs, where those are the form for pages of 16
+// bits and the attention takes several times what the copies do, by a rough model of both.  Sixty shapes (one to 24 sequences,
+// 25 to 25650 new tokens, 176 to 180672 of keys, windows among them), time of the one-CTA form over time with expanded pages: at
+// head_dim 128 where pairs are the form and the ratio is above 3, 1.03 to 1.21, below it 0.50 to 1.39, in the mean 0.93.  At head_dim
+// 256 the one-CTA form has 128 rows and one CTA per SM, and 1.00 to 2.84 on all whose key range is not split and whose ratio is above
+// 0.25.
+constexpr size_t kQ4ExpandedMax = 256u << 20;     // bytes of pages
+constexpr double kQ4ExpandWorth128 = 3.0, kQ4ExpandWorth256 = 0.25;
+bool q4_expands(int batch, int total_q, int64_t total_kv, int hq, int hkv, int head_dim, int max_len_extend, bool cross,
+                int window, int sms) {
+  if (total_kv <= 0 || static_cast<size_t>(total_kv) * hkv * head_dim * 4 > kQ4ExpandedMax) return false;
+  const PrefillPlan pl = plan_prefill(batch, total_q, total_kv, hq, hkv, head_dim, max_len_extend, window, sms);
+  if (!prefill_pairs(batch, total_q, total_kv, hq / hkv, hkv, head_dim, max_len_extend, cross, window, pl.kv_chunk, true, sms))
+    return false;
+  double keys = std::max(1., static_cast<double>(total_kv) / batch - (cross ? 0. : 0.5 * total_q / batch));
+  if (window > 0) keys = std::min<double>(keys, window + max_len_extend);
+  const double attend_us = 4. * head_dim * hq * static_cast<double>(total_q) * keys / 1e9;             // at 1 PFLOP/s
+  const double copy_us = 5. + (static_cast<double>(total_kv) * hkv * 5.2 + static_cast<double>(total_q) * hq * 4.) * head_dim / 4e6;
+  return attend_us > (head_dim == 256 ? kQ4ExpandWorth256 : kQ4ExpandWorth128) * copy_us;
+}
+size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+// K rows, V rows, page ids, q rows and their powers.
+size_t q4_expanded_bytes(int total_q, int64_t total_kv, int64_t total_pages, int hq, int hkv, int head_dim, int dtype) {
+  const size_t rows = rounded(static_cast<size_t>(total_kv) * hkv * head_dim * 2);
+  const size_t q_rows = static_cast<size_t>(total_q) * hq;
+  return 2 * rows + rounded(total_pages * sizeof(int32_t)) +
+         (dtype == MSGL_DTYPE_BF16 ? rounded(q_rows * head_dim * 2) + rounded(q_rows * sizeof(float)) : 0);
 }
 
 }  // namespace
@@ -315,10 +345,25 @@ size_t msgl_prefill_workspace_bytes_q4(int batch, int total_q, int64_t total_pag
   return kStatusBytes + pl.ticket_bytes + pl.part_bytes;
 }
 
+size_t msgl_prefill_expanded_bytes_q4(int batch, int total_q, int64_t total_pages, int page_size, int num_q_heads,
+                                      int num_kv_heads, int head_dim, int dtype, int max_len_extend, int is_cross_attention,
+                                      int sliding_window_size) {
+  if (batch <= 0 || batch > 65535 || total_q <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+      (head_dim != 128 && head_dim != 256) || total_pages < 0 || page_size <= 0 || total_pages >= (1ll << 31) / page_size)
+    return 0;
+  max_len_extend = std::max(1, max_len_extend);
+  const int sms = sm_count_cached();
+  const int64_t total_kv = total_pages * page_size;
+  return q4_expands(batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, max_len_extend, is_cross_attention != 0,
+                    sliding_window_size, sms > 0 ? sms : 148)
+             ? q4_expanded_bytes(total_q, total_kv, total_pages, num_q_heads, num_kv_heads, head_dim, dtype)
+             : 0;
+}
+
 int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const void* v_cache, const int32_t* qo_indptr,
                                     const int32_t* page_indptr, const int32_t* page_indices, const int32_t* kv_lens,
                                     const int32_t* prefix_lens, const void* gate, void* out, void* workspace,
-                                    size_t workspace_bytes, int batch, int total_q, int num_q_heads, int num_kv_heads,
+                                    size_t workspace_bytes, void* expanded, size_t expanded_bytes, int batch, int total_q, int num_q_heads, int num_kv_heads,
                                     int head_dim, int64_t num_slots, int dtype, float sm_scale, int max_len_extend,
                                     int is_cross_attention, int sliding_window_size, int page_size, int64_t total_pages,
                                     void* stream) {
@@ -341,7 +386,7 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
       (total_pages > 0 && !page_indices))
     return fail(MSGL_BAD_ARG, std::string(op) + "null tensor pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(gate) ||
-      !aligned16(workspace))
+      !aligned16(workspace) || !aligned16(expanded))
     return fail(MSGL_BAD_ARG, std::string(op) + "q, the pools, out, gate and the workspace must be 16-byte aligned");
   const int sms = sm_count_cached();
   if (sms <= 0) return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot query the device");
@@ -410,6 +455,73 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
   p.page_recip = msgl::reciprocal(page_size);
   p.chunk_recip = msgl::reciprocal(p.kv_chunk);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t total_kv = total_pages * page_size;
+  if (expanded != nullptr && batch <= 65535 &&
+      q4_expands(batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, max_len_extend, is_cross_attention != 0,
+                 sliding_window_size, sms) &&
+      expanded_bytes >= q4_expanded_bytes(total_q, total_kv, total_pages, num_q_heads, num_kv_heads, head_dim, dtype)) {
+    const int64_t pairs =
+        msgl::prefill_item_bound(batch, total_q, total_kv, p.group, 256, max_len_extend, 0) * num_kv_heads;
+    if (pairs * 2 > 0x7fffffffLL) return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
+    const size_t rows = rounded(static_cast<size_t>(total_kv) * num_kv_heads * head_dim * 2);
+    unsigned char* at = static_cast<unsigned char*>(expanded);
+    msgl::Kv4ExpandParams x{};
+    x.k_pool = static_cast<const unsigned char*>(k_cache);
+    x.v_pool = static_cast<const unsigned char*>(v_cache);
+    x.page_indices = page_indices;
+    x.k_rows = reinterpret_cast<__half*>(at);
+    x.v_rows = reinterpret_cast<__half*>(at + rows);
+    x.pages = reinterpret_cast<int32_t*>(at + 2 * rows);
+    at += 2 * rows + rounded(total_pages * sizeof(int32_t));
+    x.total_pages = static_cast<int>(total_pages);
+    x.page_blocks = page_size / msgl::kKv4Rows;
+    x.hkv = num_kv_heads;
+    x.num_blocks = static_cast<int>(num_slots / msgl::kKv4Rows);
+    x.status = p.status;
+    const bool convert = dtype == MSGL_DTYPE_BF16;
+    if (convert) {
+      x.num_q_rows = static_cast<int64_t>(total_q) * num_q_heads;
+      x.q = q;
+      x.q_rows = reinterpret_cast<__half*>(at);
+      x.q_power = reinterpret_cast<float*>(at + rounded(x.num_q_rows * head_dim * 2));
+    }
+    CUtensorMap tm_k, tm_v, tg_k, tg_v, tm_rows;
+    const void* q16 = convert ? x.q_rows : q;
+    if (!make_pool_map(&tm_k, PoolBox::kPage, x.k_rows, total_kv, num_kv_heads, head_dim, MSGL_DTYPE_F16) ||
+        !make_pool_map(&tm_v, PoolBox::kPage, x.v_rows, total_kv, num_kv_heads, head_dim, MSGL_DTYPE_F16) ||
+        !make_pool_map(&tg_k, PoolBox::kRow, x.k_rows, total_kv, num_kv_heads, head_dim, MSGL_DTYPE_F16) ||
+        !make_pool_map(&tg_v, PoolBox::kRow, x.v_rows, total_kv, num_kv_heads, head_dim, MSGL_DTYPE_F16))
+      return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot build the tensor maps of the pages");
+    p.q_tma = make_query_tensor_map(&tm_rows, q16, total_q, num_q_heads, p.group, head_dim, MSGL_DTYPE_F16) ? 1 : 0;
+    if (!p.q_tma && !make_query_row_map(&tm_rows, q16, total_q, num_q_heads, head_dim, MSGL_DTYPE_F16))
+      return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot build the tensor map of the queries");
+    p.q = q16;
+    p.q_power = x.q_power;
+    p.k_cache = x.k_rows;
+    p.v_cache = x.v_rows;
+    p.page_indices = x.pages;
+    p.num_slots = total_kv;
+    p.kv_chunk = 0;
+    p.chunk_recip = 0;
+    auto run = [&](auto expand, auto kernel, int threads, int smem) -> cudaError_t {
+      cudaError_t err = launch_dependent(expand, dim3(static_cast<unsigned>(sms * 8)), dim3(256), 0, s, x);
+      if (err != cudaSuccess) return err;
+      if ((err = allow_smem(kernel, smem)) != cudaSuccess) return err;
+      return launch_clusters(2, kernel, dim3(static_cast<unsigned>(pairs * 2)), dim3(threads), smem, s, p, tm_k, tm_v, tg_k, tg_v,
+                             tm_rows);
+    };
+    auto of = [&](auto tag) -> cudaError_t {
+      using T = decltype(tag);
+      using P128 = msgl::PairShape<128, true>;
+      using P256 = msgl::PairShape<256, true>;
+      return head_dim == 128 ? run(msgl::kv4_expand_kernel<T, 128>, msgl::prefill_pair_kernel<T, 128, true, __half>,
+                                   P128::kThreads, P128::kSmemBytes)
+                             : run(msgl::kv4_expand_kernel<T, 256>, msgl::prefill_pair_kernel<T, 256, true, __half>,
+                                   P256::kThreads, P256::kSmemBytes);
+    };
+    const cudaError_t e = convert ? of(__nv_bfloat16{}) : of(__half{});
+    return e == cudaSuccess ? MSGL_OK : cuda_fail("paged_prefill_attention_q4", e);
+  }
   CUtensorMap none, tm_q;
   std::memset(&none, 0, sizeof(none));
   std::memset(&tm_q, 0, sizeof(tm_q));

@@ -302,4 +302,83 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
   }
 }
 
+// ---------------------------------------------------------------- pages laid out for the pairs of CTAs
+// A long prefill reads a key once for every 256 query rows, and to expand its codes each time is what bounds the kernel that does
+// (one CTA; 4096 tokens over 16384 1425 us).  Expanded once into f16 pages, one per entry of the index list and
+// in its order, they come by TMA and pairs of CTAs share them.  q goes with them, as f16 over a power of two per row (bf16 only).
+// Bound by memory: 2.6 bytes an element of the pool, 4 of q.
+struct Kv4ExpandParams {
+  const unsigned char *k_pool, *v_pool;
+  const int32_t* page_indices;
+  __half *k_rows, *v_rows;      // (total_pages * page_size, hkv, head_dim)
+  int32_t* pages;               // (total_pages): 0, 1, ...
+  const void* q;                // (q_rows, head_dim), or null
+  __half* q_rows;
+  float* q_power;
+  int total_pages, page_blocks, hkv, num_blocks;
+  int64_t num_q_rows;
+  int* status;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4ExpandParams p) {
+  constexpr int CH = HD / 8, G = HD / kKv4Group, RPP = 32 / CH;      // chunks of a row; rows a pass of a warp
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int32_t* ids = after_wait(p.page_indices);
+  const unsigned char* pools[2] = {after_wait(p.k_pool), after_wait(p.v_pool)};
+  const T* q = after_wait(static_cast<const T*>(p.q));
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * 8, first = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int c = lane % CH, rsub = lane / CH;
+  const int word_at = ((c % 8) * G + c / 8) * 4, pair_at = kv4_pairs_at(HD) + c / 8 * 4;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < p.total_pages; i += gridDim.x * 256ll) p.pages[i] = static_cast<int>(i);
+  // a warp a block of a head, K and V
+  const int64_t blocks = static_cast<int64_t>(p.total_pages) * p.page_blocks;
+  for (int64_t i = first; i < blocks * p.hkv; i += warps) {
+    const int64_t b = i / p.hkv;
+    const int h = static_cast<int>(i - b * p.hkv);
+    const int page = p.page_blocks == 1 ? static_cast<int>(b) : static_cast<int>(b / p.page_blocks);
+    const int64_t block = static_cast<int64_t>(__ldg(ids + page)) * p.page_blocks + (b - static_cast<int64_t>(page) * p.page_blocks);
+    const bool ok = block >= 0 && block < p.num_blocks;
+    if (!ok && p.status && lane == 0) atomicOr(p.status, 2);
+    const int64_t at = ((ok ? block : 0) * p.hkv + h) * kv4_block_bytes(HD);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const unsigned char* src = pools[j] + at;
+      uint32_t word[kKv4Rows / RPP], pair[kKv4Rows / RPP];
+#pragma unroll
+      for (int k = 0; k < kKv4Rows / RPP; ++k) {
+        const int r = k * RPP + rsub;
+        word[k] = ok ? __ldg(reinterpret_cast<const uint32_t*>(src + r * (HD / 2) + word_at)) : 0u;
+        pair[k] = ok ? __ldg(reinterpret_cast<const uint32_t*>(src + pair_at + r * (G * 4))) : 0u;
+      }
+      __half* const dst = (j == 0 ? p.k_rows : p.v_rows) + (b * kKv4Rows * p.hkv + h) * HD + c * 8;
+#pragma unroll
+      for (int k = 0; k < kKv4Rows / RPP; ++k)
+        *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(k * RPP + rsub) * p.hkv * HD) =
+            kv4_values<__half>(word[k], same_pair(T{}, __half{}, pair[k]));
+    }
+  }
+  if (q == nullptr) return;
+  const uint32_t mask = CH == 32 ? 0xffffffffu : (lane & 16) ? 0xffff0000u : 0x0000ffffu;
+  for (int64_t row = first * RPP + rsub; row < p.num_q_rows; row += warps * RPP) {
+    uint4 x = *reinterpret_cast<const uint4*>(q + row * HD + c * 8);
+    uint32_t* const w = reinterpret_cast<uint32_t*>(&x);
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, max(w[e] >> 16 & 0x7fffu, w[e] & 0x7fffu));
+#pragma unroll
+    for (int o = 1; o < CH; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+    const float power = row_power(T{}, top), inv = 1.f / power;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_pair(T{}, w[e]);
+      w[e] = MmaOp<__half>::pack(f.x * inv, f.y * inv);
+    }
+    *reinterpret_cast<uint4*>(p.q_rows + row * HD + c * 8) = x;
+    if (c == 0) p.q_power[row] = power;
+  }
+}
+
 }  // namespace msgl

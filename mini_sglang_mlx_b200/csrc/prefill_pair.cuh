@@ -188,7 +188,9 @@ struct PairBarriers {
   uint64_t s_full[3], p_full[3], pv_done[3];
 };
 
-template <typename T, int HD, bool PAGED>
+// M: type of the operands.  Where it is not T, q has been converted (p.q_power: what each row was divided by), and the pool's
+// rows are of type M.
+template <typename T, int HD, bool PAGED, typename M = T>
 __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
     prefill_pair_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tg_k,
@@ -561,8 +563,8 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
       }
     } else if (warp == Shape::kMmaWarp && rank == 0) {
       // =========================================================== MMA issuer
-      const uint32_t idesc_s = idesc_m256<T>(BN, 0);
-      const uint32_t idesc_pv = idesc_m256<T>(HD, 1);
+      const uint32_t idesc_s = idesc_m256<M>(BN, 0);
+      const uint32_t idesc_pv = idesc_m256<M>(HD, 1);
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t desc_k = smem_desc_sw128(0, 16, 1024);                 // Q / K: K-major
       const uint64_t desc_v = smem_desc_sw128(0, BN * 128, 1024);           // V: MN-major
@@ -663,7 +665,13 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
     float m_ref = -INFINITY, l = 0.f;
     bool alive = true;
     const bool sc_neg = !(p.scale_log2 > 0.f);
-    const float sc = sc_neg ? 1.f : p.scale_log2;
+    float row_scale = p.scale_log2;
+    if constexpr (!std::is_same<M, T>::value) {
+      const int pk = pk0 + rank * ROWS + r;
+      if (r < rows_valid)
+        row_scale *= p.q_power[static_cast<int64_t>(sq.q_begin + tl) * p.hq + static_cast<int64_t>(h) * G + (pk - tl * G)];
+    }
+    const float sc = sc_neg ? 1.f : row_scale;
 
     const uint32_t p_bar = cluster_addr(bar_p(0), 0);
     // the gate's rows on their way into L2: the epilogue wants them
@@ -693,7 +701,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
       reg_fence(v);
       if (sc_neg) {  // a non-positive scale: fold it into the scores so that max() commutes
 #pragma unroll
-        for (int e = 0; e < BN; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * p.scale_log2);
+        for (int e = 0; e < BN; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * row_scale);
       }
       if (need_mask) {
         if constexpr (HD == 128) {
@@ -790,7 +798,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
           const float p1 = fast_exp2(x1);
           if (e & 2) lb = add_f32x2(lb, pack_f32x2(p0, p1));
           else la = add_f32x2(la, pack_f32x2(p0, p1));
-          pk16[e >> 1] = MmaOp<T>::pack(p0, p1);
+          pk16[e >> 1] = MmaOp<M>::pack(p0, p1);
         }
         tmem_st16(s_tm + sb * BN + c * 16, pk16);  // P columns [16c, 16c+16) of this S buffer
       }

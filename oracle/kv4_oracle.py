@@ -72,22 +72,22 @@ def read(pool: torch.Tensor, slots) -> torch.Tensor:
     return torch.where(ok[:, None, None], out, 0 * out)
 
 
-def attention(q, k_pool, v_pool, slots, seen, scale):
+def attention(q, k_pool, v_pool, slots, seen, scale, device="cpu"):
     """One sequence: q ``(n, hq, d)``, its slot ids in order, ``seen (n, len(slots))``.  Returns float64 outputs and, for bounds,
-    the sum of the weights times the largest of |v|, and of half a group's range, and sum over d of |q k| scale, the largest over keys seen, per row and head."""
-    q = q.double().cpu()
+    the sum of the weights times the largest of |v|, and of its group's range, and sum over d of |q k| scale, the largest over keys seen, per row and head."""
+    q, seen = q.double().to(device), seen.to(device)
     n, hq, d = q.shape
-    k, v = read(k_pool, slots), read(v_pool, slots)
+    k, v = read(k_pool, slots).to(device), read(v_pool, slots).to(device)
     rep = hq // k.shape[1]
     k, v = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
     span = v.unflatten(-1, (-1, GROUP))
-    span = ((span.max(-1).values - span.min(-1).values)[..., None] * (8 / 15)).expand_as(span.unsqueeze(-1)[..., 0]).flatten(-2)
+    span = ((span.max(-1).values - span.min(-1).values)[..., None]).expand_as(span.unsqueeze(-1)[..., 0]).flatten(-2)
     if k.shape[0] == 0:
         z = torch.zeros(n, hq, d, dtype=torch.float64)
-        return z, z.clone(), torch.zeros(n, hq, dtype=torch.float64)
+        return z, z.clone(), z[..., 0].clone()
     score = torch.einsum("nhd,thd->hnt", q, k) * scale
     score = score.masked_fill(~seen[None], -math.inf)
     w = torch.softmax(score, -1).nan_to_num(0.0)                      # (rows without a key: zeros)
     size = torch.einsum("nhd,thd->hnt", q.abs(), k.abs()) * abs(scale)
-    return (torch.einsum("hnt,thd->nhd", w, v), torch.einsum("hnt,thd->nhd", w, torch.maximum(v.abs(), span)),
-            size.masked_fill(~seen[None], 0).amax(-1).T)
+    return (torch.einsum("hnt,thd->nhd", w, v).cpu(), torch.einsum("hnt,thd->nhd", w, torch.maximum(v.abs(), span)).cpu(),
+            size.masked_fill(~seen[None], 0).amax(-1).T.cpu())

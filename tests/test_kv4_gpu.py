@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from mini_sglang_mlx_b200 import _lib
 from mini_sglang_mlx_b200 import kernel as K
 from oracle import kv4_oracle as Q
 from oracle import paged_attention_oracle as O
@@ -235,22 +236,23 @@ def sequences(gen, kv_lens, page_size, hkv, d, dtype, spread=1.0):
     return kc, vc, indptr, order, slots
 
 
-def assert_within(out, ref, weighted, size, dtype, values_rounded, what=""):
-    """Weight times scale (or weight, and value) and the output are rounded to the type.  A weight times scale counts by the code, taken from
-    its middle: p scale |n - 8| <= 8 p scale, 8/15 of the group's range (the scale is at most range / 15 of what the store
-    was given; what it holds spans all of it, a code 0 and a code 15, where the scale was not rounded to less); `weighted` has the larger of that and |v|.  A score is off by fp32 accumulation of numbers of up to
-    256 times the codes' (2^-23 of 256 |q| scale for every of 16 products' sums, against sum |q k| >= |q| scale / 2 for all but
-    groups around zero: 2^-9 of the size covers it) and, where keys are rounded, by half a unit of its terms."""
-    u = half_unit(dtype)
-    score = size[..., None] * ((u if values_rounded else 0) + 2.0 ** -12) + 2.0 ** -20
-    tol = (u * (3 if values_rounded else 2) + 2 * score.expm1()) * weighted + u * ref.abs() + 1e-6
+def assert_within(out, ref, weighted, size, dtype):
+    """The output is rounded to the type, and in front of that in f16 (half a unit u16 = 2^-12, as f16 is what the products
+    take): decode rounds weight times scale, p scale n <= p range, where n is the code and the range its group's; prefill rounds the weight and
+    the value, p |v| each; `weighted` is the sum of the weights times the larger of |v| and the range.  A score is off by fp32
+    accumulation (2^-20 of the sum of its terms' sizes covers 256 of them) and, in prefill, by u16 of it, as keys are rounded; where the sizes of terms are those of scale n and bias instead of their
+    sum k, they are at most 2 range + |k| <= 31 |k| for all but keys near their group's zero: 2^-15 of the size."""
+    u, u16 = half_unit(dtype), 2.0 ** -12
+    score = size[..., None] * (u16 + 2.0 ** -15) + 2.0 ** -20
+    tol = (2 * u16 + 2 * score.expm1()) * weighted + u * ref.abs() + 1e-6
     err = (out.double().cpu() - ref).abs()
-    assert torch.isfinite(out).all(), what
-    assert (err <= tol).all(), f"{what}: {float((err / tol).max()):.3g} times the bound"
-    # roundings are independent: as norms they are a fraction (1/sqrt 3) of half a unit each, four of them at most
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"{float((err / tol).max()):.3g} times the bound"
+    # roundings are independent: as norms they are a fraction (1/sqrt 3) of half a unit each; u of the output, and of u16 four
+    # with up to 2.5 times the output's size (the range against |v|)
     if ref.numel() > 4096 and ref.norm() > 0:
         rel = float((out.double().cpu() - ref).norm() / ref.norm())
-        assert rel <= 2.0 * u, f"{what}: {rel:.3g} off as a norm"
+        assert rel <= u / 3 ** 0.5 + 2.5 * 2 * u16, f"{rel:.3g} off as a norm"
 
 
 DECODE = [
@@ -290,7 +292,7 @@ def test_decode(hq, hkv, d, dtype, page_size, kv_lens, gated):
         u = half_unit(dtype)
         assert (err <= (plain.double().cpu() - ref).abs() * g * (1 + 4 * u) + 2.1 * u * (ref * g).abs() + 1e-6).all()
     else:
-        assert_within(out, ref, weighted, size, dtype, False)
+        assert_within(out, ref, weighted, size, dtype)
         for b, t in enumerate(kv_lens):
             if t == 0:
                 assert (out[b] == 0).all()
@@ -317,6 +319,26 @@ PREFILL = [
 ]
 
 
+# long ones, most of which expand their pages first
+LONG = [
+    (32, 8, 128, BF16, 16, [4000], [2100], False, 0),
+    (32, 4, 128, F16, 32, [3001, 500], [1800, 1500], False, 0),
+    (16, 4, 256, BF16, 16, [2500], [1900], False, 1500),
+    (24, 2, 256, F16, 16, [700, 1], [1333, 2000], True, 0),
+    (40, 8, 128, BF16, 16, [5000], [1700], False, 0),
+]
+
+
+def test_long_prefills_expand_their_pages():
+    def expanded(hq, hkv, d, dtype, page_size, cached, new, cross, window):
+        pages = sum(-(-(a + b) // page_size) for a, b in zip(cached, new))
+        return _lib.lib().msgl_prefill_expanded_bytes_q4(len(new), sum(new), pages, page_size, hq, hkv, d, int(dtype == F16),
+                                                         max(new), cross, window)
+
+    assert sum(expanded(*case) > 0 for case in LONG) >= 3
+    assert not any(expanded(*case) for case in PREFILL)
+
+
 def mask_of(cached, new, cross, window):
     pos = (cached + torch.arange(new))[:, None]
     t = torch.arange(cached + new)
@@ -324,9 +346,10 @@ def mask_of(cached, new, cross, window):
     return seen & (t >= pos - window + 1) if window else seen
 
 
-@pytest.mark.parametrize("hq,hkv,d,dtype,page_size,cached,new,cross,window", PREFILL)
+@pytest.mark.parametrize("hq,hkv,d,dtype,page_size,cached,new,cross,window", PREFILL + LONG)
 def test_prefill(hq, hkv, d, dtype, page_size, cached, new, cross, window):
     clean()
+    long = sum(new) > 1500
     gen = torch.Generator().manual_seed(hq * d + sum(new))
     kv_lens = [a + b for a, b in zip(cached, new)]
     kc, vc, indptr, order, slots = sequences(gen, kv_lens, page_size, hkv, d, dtype)
@@ -343,10 +366,10 @@ def test_prefill(hq, hkv, d, dtype, page_size, cached, new, cross, window):
                                             sliding_window_size=window, **kw)
 
     out = call()
-    parts = [Q.attention(q[qo[b]:qo[b + 1]], kc, vc, s, mask_of(cached[b], new[b], cross, window), scale)
-             for b, s in enumerate(slots)]
+    parts = [Q.attention(q[qo[b]:qo[b + 1]], kc, vc, s, mask_of(cached[b], new[b], cross, window), scale,
+                         "cuda" if long else "cpu") for b, s in enumerate(slots)]
     ref, weighted, size = (torch.cat(x) for x in zip(*parts))
-    assert_within(out, ref, weighted, size, dtype, True)
+    assert_within(out, ref, weighted, size, dtype)
     gate = torch.randn(q.shape, generator=gen).to(dtype)
     g = torch.sigmoid(gate.double())
     u = half_unit(dtype)
