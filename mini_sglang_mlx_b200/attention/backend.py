@@ -17,6 +17,8 @@ Differences, all inside the boundary:
   (``page_indptr`` / ``page_indices`` / ``kv_lens``) and, when the page size is a
   multiple of 16, attention runs through the page-granular operators whose kernels
   fetch K/V as TMA boxes.
+* a pool held in 4 bits (``kvcache.MHAKVCacheQ4``, pages of a multiple of 16 tokens) takes the same calls: rows are quantised as
+  they are stored, and attention runs through the operators over such a pool.
 * ``num_kv_splits`` is filled in for callers that read it (``compute_num_kv_splits``;
   ``policy="reference"`` keeps the reference rule ``min(32, max(1, ceil(L/128)))``, lines
   304-307).  The decode op does not: it cuts the batch into equal shares, and takes from
@@ -33,8 +35,10 @@ import torch
 
 from .. import _lib
 from ..kernel import (_ops, build_attn_metadata, paged_decode_attention, paged_decode_attention_p16,
-                      paged_prefill_attention, paged_prefill_attention_p16, qk_norm_rope_store)
+                      paged_decode_attention_q4, paged_prefill_attention, paged_prefill_attention_p16,
+                      paged_prefill_attention_q4, qk_norm_rope_store, qk_norm_rope_store_q4)
 from ..kvcache.mha_pool import MHAKVCache
+from ..kvcache.mha_pool_q4 import MHAKVCacheQ4
 
 MAX_KV_SPLITS = 32
 
@@ -131,6 +135,9 @@ class AttnBackend:
         self._paged_ops = self.page_size % 16 == 0
         self._index_page = self.page_size if self._paged_ops else 1
         self._own_pool = type(kvcache) is MHAKVCache   # a pool of another class keeps its own store_kv
+        self._pool_q4 = isinstance(kvcache, MHAKVCacheQ4)
+        if self._pool_q4 and not self._paged_ops:
+            raise ValueError(f"a 4-bit pool takes pages of a multiple of 16 tokens, got page_size={page_size}")
         self._sm_count: Optional[int] = None
         self._staging: List[torch.Tensor] = []        # pinned (3, capacity) int32 buffers, in turn
         self._staging_events: List[torch.cuda.Event] = []
@@ -186,7 +193,15 @@ class AttnBackend:
     def _attend(self, q, k_cache, v_cache, metadata, is_cross_attention: bool,
                 sliding_window_size: int, gate=None) -> torch.Tensor:
         paged = self._paged_ops and metadata.page_indices is not None
+        if self._pool_q4 and not paged:
+            raise ValueError("a 4-bit pool takes metadata with page ids")
         if isinstance(metadata, PrefillMetadata):
+            if self._pool_q4:
+                return paged_prefill_attention_q4(
+                    q, k_cache, v_cache, metadata.qo_indptr, metadata.page_indptr, metadata.page_indices,
+                    metadata.kv_lens, metadata.prefix_lens, self.sm_scale, metadata.max_len_extend,
+                    page_size=metadata.page_size, is_cross_attention=is_cross_attention,
+                    sliding_window_size=sliding_window_size, gate=gate)
             if paged:
                 return paged_prefill_attention_p16(
                     q, k_cache, v_cache, metadata.qo_indptr, metadata.page_indptr, metadata.page_indices,
@@ -201,6 +216,10 @@ class AttnBackend:
         assert isinstance(metadata, DecodeMetadata)
         assert not is_cross_attention and sliding_window_size == 0, (
             "is_cross_attention / sliding_window_size are only supported on the prefill path.")
+        if self._pool_q4:
+            return paged_decode_attention_q4(
+                q, k_cache, v_cache, metadata.page_indptr, metadata.page_indices, metadata.kv_lens, self.sm_scale,
+                page_size=metadata.page_size, gate=gate)
         if paged:
             return paged_decode_attention_p16(
                 q, k_cache, v_cache, metadata.page_indptr, metadata.page_indices, metadata.kv_lens,
@@ -217,7 +236,8 @@ class AttnBackend:
                                  gate: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``forward`` for a layer that hands over its raw projections: the per-head q/k
         RMSNorm, the rotary embedding at ``batch.attn_metadata.positions`` and the K/V store
-        run as one pass (``qk_norm_rope_store``; q is updated in place), then paged attention.
+        run as one pass (``qk_norm_rope_store``; q is updated in place, but for a 4-bit pool, where it is
+        read), then paged attention.
 
         Equivalent to the reference layer's ``q_norm``, ``k_norm``, ``rope``, ``rope`` followed by
         ``AttnBackend.forward`` (mini_sglang_mlx/models/qwen3.py:58-68)."""
@@ -226,6 +246,10 @@ class AttnBackend:
         metadata = batch.attn_metadata
         k_cache = self.kvcache.k_cache(layer_id)
         v_cache = self.kvcache.v_cache(layer_id)
+        if self._pool_q4:
+            q = qk_norm_rope_store_q4(q, k, v, q_norm_weight, k_norm_weight, metadata.positions, batch.out_loc, k_cache,
+                                      v_cache, rope_base=rope_base, eps=rms_norm_eps, rotary_dim=rotary_dim)
+            return self._attend(q, k_cache, v_cache, metadata, is_cross_attention, sliding_window_size, gate)
         out = self._layer(q, k, v, k_cache, v_cache, batch.out_loc,
                           (q_norm_weight, k_norm_weight, metadata.positions, rope_base, rms_norm_eps, rotary_dim),
                           metadata, is_cross_attention, sliding_window_size, gate)

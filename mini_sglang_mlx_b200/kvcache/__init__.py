@@ -1,5 +1,6 @@
 from .base import BaseCacheHandle, SizeInfo  # noqa: F401
 from .mha_pool import MHAKVCache  # noqa: F401
+from .mha_pool_q4 import MHAKVCacheQ4  # noqa: F401
 from .naive_manager import NaiveCacheManager  # noqa: F401
 from .radix_manager import RadixCacheHandle, RadixCacheManager  # noqa: F401
 
