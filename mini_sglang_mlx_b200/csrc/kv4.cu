@@ -29,6 +29,7 @@ int check_pool(const char* op, int num_kv_heads, int head_dim, int64_t num_slots
   return MSGL_OK;
 }
 
+constexpr int64_t kItemsFill = 148 * 32;     // groups of lanes that keep a B200 busy
 unsigned grid_of(int64_t threads, int per_sm) {
   int sms = sm_count_cached();
   if (sms <= 0) sms = 148;
@@ -156,6 +157,8 @@ int msgl_store_kv_cache_q4(void* k_cache, void* v_cache, const int32_t* indices,
   const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
   if (length > 1 && (k_token_stride < row || v_token_stride < row))
     return fail(MSGL_BAD_SHAPE, std::string(op) + "row stride smaller than num_kv_heads*head_dim");
+  if (static_cast<int64_t>(length) * num_kv_heads >= (1ll << 31))
+    return fail(MSGL_BAD_SHAPE, std::string(op) + "too many rows for one call");
   if (length == 0) return MSGL_OK;
   if (!k_cache || !v_cache || !indices || !k || !v) return fail(MSGL_BAD_ARG, std::string(op) + "null tensor pointer");
   auto aligned = [](const void* ptr, int a) { return reinterpret_cast<uintptr_t>(ptr) % a == 0; };
@@ -173,6 +176,7 @@ int msgl_store_kv_cache_q4(void* k_cache, void* v_cache, const int32_t* indices,
   p.num_slots = num_slots;
   p.n = length;
   p.hkv = num_kv_heads;
+  p.hkv_recip = msgl::row_reciprocal(num_kv_heads);
   p.wide = aligned16(k) && aligned16(v) && k_token_stride % 8 == 0 && v_token_stride % 8 == 0;
   p.status = static_cast<int*>(status_word);
   auto* kernel = head_dim == 256 ? (dtype == MSGL_DTYPE_BF16 ? msgl::kv4_store_kernel<__nv_bfloat16, 256>
@@ -189,6 +193,8 @@ int msgl_load_kv_cache_q4(const void* k_cache, const void* v_cache, const int32_
   const char* op = "load_kv_cache_q4: ";
   if (length < 0) return fail(MSGL_BAD_SHAPE, std::string(op) + "negative length");
   if (const int rc = check_pool(op, num_kv_heads, head_dim, num_slots, dtype)) return rc;
+  if (static_cast<int64_t>(length) * num_kv_heads >= (1ll << 31))
+    return fail(MSGL_BAD_SHAPE, std::string(op) + "too many rows for one call");
   if (length == 0) return MSGL_OK;
   if (!k_cache || !v_cache || !indices || !k || !v) return fail(MSGL_BAD_ARG, std::string(op) + "null tensor pointer");
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k) || !aligned16(v))
@@ -202,6 +208,7 @@ int msgl_load_kv_cache_q4(const void* k_cache, const void* v_cache, const int32_
   p.num_slots = num_slots;
   p.n = length;
   p.hkv = num_kv_heads;
+  p.hkv_recip = msgl::row_reciprocal(num_kv_heads);
   p.status = static_cast<int*>(status_word);
   auto* kernel = head_dim == 256 ? (dtype == MSGL_DTYPE_BF16 ? msgl::kv4_load_kernel<__nv_bfloat16, 256>
                                                              : msgl::kv4_load_kernel<__half, 256>)
@@ -238,7 +245,10 @@ int msgl_qk_norm_rope_store_q4(const void* q, const void* k, const void* v, cons
       k_token_stride % 4 != 0 || v_token_stride % 4 != 0 || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
     return fail(MSGL_BAD_ARG, std::string(op) + "q, k and v rows and the norm weights must be 8-byte aligned, the pools and "
                                                 "the result 16-byte aligned");
-  constexpr int R = msgl::kKv4RowsPerItem;
+  // rows of an item: few while there are not items enough to fill the GPU, then as many as share a token's angles (8 q rows)
+  const int64_t all_rows = static_cast<int64_t>(n_tokens) * (num_q_heads + 2 * num_kv_heads);
+  int R = 1;
+  while (R < 8 && all_rows > static_cast<int64_t>(R) * kItemsFill) R *= 2;
   const int64_t items = static_cast<int64_t>(n_tokens) * ((num_q_heads + R - 1) / R + 2 * ((num_kv_heads + R - 1) / R));
   if (items >= (1ll << 31)) return fail(MSGL_BAD_ARG, std::string(op) + "too many rows for one call");
   msgl::Kv4ProjectParams p{};
@@ -256,6 +266,7 @@ int msgl_qk_norm_rope_store_q4(const void* q, const void* k, const void* v, cons
   p.hq = num_q_heads;
   p.hkv = num_kv_heads;
   p.rotary_dim = rotary_dim;
+  p.item_rows = R;
   p.q_stride = q_token_stride;
   p.k_stride = k_token_stride;
   p.v_stride = v_token_stride;
@@ -267,7 +278,7 @@ int msgl_qk_norm_rope_store_q4(const void* q, const void* k, const void* v, cons
                                                              : msgl::kv4_project_kernel<__half, 256>)
                                  : (dtype == MSGL_DTYPE_BF16 ? msgl::kv4_project_kernel<__nv_bfloat16, 128>
                                                              : msgl::kv4_project_kernel<__half, 128>);
-  const cudaError_t e = launch_dependent(kernel, dim3(grid_of(items * msgl::kv4_project_lanes(head_dim), 16)), dim3(256), 0,
+  const cudaError_t e = launch_dependent(kernel, dim3(grid_of(items * msgl::kv4_project_lanes(head_dim), 4)), dim3(256), 0,
                                          static_cast<cudaStream_t>(stream), p);
   return e == cudaSuccess ? MSGL_OK : cuda_fail("qk_norm_rope_store_q4", e);
 }

@@ -14,6 +14,8 @@
 // its halves, two neighbours of a 16-bit row.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace msgl {
@@ -150,19 +152,14 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint32_t (&x)[W], uint32_t mask
       mx = max2_nan<T>(mx, x[w]);
       mn = min2_nan<T>(mn, x[w]);
     }
+    // (max, -min) in one word: one exchange for both
+    uint32_t ends = max2_nan<T>(__byte_perm(mx, mn ^ 0x80008000u, 0x5410), __byte_perm(mx, mn ^ 0x80008000u, 0x7632));
 #pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) {
-      mx = max2_nan<T>(mx, __shfl_xor_sync(mask, mx, o));
-      mn = min2_nan<T>(mn, __shfl_xor_sync(mask, mn, o));
-    }
-    const float2 a = unpack_pair(T{}, mx), b = unpack_pair(T{}, mn);
-    hi = fmaxf(a.x, a.y);
-    lo = fminf(b.x, b.y);
-    // (fmaxf would drop a NaN of one half)
-    if ((fabsf(a.x) <= kKv4Max && fabsf(a.y) <= kKv4Max && fabsf(b.x) <= kKv4Max &&
-         fabsf(b.y) <= kKv4Max) ||
-        again)
-      break;
+    for (int o = 1; o < LANES; o <<= 1) ends = max2_nan<T>(ends, __shfl_xor_sync(mask, ends, o));
+    const float2 e = unpack_pair(T{}, ends);
+    hi = e.x;
+    lo = -e.y;
+    if ((fabsf(hi) <= kKv4Max && fabsf(lo) <= kKv4Max) || again) break;
     if (status) atomicOr(status, kKv4Reported);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -172,12 +169,18 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint32_t (&x)[W], uint32_t mask
       x[w] = MmaOp<T>::pack(v.x, v.y);
     }
   }
-  const T s16 = MmaOp<T>::from_float((hi - lo) / 15.f);
+  const float range = hi - lo;
+  float fifteenth = range * (1.f / 15.f);
+  fifteenth = fmaf(fmaf(-15.f, fifteenth, range), 1.f / 15.f, fifteenth);
+  const T s16 = MmaOp<T>::from_float(fifteenth);
   const float scale = to_f32(s16);
   const bool flat = !(scale >= 7.888609052210118e-31f);   // 2^-100
   pair = MmaOp<T>::pack(flat ? 0.f : scale, lo);
-  const float inv = flat ? 0.f : __frcp_rn(scale);
+  const float inv = flat ? 0.f : rcp_approx(scale);
   const uint64_t lo2 = pack_f32x2(-lo, -lo), inv2 = pack_f32x2(inv, inv), scale2 = pack_f32x2(-scale, -scale);
+  const uint64_t magic = pack_f32x2(12582912.f, 12582912.f);     // 1.5 * 2^23: the sum's lowest bits are the rounded number
+  // (a quotient is over 15.5 only where the scale was rounded down by more than 1/32, i.e. is subnormal)
+  const bool clamp = std::is_same<T, __half>::value && scale < 6.103515625e-5f;
   uint32_t out = 0;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
@@ -186,16 +189,28 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint32_t (&x)[W], uint32_t mask
     uint64_t q = mul_f32x2(a, inv2);
     q = fma_f32x2(fma_f32x2(q, scale2, a), inv2, q);
     float q0, q1;
-    unpack_f32x2(q, q0, q1);
-    // (rint by the addition of 1.5 * 2^23; what is over 15 comes from a scale that was rounded down)
-    const uint32_t n0 = __float_as_uint(fminf(q0, 15.f) + 12582912.f) & 15u;
-    const uint32_t n1 = __float_as_uint(fminf(q1, 15.f) + 12582912.f) & 15u;
-    out |= (n0 | n1 << 16) << (4 * w);
+    if (clamp) {
+      unpack_f32x2(q, q0, q1);
+      q = pack_f32x2(fminf(q0, 15.f), fminf(q1, 15.f));
+    }
+    unpack_f32x2(add_f32x2(q, magic), q0, q1);
+    out += __byte_perm(__float_as_uint(q0), __float_as_uint(q1), 0x5410) << (4 * w);
   }
   return out;
 }
 
 // ---------------------------------------------------------------- rows into the pool
+// Token of a row (token * heads + head) without a division: the high half of a product with ceil(2^32 / heads) is it or one more.
+__host__ __device__ __forceinline__ uint32_t row_reciprocal(uint32_t heads) {
+  return heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads);
+}
+__device__ __forceinline__ uint32_t token_of(uint32_t row, uint32_t heads, uint32_t recip) {
+  if (recip == 0u) return row;
+  const uint32_t t = __umulhi(row, recip);
+  return t * heads > row ? t - 1 : t;
+}
+
+// Eight lanes a group, sixteen bytes of K and as many of V a lane.  What bounds it is instruction issue.
 struct Kv4StoreParams {
   unsigned char *k_pool, *v_pool;
   const void *k, *v;          // (n, hkv, head_dim), dense heads
@@ -203,6 +218,7 @@ struct Kv4StoreParams {
   int64_t k_stride, v_stride; // elements between tokens
   int64_t num_slots;
   int n, hkv;
+  uint32_t hkv_recip;         // see row_of_token
   int wide;                   // rows are 16-byte aligned
   int* status;
 };
@@ -217,11 +233,11 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreParams p) {
   const T* v = after_wait(static_cast<const T*>(p.v));
   const int lane = threadIdx.x & 31;
   const uint32_t mask = 0xffu << (lane & 24);       // the eight lanes of a group
-  const int64_t total = static_cast<int64_t>(p.n) * p.hkv * CH;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t row = i / CH;
-    const int c = static_cast<int>(i - row * CH);   // elements 8 c .. 8 c + 7
-    const int t = static_cast<int>(row / p.hkv), h = static_cast<int>(row - static_cast<int64_t>(t) * p.hkv);
+  constexpr uint32_t PER = 256 / CH;                // rows of a CTA at a time
+  const uint32_t rows = static_cast<uint32_t>(p.n) * p.hkv;
+  const int c = threadIdx.x % CH;                   // elements 8 c .. 8 c + 7
+  for (uint32_t row = blockIdx.x * PER + threadIdx.x / CH; row < rows; row += gridDim.x * PER) {
+    const uint32_t t = token_of(row, p.hkv, p.hkv_recip), h = row - t * p.hkv;
     const int slot = slots[t];
     if (slot < 0 || slot >= p.num_slots) {
       if (p.status) atomicOr(p.status, 2);
@@ -262,6 +278,7 @@ struct Kv4LoadParams {
   const int32_t* slots;
   int64_t num_slots;
   int n, hkv;
+  uint32_t hkv_recip;
   int* status;
 };
 
@@ -272,11 +289,11 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
   grid_dependency_launch();
   const int32_t* slots = after_wait(p.slots);
   const unsigned char* pools[2] = {after_wait(p.k_pool), after_wait(p.v_pool)};
-  const int64_t total = static_cast<int64_t>(p.n) * p.hkv * CH;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t row = i / CH;
-    const int c = static_cast<int>(i - row * CH);
-    const int t = static_cast<int>(row / p.hkv), h = static_cast<int>(row - static_cast<int64_t>(t) * p.hkv);
+  constexpr uint32_t PER = 256 / CH;
+  const uint32_t rows = static_cast<uint32_t>(p.n) * p.hkv;
+  const int c = threadIdx.x % CH;
+  for (uint32_t row = blockIdx.x * PER + threadIdx.x / CH; row < rows; row += gridDim.x * PER) {
+    const uint32_t t = token_of(row, p.hkv, p.hkv_recip), h = row - t * p.hkv;
     const int slot = slots[t];
     const bool ok = slot >= 0 && slot < p.num_slots;
     if (!ok && p.status) atomicOr(p.status, 2);
@@ -297,7 +314,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
         reinterpret_cast<uint32_t*>(&o)[e] = MmaOp<T>::pack(fmaf(static_cast<float>(n & 15u), sb.x, sb.y),
                                                             fmaf(static_cast<float>(n >> 16 & 15u), sb.x, sb.y));
       }
-      reinterpret_cast<uint4*>(j == 0 ? p.k : p.v)[i] = o;
+      reinterpret_cast<uint4*>(j == 0 ? p.k : p.v)[static_cast<int64_t>(row) * CH + c] = o;
     }
   }
 }

@@ -8,7 +8,9 @@
 // in the last place: the angle is kept in turns, position times a frequency of two floats, exact to 2^-33 turns at 10^5
 // tokens (one float of frequency leaves an angle of 10^5 radians 6e-3 off).
 //
-// A work item is up to four rows of one token and one kind (q, k or v).  head_dim / 8 lanes take it; lane l holds elements
+// A work item is a few rows of one token and one kind (q, k or v), one after the other, the next on its way: angles and
+// weights are the item's, and the code is short (with four rows unrolled the kernel waited for instructions as much as for
+// anything).  head_dim / 8 lanes take it; lane l holds elements
 // 4 l .. 4 l + 3 of the lower half of a row and as many half a row further on, so that with rotary_dim = head_dim a pair is in
 // one lane, and a group of 64 is in sixteen lanes.
 #pragma once
@@ -24,18 +26,21 @@ struct Kv4ProjectParams {
   const int32_t *positions, *slots;
   unsigned char *k_pool, *v_pool;
   int n, hq, hkv, rotary_dim;
+  int item_rows;             // rows of an item at most
   int64_t q_stride, k_stride, v_stride;
   int64_t num_slots;
   double log2_base;
   float eps;
   int* status;
 };
-constexpr int kKv4RowsPerItem = 4;
 __host__ __device__ constexpr int kv4_project_lanes(int hd) { return hd / 8; }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv4_project_kernel(const Kv4ProjectParams p) {
-  constexpr int LANES = kv4_project_lanes(HD), R = kKv4RowsPerItem, G = HD / kKv4Group;
+__global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectParams p) {
+  constexpr int LANES = kv4_project_lanes(HD), G = HD / kKv4Group;
+  const int R = p.item_rows;
+  __shared__ __align__(16) float s_part[HD == 256 ? 256 * 4 : 256 * 8];   // squares on their way to the lanes that sum them
+  __shared__ __align__(16) float s_weight[2][HD];
   const int lane = threadIdx.x & 31;
   const int hl = lane & (LANES - 1);
   const uint32_t hmask = LANES == 32 ? 0xffffffffu : (lane & 16) ? 0xffff0000u : 0x0000ffffu;
@@ -59,6 +64,11 @@ __global__ void __launch_bounds__(256) kv4_project_kernel(const Kv4ProjectParams
   const T* const v = after_wait(static_cast<const T*>(p.v));
   const int32_t* const positions = after_wait(p.positions);
   const int32_t* const slots = after_wait(p.slots);
+  for (int e = threadIdx.x; e < 2 * HD; e += 256) {
+    const T* w = static_cast<const T*>(e < HD ? p.q_weight : p.k_weight);
+    if (w != nullptr) s_weight[e / HD][e % HD] = to_f32(w[e % HD]);
+  }
+  __syncthreads();
   const uint32_t gq = (p.hq + R - 1) / R, gk = (p.hkv + R - 1) / R;
   const uint32_t groups = gq + 2 * gk;
   const uint32_t total = static_cast<uint32_t>(p.n) * groups;
@@ -69,14 +79,6 @@ __global__ void __launch_bounds__(256) kv4_project_kernel(const Kv4ProjectParams
     const int h0 = static_cast<int>(is_q ? g : is_v ? g - gq - gk : g - gq) * R;
     const int cnt = min(R, (is_q ? p.hq : p.hkv) - h0);
     const T* src = (is_q ? q + tok * p.q_stride : is_v ? v + tok * p.v_stride : k + tok * p.k_stride) + h0 * HD;
-    uint2 lo[R], hi[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r < cnt) {
-        lo[r] = reinterpret_cast<const uint2*>(src + r * HD)[hl];
-        hi[r] = reinterpret_cast<const uint2*>(src + r * HD)[LANES + hl];
-      }
-    }
     int slot = 0;
     if (!is_q) {
       slot = slots[tok];
@@ -85,9 +87,13 @@ __global__ void __launch_bounds__(256) kv4_project_kernel(const Kv4ProjectParams
         continue;
       }
     }
+    uint64_t cs[2], sn[2], sm[2];       // cos, sin; what the other member of a pair is multiplied with in the lower half
+    const bool norm = (is_q ? p.q_weight : p.k_weight) != nullptr;
+    const float* weight = s_weight[is_q ? 0 : 1];
+    uint2 lo = reinterpret_cast<const uint2*>(src)[hl], hi = reinterpret_cast<const uint2*>(src)[LANES + hl];
     if (!is_v) {
       const float pos = static_cast<float>(positions[tok]);
-      float cs[4], sn[4];
+      float c4[4], s4[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float t = pos * f_hi[e];
@@ -96,114 +102,120 @@ __global__ void __launch_bounds__(256) kv4_project_kernel(const Kv4ProjectParams
         const float off = 6.2831854820251465f * (rest - (x - part));   // what the sum lost, in radians
         float s0, c0;
         sincospif(2.f * x, &s0, &c0);
-        sn[e] = fmaf(off, c0, s0);
-        cs[e] = fmaf(-off, s0, c0);
+        s4[e] = fmaf(off, c0, s0);
+        c4[e] = fmaf(-off, s0, c0);
       }
-      const T* wt = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
-      uint2 wl = make_uint2(0u, 0u), wh = wl;
-      if (wt != nullptr) {
-        wl = reinterpret_cast<const uint2*>(wt)[hl];
-        wh = reinterpret_cast<const uint2*>(wt)[LANES + hl];
-      }
+      const float sign = in_lane || hl < xm ? -1.f : 1.f;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r >= cnt) break;
-        float a[4], b[4];
-        auto open = [](const uint2& x, float (&f)[4]) {
-          const float2 u = unpack_pair(T{}, x.x), w = unpack_pair(T{}, x.y);
-          f[0] = u.x;
-          f[1] = u.y;
-          f[2] = w.x;
-          f[3] = w.y;
+      for (int w = 0; w < 2; ++w) {
+        cs[w] = pack_f32x2(c4[2 * w], c4[2 * w + 1]);
+        sn[w] = pack_f32x2(s4[2 * w], s4[2 * w + 1]);
+        sm[w] = pack_f32x2(sign * s4[2 * w], sign * s4[2 * w + 1]);
+      }
+    }
+#pragma unroll 1
+    for (int r = 0; r < cnt; ++r) {
+      uint2 lo1 = lo, hi1 = hi;
+      if (r + 1 < cnt) {
+        lo1 = reinterpret_cast<const uint2*>(src + (r + 1) * HD)[hl];
+        hi1 = reinterpret_cast<const uint2*>(src + (r + 1) * HD)[LANES + hl];
+      }
+      if (!is_v) {
+        auto open = [](uint32_t x) {
+          const float2 f = unpack_pair(T{}, x);
+          return pack_f32x2(f.x, f.y);
         };
-        auto close = [](const float (&f)[4]) { return make_uint2(MmaOp<T>::pack(f[0], f[1]), MmaOp<T>::pack(f[2], f[3])); };
-        open(lo[r], a);
-        open(hi[r], b);
-        if (wt != nullptr) {
+        auto close = [](uint64_t x) {
+          float f0, f1;
+          unpack_f32x2(x, f0, f1);
+          return MmaOp<T>::pack(f0, f1);
+        };
+        uint64_t a[2] = {open(lo.x), open(lo.y)}, b[2] = {open(hi.x), open(hi.y)};
+        if (norm) {
           // Sum of the squares, of elements 32 apart first and then of neighbours.  Lane l = 8 i + m holds elements 4 m .. 4 m + 3
-          // of the row's i-th 32 in its lower half, and of the i-th 32 of its upper half.
-          float t4[4];
+          // of the row's i-th 32 in its lower half, and of the i-th 32 of its upper half; through shared memory it gets all that
+          // is at 4 m + i (head_dim 256, four lanes), or at 4 m + 2 i and 4 m + 2 i + 1 (128, two).
+          const int m = hl & 7, i = hl >> 3;
+          float ss;
           if constexpr (LANES == 32) {
-            float u4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u4[e] = __fadd_rn(__fmul_rn(a[e], a[e]), __fmul_rn(b[e], b[e]));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              t4[e] = __shfl_sync(hmask, u4[e], hl & 7);
-#pragma unroll
-              for (int i = 1; i < 4; ++i) t4[e] = __fadd_rn(t4[e], __shfl_sync(hmask, u4[e], (hl & 7) + 8 * i));
-            }
+            float* part = s_part + (threadIdx.x >> 5) * 128;
+            float4 u;
+            unpack_f32x2(add_f32x2(mul_f32x2(a[0], a[0]), mul_f32x2(b[0], b[0])), u.x, u.y);
+            unpack_f32x2(add_f32x2(mul_f32x2(a[1], a[1]), mul_f32x2(b[1], b[1])), u.z, u.w);
+            __syncwarp();
+            reinterpret_cast<float4*>(part)[hl] = u;
+            __syncwarp();
+            const float* at = part + 4 * m + i;
+            ss = __fadd_rn(__fadd_rn(__fadd_rn(at[0], at[32]), at[64]), at[96]);
+            ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, 8));
+            ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, 16));
           } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = __fmul_rn(a[e], a[e]), y = __fmul_rn(b[e], b[e]);
-              const float ox = __shfl_xor_sync(hmask, x, 8), oy = __shfl_xor_sync(hmask, y, 8);
-              t4[e] = __fadd_rn(__fadd_rn(__fadd_rn(x, ox), hl & 8 ? oy : y), hl & 8 ? y : oy);
-            }
+            float* part = s_part + (threadIdx.x >> 4) * 128;
+            float4 u, v;
+            unpack_f32x2(mul_f32x2(a[0], a[0]), u.x, u.y);
+            unpack_f32x2(mul_f32x2(a[1], a[1]), u.z, u.w);
+            unpack_f32x2(mul_f32x2(b[0], b[0]), v.x, v.y);
+            unpack_f32x2(mul_f32x2(b[1], b[1]), v.z, v.w);
+            __syncwarp(hmask);
+            reinterpret_cast<float4*>(part)[hl] = u;
+            reinterpret_cast<float4*>(part)[16 + hl] = v;
+            __syncwarp(hmask);
+            const uint64_t* at = reinterpret_cast<const uint64_t*>(part + 4 * m + 2 * i);
+            float t0, t1;
+            unpack_f32x2(add_f32x2(add_f32x2(add_f32x2(at[0], at[16]), at[32]), at[48]), t0, t1);
+            ss = __fadd_rn(t0, t1);
+            ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, 8));
           }
-          float ss = __fadd_rn(__fadd_rn(t4[0], t4[1]), __fadd_rn(t4[2], t4[3]));
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, o));
           const float inv = rsqrtf(ss * (1.f / HD) + p.eps);
-          float x[4], y[4];
-          open(wl, x);
-          open(wh, y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            a[e] = a[e] * inv * x[e];
-            b[e] = b[e] * inv * y[e];
-          }
-          open(close(a), a);
-          open(close(b), b);
+          const uint64_t inv2 = pack_f32x2(inv, inv);
+          const ulonglong2 wl = reinterpret_cast<const ulonglong2*>(weight)[hl], wh = reinterpret_cast<const ulonglong2*>(weight)[LANES + hl];
+          a[0] = open(close(mul_f32x2(mul_f32x2(a[0], inv2), wl.x)));
+          a[1] = open(close(mul_f32x2(mul_f32x2(a[1], inv2), wl.y)));
+          b[0] = open(close(mul_f32x2(mul_f32x2(b[0], inv2), wh.x)));
+          b[1] = open(close(mul_f32x2(mul_f32x2(b[1], inv2), wh.y)));
         }
         if (in_lane) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = a[e];
-            a[e] = __fsub_rn(__fmul_rn(x, cs[e]), __fmul_rn(b[e], sn[e]));
-            b[e] = __fadd_rn(__fmul_rn(b[e], cs[e]), __fmul_rn(x, sn[e]));
+          for (int w = 0; w < 2; ++w) {
+            const uint64_t x = a[w];
+            a[w] = add_f32x2(mul_f32x2(x, cs[w]), mul_f32x2(b[w], sm[w]));
+            b[w] = add_f32x2(mul_f32x2(b[w], cs[w]), mul_f32x2(x, sn[w]));
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float other = __shfl_xor_sync(hmask, a[e], xm);
-            if (rot_lane) a[e] = __fadd_rn(__fmul_rn(a[e], cs[e]), __fmul_rn(other, hl >= xm ? sn[e] : -sn[e]));
+          for (int w = 0; w < 2; ++w) {
+            const uint64_t other = __shfl_xor_sync(hmask, static_cast<unsigned long long>(a[w]), xm);
+            if (rot_lane) a[w] = add_f32x2(mul_f32x2(a[w], cs[w]), mul_f32x2(other, sm[w]));
           }
         }
-        lo[r] = close(a);
-        hi[r] = close(b);
+        lo = make_uint2(close(a[0]), close(a[1]));
+        hi = make_uint2(close(b[0]), close(b[1]));
       }
-    }
-    if (is_q) {
-      T* dst = static_cast<T*>(p.q_out) + (static_cast<int64_t>(tok) * p.hq + h0) * HD;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (r < cnt) {
-          reinterpret_cast<uint2*>(dst + r * HD)[hl] = lo[r];
-          reinterpret_cast<uint2*>(dst + r * HD)[LANES + hl] = hi[r];
-        }
+      if (is_q) {
+        T* dst = static_cast<T*>(p.q_out) + (static_cast<int64_t>(tok) * p.hq + h0 + r) * HD;
+        reinterpret_cast<uint2*>(dst)[hl] = lo;
+        reinterpret_cast<uint2*>(dst)[LANES + hl] = hi;
+      } else {
+        // (lower half of the row: groups 0 .. G/2 - 1, lane l in group l / 16, word 8 g + (l % 16) / 2 in the order of the row;
+        // an even lane writes the word of the lower half, its neighbour that of the upper half)
+        const int row = slot % kKv4Rows;
+        const int gw = hl / 16 + (hl & 1) * (G / 2), r8 = (hl & 15) >> 1;
+        unsigned char* block = (is_v ? p.v_pool : p.k_pool) +
+                               (static_cast<int64_t>(slot / kKv4Rows) * p.hkv + h0 + r) * kv4_block_bytes(HD);
+        uint32_t xl[2] = {lo.x, lo.y}, xh[2] = {hi.x, hi.y};
+        uint32_t pl, ph;
+        const uint32_t cl = kv4_quantise<T, 2>(xl, gmask, pl, p.status) << (8 * (hl & 1));
+        const uint32_t ch = kv4_quantise<T, 2>(xh, gmask, ph, p.status) << (8 * (hl & 1));
+        // what the neighbour writes goes to it
+        const uint32_t other = __shfl_xor_sync(gmask, (hl & 1) ? cl : ch, 1);
+        *reinterpret_cast<uint32_t*>(block + row * (HD / 2) + (r8 * G + gw) * 4) = other | ((hl & 1) ? ch : cl);
+        if ((hl & 15) < 2)
+          *reinterpret_cast<uint32_t*>(block + kv4_pairs_at(HD) + (row * G + gw) * 4) = (hl & 1) ? ph : pl;
       }
-      continue;
-    }
-    const int row = slot % kKv4Rows;
-    // (lower half of the row: groups 0 .. G/2 - 1, lane l in group l / 16, word 8 g + (l % 16) / 2 in the order of the row;
-    // an even lane writes the word of the lower half, its neighbour that of the upper half)
-    const int gl = hl / 16;
-    const int gw = gl + (hl & 1) * (G / 2), r8 = (hl & 15) >> 1;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r >= cnt) break;
-      unsigned char* block = (is_v ? p.v_pool : p.k_pool) +
-                             (static_cast<int64_t>(slot / kKv4Rows) * p.hkv + h0 + r) * kv4_block_bytes(HD);
-      uint32_t xl[2] = {lo[r].x, lo[r].y}, xh[2] = {hi[r].x, hi[r].y};
-      uint32_t pl, ph;
-      const uint32_t cl = kv4_quantise<T, 2>(xl, gmask, pl, p.status) << (8 * (hl & 1));
-      const uint32_t ch = kv4_quantise<T, 2>(xh, gmask, ph, p.status) << (8 * (hl & 1));
-      // what the neighbour writes goes to it
-      const uint32_t other = __shfl_xor_sync(gmask, (hl & 1) ? cl : ch, 1);
-      *reinterpret_cast<uint32_t*>(block + row * (HD / 2) + (r8 * G + gw) * 4) = other | ((hl & 1) ? ch : cl);
-      if ((hl & 15) < 2)
-        *reinterpret_cast<uint32_t*>(block + kv4_pairs_at(HD) + (row * G + gw) * 4) = (hl & 1) ? ph : pl;
+      lo = lo1;
+      hi = hi1;
     }
   }
 }
