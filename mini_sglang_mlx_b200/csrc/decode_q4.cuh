@@ -59,7 +59,7 @@ struct Q4DecodeParams {
 __host__ __device__ constexpr int q4_merge_row(int hd) { return hd + 4; }
 __host__ __device__ constexpr int q4_partial_floats(int hd) { return hd + 4; }
 __host__ __device__ constexpr int q4_decode_smem(int hd, int warps, int stages) {
-  return warps * stages * 2 * kv4_block_bytes(hd) + warps * 4 * q4_merge_row(hd) * 4 + warps * 8 * 4;
+  return warps * stages * 2 * kv4_block_bytes(hd) + warps * 8 * q4_merge_row(hd) * 4 + warps * 16 * 4;
 }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
   const int ct = BLOCKS || COLS < 16 ? static_cast<int>(blockIdx.x) / p.hkv % p.col_tiles : 0;
   const int share_id = static_cast<int>(blockIdx.x) / p.hkv / p.col_tiles;
   unsigned char* const ring = smem_raw + warp * (STAGES * U * 2 * BLK);
-  float* const sm_o = reinterpret_cast<float*>(smem_raw + WARPS * STAGES * U * 2 * BLK);   // [WARPS][4][MROW]
-  float* const sm_ml = sm_o + WARPS * 4 * MROW;                                       // [WARPS][4][2]
+  float* const sm_o = reinterpret_cast<float*>(smem_raw + WARPS * STAGES * U * 2 * BLK);   // [WARPS][8][MROW]
+  float* const sm_ml = sm_o + WARPS * 8 * MROW;                                       // [WARPS][8][2]
   if (lane < STAGES) mbar_init(smem_u32(&s_bar[warp * STAGES + lane]), 1);
   fence_mbar_init();
   __syncwarp();
@@ -204,14 +204,35 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
   // 32 / U steps, U lanes a step: -1 a page that is not in the pool, -2 none.
   constexpr int BATCH = 32 / U;
   constexpr uint32_t ALL = (1u << U) - 1;
-  if (lane == 0) {
-    Ahead a;
-    a.b = b0;
-    a.step = warp;
-    a.more = segment(b0, beg0, a.s);
-    s_ahead[warp] = a;
-  }
+  Segment cs;
+  bool go = segment(b0, beg0, cs);
+  if (lane == 0) s_ahead[warp] = Ahead{cs, b0, warp, go};
   __syncwarp();
+  // query row of a column of this CTA
+  auto row_of = [&](int b, int tok0, int col) -> int64_t {
+    if constexpr (!BLOCKS) return static_cast<int64_t>(b) * p.hq + h * p.group + ct * COLS + col;
+    const int n = ct * COLS + col, t = n / p.group;
+    return static_cast<int64_t>(tok0 + t) * p.hq + h * p.group + (n - t * p.group);
+  };
+  // a segment's q as it is, word (r8, g) = (2 c + w / G, w % G) of a lane's column; the first one's on its way under the page ids
+  uint32_t qf[NT][WORDS][4];
+  auto fetch_q = [&](int b) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + r;
+      const T* qr = q + (col < cs.cols ? row_of(b, cs.k.tok0, col) : 0) * HD + 16 * c;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (col < cs.cols) x = __ldg(reinterpret_cast<const uint4*>(qr + (w % G) * 64 + (w / G) * 8));
+        qf[nt][w][0] = x.x;
+        qf[nt][w][1] = x.y;
+        qf[nt][w][2] = x.z;
+        qf[nt][w][3] = x.w;
+      }
+    }
+  };
+  if (go) fetch_q(b0);
   int have = 0, at = 0;            // steps of this batch, next one
   int my_block = -2;
   uint32_t bad = 0;                // blocks in the ring whose page is not in the pool
@@ -275,8 +296,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
                                              // of V then lie in two bank halves
   const int tv = 2 * c + (c & 1), tw = 2 * c + 1 - (c & 1);   // tokens of k index 2 c and 2 c + 1
   int cg = warp;
-  Segment cs;
-  for (int b = b0, beg = beg0; segment(b, beg, cs); beg = behind(cs), ++b) {
+  for (int b = b0; go; go = segment(b + 1, behind(cs), cs), ++b) {
     if (h == 0 && ct == 0 && tid == 0 && cs.beg >= r0 && p.status && __ldg(lens + b) != cs.k.len)
       atomicOr(p.status, 2);    // a length that is negative or beyond the sequence's pages: clamped, reported
     if (BLOCKS && h == 0 && ct == 0 && tid == 0 && cs.beg >= r0 && p.status &&
@@ -285,33 +305,18 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
     if (cs.cols <= 0 || (cs.ng == 0 && cs.k.blocks > 0)) continue;
     if (lane == 0) s_current[warp] = cs;
     __syncwarp();
-    // query row of a column of this CTA
-    auto row_of = [&](int col) -> int64_t {
-      if constexpr (!BLOCKS) return static_cast<int64_t>(b) * p.hq + h * p.group + ct * COLS + col;
-      const int n = ct * COLS + col, t = n / p.group;
-      return static_cast<int64_t>(cs.k.tok0 + t) * p.hq + h * p.group + (n - t * p.group);
-    };
+    if (b != b0) fetch_q(b);
     // ---- q: B fragments of the k steps (two of a word), 16 times q where the codes are the lowest bits of the fraction, and
     // a group's sum of q (2^-20 of it, as the products have it) for this lane's two columns
-    uint32_t qf[NT][WORDS][4];
     float qs[NT][G][2], cscale[NT][2];
     int tok[NT][2];          // BLOCKS: token of this lane's columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int col = nt * 8 + r;
-      const T* qr = q + (col < cs.cols ? row_of(col) : 0) * HD + 16 * c;
       uint32_t top = 0;
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w) {        // word (r8, g) = (2 c + w / G, w % G)
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (col < cs.cols) x = *reinterpret_cast<const uint4*>(qr + (w % G) * 64 + (w / G) * 8);
-        qf[nt][w][0] = x.x;
-        qf[nt][w][1] = x.y;
-        qf[nt][w][2] = x.z;
-        qf[nt][w][3] = x.w;
+      for (int w = 0; w < WORDS; ++w)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = max(top, max(qf[nt][w][i] >> 16 & 0x7fffu, qf[nt][w][i] & 0x7fffu));
-      }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float power = row_power(T{}, top), inv = 1.f / power;
@@ -561,18 +566,18 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
     cg -= steps;
     cs = s_current[warp];
 
-    // ---- end of the segment: the warps' sums are merged, four columns (those of one j) at a time
+    // ---- end of the segment: the warps' sums are merged, eight columns at a time
     const bool whole = cs.ng == cs.k.blocks;
     const int64_t slot = (((2ll * share_id + (cs.beg >= r0 ? 1 : 0)) * p.hkv + h) * p.col_tiles + ct) * COLS;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      if (nt * 8 >= cs.cols) break;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (nt * 8 + j >= cs.cols) continue;         // (none of the columns 8 nt + j, + 2, + 4, + 6)
         float lj = l[nt][j];
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) lj += __shfl_xor_sync(0xffffffffu, lj, x);
-        float* row = sm_o + (warp * 4 + c) * MROW + 8 * r;
+        float* row = sm_o + (warp * 8 + 2 * c + j) * MROW + 8 * r;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           float bj = pbias[nt][g][j];
@@ -588,45 +593,46 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
           *reinterpret_cast<float4*>(row + g * 64) = make_float4(x[0], x[1], x[2], x[3]);
           *reinterpret_cast<float4*>(row + g * 64 + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
-        if (r == 0) *reinterpret_cast<float2*>(sm_ml + (warp * 4 + c) * 2) = make_float2(m[nt][j], lj);
-        __syncthreads();
-        for (int e = tid; e < HD; e += WARPS * 32) {      // float4 pieces of the four columns
-          const int cc = e / (HD / 4), d = e % (HD / 4) * 4;
-          const int col = nt * 8 + 2 * cc + j;
-          if (col >= cs.cols) continue;
-          float M = -INFINITY, den = 0.f;
-#pragma unroll
-          for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_ml[(w * 4 + cc) * 2]);
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < WARPS; ++w) {
-            const float mw = sm_ml[(w * 4 + cc) * 2];
-            const float wgt = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
-            den = fmaf(wgt, sm_ml[(w * 4 + cc) * 2 + 1], den);
-            const float4 y = *reinterpret_cast<const float4*>(sm_o + (w * 4 + cc) * MROW + d);
-            x.x = fmaf(wgt, y.x, x.x);
-            x.y = fmaf(wgt, y.y, x.y);
-            x.z = fmaf(wgt, y.z, x.z);
-            x.w = fmaf(wgt, y.w, x.w);
-          }
-          if (whole) {
-            const float inv = den == 0.f ? 0.f : 1.f / den;
-            const int64_t at = row_of(col) * HD + d;
-            alignas(8) T y[4] = {MmaOp<T>::from_float(x.x * inv), MmaOp<T>::from_float(x.y * inv),
-                                 MmaOp<T>::from_float(x.z * inv), MmaOp<T>::from_float(x.w * inv)};
-            if (p.gate != nullptr) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) y[k] = apply_gate<T>(to_f32(y[k]), static_cast<const T*>(p.gate)[at + k]);
-            }
-            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = *reinterpret_cast<const uint2*>(y);
-          } else {
-            float* to = p.part + (slot + col) * PROW;
-            *reinterpret_cast<float4*>(to + d) = x;
-            if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(M, den);
-          }
-        }
-        __syncthreads();
+        if (r == 0) *reinterpret_cast<float2*>(sm_ml + (warp * 8 + 2 * c + j) * 2) = make_float2(m[nt][j], lj);
       }
+      __syncthreads();
+#pragma unroll 1
+      for (int e = tid; e < 2 * HD; e += WARPS * 32) {      // float4 pieces of the eight columns
+        const int cc = e / (HD / 4), d = e % (HD / 4) * 4;
+        const int col = nt * 8 + cc;
+        if (col >= cs.cols) break;
+        float M = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_ml[(w * 8 + cc) * 2]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float2 ml = *reinterpret_cast<const float2*>(sm_ml + (w * 8 + cc) * 2);
+          const float wgt = fast_exp2(ml.x - M);
+          den = fmaf(wgt, ml.y, den);
+          const float4 y = *reinterpret_cast<const float4*>(sm_o + (w * 8 + cc) * MROW + d);
+          x.x = fmaf(wgt, y.x, x.x);
+          x.y = fmaf(wgt, y.y, x.y);
+          x.z = fmaf(wgt, y.z, x.z);
+          x.w = fmaf(wgt, y.w, x.w);
+        }
+        if (whole) {
+          const float inv = den == 0.f ? 0.f : 1.f / den;
+          const int64_t at = row_of(b, cs.k.tok0, col) * HD + d;
+          alignas(8) T y[4] = {MmaOp<T>::from_float(x.x * inv), MmaOp<T>::from_float(x.y * inv),
+                               MmaOp<T>::from_float(x.z * inv), MmaOp<T>::from_float(x.w * inv)};
+          if (p.gate != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = apply_gate<T>(to_f32(y[k]), static_cast<const T*>(p.gate)[at + k]);
+          }
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = *reinterpret_cast<const uint2*>(y);
+        } else {
+          float* to = p.part + (slot + col) * PROW;
+          *reinterpret_cast<float4*>(to + d) = x;
+          if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(M, den);
+        }
+      }
+      __syncthreads();
     }
     if (!whole) {          // at most the first and the last segment of the share
       const int i = parts++ & 1;

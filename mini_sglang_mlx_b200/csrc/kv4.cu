@@ -51,7 +51,7 @@ Q4Plan plan_q4(int batch, int columns, int hkv, int head_dim, int64_t blocks, in
   Q4Plan pl{};
   pl.cols = head_dim == 128 && columns > 8 ? 16 : 8;
   pl.col_tiles = (columns + pl.cols - 1) / pl.cols;
-  constexpr int ctas_per_sm = 1;
+  const int ctas_per_sm = head_dim == 128 && pl.cols == 8 ? 2 : 1;
   const int64_t wave = std::max(1, sms * ctas_per_sm / (hkv * pl.col_tiles));
   blocks += static_cast<int64_t>(batch) * kQ4Pad;
   pl.shares = wave * std::max<int64_t>(1, (blocks + wave * kQ4MaxShare - 1) / (wave * kQ4MaxShare));
@@ -73,8 +73,8 @@ template <bool BLOCKS>
 cudaError_t launch_q4_any(const msgl::Q4DecodeParams& p, int head_dim, int cols, int dtype, cudaStream_t s) {
   auto go = [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    if (head_dim == 256) return launch_q4<T, 256, 1, BLOCKS, 1, 12, 3, 1>(p, s);
-    return cols == 8 ? launch_q4<T, 128, 1, BLOCKS, 2, 12, 3, 1>(p, s) : launch_q4<T, 128, 2, BLOCKS, 1, 12, 6, 1>(p, s);
+    if (head_dim == 256) return launch_q4<T, 256, 1, BLOCKS, 2, 8, 2, 1>(p, s);
+    return cols == 8 ? launch_q4<T, 128, 1, BLOCKS, 4, 4, 2, 2>(p, s) : launch_q4<T, 128, 2, BLOCKS, 2, 8, 3, 1>(p, s);
   };
   return dtype == MSGL_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }
