@@ -132,6 +132,20 @@ bool msgl_host::make_pool_map(CUtensorMap* out, PoolBox form, const void* base, 
   if (!enc || num_slots <= 0 || num_slots >= (1ll << 32) || reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
   const cuuint64_t row = static_cast<cuuint64_t>(num_kv_heads) * head_dim, slots = static_cast<cuuint64_t>(num_slots);
   const bool head = form == PoolBox::kHead;
+  if (form == PoolBox::kPacked) {
+    const cuuint64_t rows = slots / 16 * num_kv_heads * (head_dim / 128);
+    const cuuint64_t dims[2] = {144, rows}, strides[1] = {1152};
+    const cuuint32_t box[2] = {144, 1}, step[2] = {1, 1};
+    CUtensorMap m;
+    if (rows == 0 || rows >= (1ull << 31) ||
+        enc(&m, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<void*>(base), dims, strides, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+    c = Cached{base, num_slots, num_kv_heads, head_dim, dtype, form, m};
+    *out = m;
+    return true;
+  }
   const cuuint64_t dims[3] = {head ? 64 : row, slots, row / 64};
   const cuuint64_t strides[2] = {row * 2, 128};
   const cuuint32_t box[3] = {64, form == PoolBox::kRow ? 1u : static_cast<cuuint32_t>(msgl::kTmaBoxRows),

@@ -325,6 +325,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tma
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+// Four rows of a 2-D tensor whose map has boxes of one row, from its first column.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* tmap, const int (&rows)[4], uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(0), "r"(rows[0]), "r"(rows[1]), "r"(rows[2]), "r"(rows[3]), "r"(bar)
+      : "memory");
+}
 // Untiled bulk copies (16-byte aligned addresses, sizes a multiple of 16 bytes).
 // global -> shared, its bytes counted on `bar` as they land:
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {

@@ -9,8 +9,11 @@
 // rows, any other an fp32 partial (weighted sum, maximum, sum of the weights), and the CTA that arrives last at the
 // (sequence, head)'s counter merges its pieces.  One launch.
 //
-// A block of a head (codes, scales and biases of K: 9 head_dim bytes, and of V) comes with two bulk copies into a ring of the
-// warp's own; the warps of a CTA take the blocks of a segment in turn.
+// A block of a head (codes, scales and biases of K: 9 head_dim bytes, and of V) is contiguous.  The warps of a CTA take the blocks of
+// a segment in turn, U at a step, into a ring of their own; the pool is a tensor of rows of 1152 bytes, so a step's four rows of K come with
+// one tile::gather4 load, and as many of V (rows past the tensor's end, for blocks that are not there and pages that are not in
+// the pool, read as zeros, i.e. as zero keys and values).  A copy instruction costs its warp 67 to 93 cycles, and with one for
+// every block of K and of V a fifth of the loop was that.
 //
 // Arithmetic.  The codes go to the tensor cores as they are, because small integers are f16 numbers already: the pattern n 2^k, inside
 // the fraction, is n 2^(k-24).  A word masked, shifted by eight and masked, gives its elements two by two.
@@ -53,6 +56,7 @@ struct Q4DecodeParams {
   int min_share, pad;         // blocks a share holds at least; blocks that the end of a segment counts for
   int is_cross, window;       // BLOCKS
   int64_t num_blocks;
+  int num_rows;               // of the pools as tensors
   float scale_log2;
 };
 
@@ -69,13 +73,15 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 }
 // U blocks a step and stage: with two, the next block's loads and products fill the first one's waits.
 template <typename T, int HD, int NT, bool BLOCKS, int U, int WARPS, int STAGES, int MINB>
-__global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4DecodeParams p) {
+__global__ void __launch_bounds__(WARPS * 32, MINB)
+    q4_decode_kernel(const Q4DecodeParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int G = HD / kKv4Group;          // groups of a row
   constexpr int BLK = kv4_block_bytes(HD);
   constexpr int ROW = HD / 2;                // code bytes of a row
   constexpr int PAIRS = kv4_pairs_at(HD);
   constexpr int MROW = q4_merge_row(HD), PROW = q4_partial_floats(HD);
   constexpr int COLS = 8 * NT;
+  constexpr bool GATHER = U * HD == 512;     // four rows of the tensor a step (else: bulk copies)
   constexpr int WORDS = 2 * G;               // words of a K row per lane
   constexpr float kSlack = 8.f;
   constexpr float kNoScore = -1.5e38f;       // reference maximum of a column without a key (its sums are zero)
@@ -113,6 +119,10 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
   float* const sm_o = reinterpret_cast<float*>(smem_raw + WARPS * STAGES * U * 2 * BLK);   // [WARPS][8][MROW]
   float* const sm_ml = sm_o + WARPS * 8 * MROW;                                       // [WARPS][8][2]
   if (lane < STAGES) mbar_init(smem_u32(&s_bar[warp * STAGES + lane]), 1);
+  if (GATHER && tid == 0) {
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+  }
   fence_mbar_init();
   __syncwarp();
   grid_dependency_wait();
@@ -267,23 +277,38 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
     return a.more != 0;
   };
   const int64_t block_bytes = static_cast<int64_t>(p.hkv) * BLK, head_at = static_cast<int64_t>(h) * BLK;
-  auto issue = [&](int stage) {    // this warp's next step into a stage, if it has one
+  auto issue = [&](int stage) {    // this warp's next step into a stage, if it has one: its blocks of K, then of V
     if (at == have && !refill()) return;
-    const int block = __shfl_sync(0xffffffffu, my_block, at * U + lane % U);
-    ++at;
-    const uint32_t in = __ballot_sync(0xffffffffu, block >= 0) & ALL;
     const uint32_t bar = smem_u32(&s_bar[warp * STAGES + stage]);
-    if (bad != 0 || in != ALL) {
-      const uint32_t out = __ballot_sync(0xffffffffu, block == -1) & ALL;
-      bad = (bad & ~(ALL << (stage * U))) | out << (stage * U);
+    const uint32_t dst = smem_u32(ring) + stage * (2 * U * BLK);
+    if constexpr (GATHER) {
+      constexpr int PARTS = 4 / U;           // rows of the tensor a block
+      int row[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int block = __shfl_sync(0xffffffffu, my_block, at * U + i / PARTS);
+        row[i] = block < 0 ? p.num_rows : (block * p.hkv + h) * PARTS + i % PARTS;
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, 2 * U * BLK);
+        tma_gather4(dst, &tm_k, row, bar);
+        tma_gather4(dst + U * BLK, &tm_v, row, bar);
+      }
+    } else {
+      const int block = __shfl_sync(0xffffffffu, my_block, at * U + lane % U);
+      const uint32_t in = __ballot_sync(0xffffffffu, block >= 0) & ALL;
+      if (bad != 0 || in != ALL) {
+        const uint32_t out = __ballot_sync(0xffffffffu, block == -1) & ALL;
+        bad = (bad & ~(ALL << (stage * U))) | out << (stage * U);
+      }
+      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(in) * (2 * BLK));
+      if (lane < U && block >= 0) {
+        const int64_t off = block * block_bytes + head_at;
+        bulk_load(dst + lane * BLK, kp + off, BLK, bar);
+        bulk_load(dst + (U + lane) * BLK, vp + off, BLK, bar);
+      }
     }
-    if (lane == 0) mbar_arrive_expect_tx(bar, __popc(in) * (2 * BLK));
-    if (lane < U && block >= 0) {
-      const int64_t off = block * block_bytes + head_at;
-      const uint32_t dst = smem_u32(ring) + (stage * U + lane) * (2 * BLK);
-      bulk_load(dst, kp + off, BLK, bar);
-      bulk_load(dst + BLK, vp + off, BLK, bar);
-    }
+    ++at;
   };
 #pragma unroll 1
   for (int i = 0; i < STAGES; ++i) issue(i);
@@ -385,177 +410,183 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) q4_decode_kernel(const Q4Dec
       }
       const unsigned char* const step_at = ring + stage * (U * 2 * BLK);
       const int t0 = t_lo + cg * (U * kKv4Rows);
-      // pairs of tokens rho and rho + 8
-      uint32_t kpair[U][2][G], vpair[U][2][G];
+      auto step = [&](auto blocks) {
+        constexpr int N = decltype(blocks)::value;
+        // pairs of tokens rho and rho + 8
+        uint32_t kpair[N][2][G], vpair[N][2][G];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const unsigned char* at = step_at + u * (2 * BLK) + PAIRS + (rho + 8 * t) * (G * 4);
-          read_words<G * 4>(kpair[u][t], at);
-          read_words<G * 4>(vpair[u][t], at + BLK);
+          for (int t = 0; t < 2; ++t) {
+            const unsigned char* at = step_at + u * BLK + PAIRS + (rho + 8 * t) * (G * 4);
+            read_words<G * 4>(kpair[u][t], at);
+            read_words<G * 4>(vpair[u][t], at + U * BLK);
+          }
+        if (t0 + N * kKv4Rows > t_hi || (!GATHER && bad != 0)) {   // rows behind the end hold anything; a page outside the pool: zeros
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (t0 + u * kKv4Rows + rho + 8 * t >= t_hi || (!GATHER && (bad >> (stage * U + u) & 1u))) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) kpair[u][t][g] = vpair[u][t][g] = 0u;
+              }
         }
-      if (t0 + U * kKv4Rows > t_hi || bad != 0) {   // rows behind the end hold anything; a page outside the pool: zeros
+        // ---- scores
+        float s[N][NT][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < N; ++u) {
+          const unsigned char* const kb = step_at + u * BLK;
+          uint32_t w0[WORDS], w1[WORDS];       // words of tokens rho and rho + 8
+          read_words<4 * WORDS>(w0, kb + rho * ROW + c * (4 * WORDS));
+          read_words<4 * WORDS>(w1, kb + (rho + 8) * ROW + c * (4 * WORDS));
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (t0 + u * kKv4Rows + rho + 8 * t >= t_hi || (bad >> (stage * U + u) & 1u)) {
+          for (int g = 0; g < G; ++g) {
+            float acc[NT][4];
 #pragma unroll
-              for (int g = 0; g < G; ++g) kpair[u][t][g] = vpair[u][t][g] = 0u;
+            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+            for (int w = g; w < WORDS; w += G) {
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const uint32_t x = w0[w] >> (4 * i), y = w1[w] >> (4 * i);
+                const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) Mma::run(acc[nt], a, qf[nt][w][i], qf[nt][w][i + 1]);
+              }
             }
-      }
-      // ---- scores
-      float s[U][NT][4];
+            const float2 p0 = unpack_pair(T{}, kpair[u][0][g]), p1 = unpack_pair(T{}, kpair[u][1][g]);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned char* const kb = step_at + u * (2 * BLK);
-        uint32_t w0[WORDS], w1[WORDS];       // words of tokens rho and rho + 8
-        read_words<4 * WORDS>(w0, kb + rho * ROW + c * (4 * WORDS));
-        read_words<4 * WORDS>(w1, kb + (rho + 8) * ROW + c * (4 * WORDS));
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          float acc[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
-          for (int w = g; w < WORDS; w += G) {
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const uint32_t x = w0[w] >> (4 * i), y = w1[w] >> (4 * i);
-              const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) Mma::run(acc[nt], a, qf[nt][w][i], qf[nt][w][i + 1]);
+              for (int j = 0; j < 2; ++j) {
+                s[u][nt][j] = fmaf(p0.x, acc[nt][j], g == 0 ? p0.y * qs[nt][g][j] : fmaf(p0.y, qs[nt][g][j], s[u][nt][j]));
+                s[u][nt][2 + j] = fmaf(p1.x, acc[nt][2 + j], g == 0 ? p1.y * qs[nt][g][j] : fmaf(p1.y, qs[nt][g][j], s[u][nt][2 + j]));
+              }
             }
           }
-          const float2 p0 = unpack_pair(T{}, kpair[u][0][g]), p1 = unpack_pair(T{}, kpair[u][1][g]);
+        }
+        float smax = 0.f;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            smax = max3(smax, unpack_pair(T{}, vpair[u][0][g]).x, unpack_pair(T{}, vpair[u][1][g]).x);
+        // ---- exponents over the reference (one that is not there yet is far below every score)
+        float x[N][NT][4], over = -INFINITY;
+        auto seen = [&](int u, int nt, int j) -> bool {
+          const int t = t0 + u * kKv4Rows + rho + 8 * (j >> 1);
+          if constexpr (!BLOCKS) return t < t_hi;
+          const int pos = prefix + tok[nt][j & 1];
+          return t < t_hi && (p.is_cross || t <= pos) && (p.window == 0 || t > pos - p.window);
+        };
+        const bool edge = t0 + N * kKv4Rows > all_hi || t0 < all_lo;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[u][nt][j] *= cscale[nt][j & 1];
+          }
+        if (edge) {
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[u][nt][j] = seen(u, nt, j) ? s[u][nt][j] : -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][nt][j] = s[u][nt][j] - m[nt][j & 1];
+            over = max3(max3(over, x[u][nt][0], x[u][nt][1]), x[u][nt][2], x[u][nt][3]);
+          }
+        if (__any_sync(0xffffffffu, over > limit || smax > vlim)) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
+          if (smax > vlim) {
+            const uint32_t e = (__float_as_uint(smax) >> 23) + 1;
+            vlim = __uint_as_float(e << 23);
+            limit = kSlack - max(static_cast<int>(e) - 127, kLeastExponent);
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              s[u][nt][j] = fmaf(p0.x, acc[nt][j], g == 0 ? p0.y * qs[nt][g][j] : fmaf(p0.y, qs[nt][g][j], s[u][nt][j]));
-              s[u][nt][2 + j] = fmaf(p1.x, acc[nt][2 + j], g == 0 ? p1.y * qs[nt][g][j] : fmaf(p1.y, qs[nt][g][j], s[u][nt][2 + j]));
-            }
-          }
-        }
-      }
-      float smax = 0.f;
+              float mx = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+              for (int u = 0; u < N; ++u) mx = max3(mx, s[u][nt][j], s[u][nt][2 + j]);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-          smax = max3(smax, unpack_pair(T{}, vpair[u][0][g]).x, unpack_pair(T{}, vpair[u][1][g]).x);
-      // ---- exponents over the reference (one that is not there yet is far below every score)
-      float x[U][NT][4], over = -INFINITY;
-      auto seen = [&](int u, int nt, int j) -> bool {
-        const int t = t0 + u * kKv4Rows + rho + 8 * (j >> 1);
-        if constexpr (!BLOCKS) return t < t_hi;
-        const int pos = prefix + tok[nt][j & 1];
-        return t < t_hi && (p.is_cross || t <= pos) && (p.window == 0 || t > pos - p.window);
-      };
-      const bool edge = t0 + U * kKv4Rows > all_hi || t0 < all_lo;
+              for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              mx = fmaxf(mx + (kSlack - limit), m[nt][j]);
+              const float a = fast_exp2(m[nt][j] - mx);
+              m[nt][j] = mx;
+              l[nt][j] *= a;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+              for (int g = 0; g < G; ++g) {
+                pbias[nt][g][j] *= a;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+                for (int i = 0; i < 4; ++i) {
+                  o[nt][g][i][j] *= a;
+                  o[nt][g][i][2 + j] *= a;
+                }
+              }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[u][nt][j] *= cscale[nt][j & 1];
-        }
-      if (edge) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[u][nt][j] = seen(u, nt, j) ? s[u][nt][j] : -INFINITY;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[u][nt][j] = s[u][nt][j] - m[nt][j & 1];
-          over = max3(max3(over, x[u][nt][0], x[u][nt][1]), x[u][nt][2], x[u][nt][3]);
-        }
-      if (__any_sync(0xffffffffu, over > limit || smax > vlim)) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
-        if (smax > vlim) {
-          const uint32_t e = (__float_as_uint(smax) >> 23) + 1;
-          vlim = __uint_as_float(e << 23);
-          limit = kSlack - max(static_cast<int>(e) - 127, kLeastExponent);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < U; ++u) mx = max3(mx, s[u][nt][j], s[u][nt][2 + j]);
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            mx = fmaxf(mx + (kSlack - limit), m[nt][j]);
-            const float a = fast_exp2(m[nt][j] - mx);
-            m[nt][j] = mx;
-            l[nt][j] *= a;
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-              pbias[nt][g][j] *= a;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                o[nt][g][i][j] *= a;
-                o[nt][g][i][2 + j] *= a;
+              for (int u = 0; u < N; ++u) {
+                x[u][nt][j] = s[u][nt][j] - mx;
+                x[u][nt][2 + j] = s[u][nt][2 + j] - mx;
               }
             }
+          }
+        }
+        uint32_t pf[N][NT][G][2];      // P_g as B fragments
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              x[u][nt][j] = s[u][nt][j] - mx;
-              x[u][nt][2 + j] = s[u][nt][2 + j] - mx;
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][nt][j] = fast_exp2(x[u][nt][j]);
+            l[nt][0] += x[u][nt][0] + x[u][nt][2];
+            l[nt][1] += x[u][nt][1] + x[u][nt][3];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float2 p0 = unpack_pair(T{}, vpair[u][0][g]), p1 = unpack_pair(T{}, vpair[u][1][g]);
+              pbias[nt][g][0] = fmaf(x[u][nt][0], p0.y, fmaf(x[u][nt][2], p1.y, pbias[nt][g][0]));
+              pbias[nt][g][1] = fmaf(x[u][nt][1], p0.y, fmaf(x[u][nt][3], p1.y, pbias[nt][g][1]));
+              pf[u][nt][g][0] = transpose_8x8(Mma::pack(x[u][nt][0] * p0.x, x[u][nt][1] * p0.x));
+              pf[u][nt][g][1] = transpose_8x8(Mma::pack(x[u][nt][2] * p1.x, x[u][nt][3] * p1.x));
+            }
+          }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          const unsigned char* const vb = step_at + (U + u) * BLK + r * (4 * G);
+          uint32_t v0[G], v1[G], v2[G], v3[G];      // word r of tokens tv, tw, tv + 8, tw + 8
+          read_words<4 * G>(v0, vb + tv * ROW);
+          read_words<4 * G>(v1, vb + tw * ROW);
+          read_words<4 * G>(v2, vb + (tv + 8) * ROW);
+          read_words<4 * G>(v3, vb + (tw + 8) * ROW);
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const uint32_t lo0 = __byte_perm(v0[g], v1[g], 0x5410), hi0 = __byte_perm(v0[g], v1[g], 0x7632);
+            const uint32_t lo1 = __byte_perm(v2[g], v3[g], 0x5410), hi1 = __byte_perm(v2[g], v3[g], 0x7632);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu;
+              const uint32_t a[4] = {lo0 >> (8 * (i >> 1)) & mask, hi0 >> (8 * (i >> 1)) & mask, lo1 >> (8 * (i >> 1)) & mask,
+                                     hi1 >> (8 * (i >> 1)) & mask};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) Mma::run(o[nt][g][i], a, pf[u][nt][g][0], pf[u][nt][g][1]);
             }
           }
         }
-      }
-      uint32_t pf[U][NT][G][2];      // P_g as B fragments
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[u][nt][j] = fast_exp2(x[u][nt][j]);
-          l[nt][0] += x[u][nt][0] + x[u][nt][2];
-          l[nt][1] += x[u][nt][1] + x[u][nt][3];
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const float2 p0 = unpack_pair(T{}, vpair[u][0][g]), p1 = unpack_pair(T{}, vpair[u][1][g]);
-            pbias[nt][g][0] = fmaf(x[u][nt][0], p0.y, fmaf(x[u][nt][2], p1.y, pbias[nt][g][0]));
-            pbias[nt][g][1] = fmaf(x[u][nt][1], p0.y, fmaf(x[u][nt][3], p1.y, pbias[nt][g][1]));
-            pf[u][nt][g][0] = transpose_8x8(Mma::pack(x[u][nt][0] * p0.x, x[u][nt][1] * p0.x));
-            pf[u][nt][g][1] = transpose_8x8(Mma::pack(x[u][nt][2] * p1.x, x[u][nt][3] * p1.x));
-          }
-        }
-      // ---- O^T += V^T P^T
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned char* const vb = step_at + u * (2 * BLK) + BLK + r * (4 * G);
-        uint32_t v0[G], v1[G], v2[G], v3[G];      // word r of tokens tv, tw, tv + 8, tw + 8
-        read_words<4 * G>(v0, vb + tv * ROW);
-        read_words<4 * G>(v1, vb + tw * ROW);
-        read_words<4 * G>(v2, vb + (tv + 8) * ROW);
-        read_words<4 * G>(v3, vb + (tw + 8) * ROW);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const uint32_t lo0 = __byte_perm(v0[g], v1[g], 0x5410), hi0 = __byte_perm(v0[g], v1[g], 0x7632);
-          const uint32_t lo1 = __byte_perm(v2[g], v3[g], 0x5410), hi1 = __byte_perm(v2[g], v3[g], 0x7632);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu;
-            const uint32_t a[4] = {lo0 >> (8 * (i >> 1)) & mask, hi0 >> (8 * (i >> 1)) & mask, lo1 >> (8 * (i >> 1)) & mask,
-                                   hi1 >> (8 * (i >> 1)) & mask};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) Mma::run(o[nt][g][i], a, pf[u][nt][g][0], pf[u][nt][g][1]);
-          }
-        }
-      }
+      };
+      // (the last block of a segment, and the only one of a short sequence, by itself: a step of four takes 2900 cycles)
+      if (U > 1 && t0 + kKv4Rows >= t_hi) step(std::integral_constant<int, 1>{});
+      else step(std::integral_constant<int, U>{});
       __syncwarp();                 // every lane has read the stage: it is free
       issue(stage);
       if (++stage == STAGES) {

@@ -81,6 +81,7 @@ enum class PoolBox {
   kHead,   // 3-D (64 elements, slots, blocks of 64 elements of a row): 16 token rows x all head_dim elements of one head, a block
            // of columns after the other, as the decode kernel's tiles lie in shared memory.  (A copy instruction costs
            // its warp 67 cycles whatever its size: one per tile instead of two or four.)
+  kPacked, // 2-D, for tile::gather4: a pool held in 4 bits as rows of 1152 bytes (144 elements of 8), one or two to a block of a head
 };
 bool make_pool_map(CUtensorMap* out, PoolBox form, const void* base, int64_t num_slots, int num_kv_heads, int head_dim,
                    int dtype);

@@ -62,19 +62,20 @@ Q4Plan plan_q4(int batch, int columns, int hkv, int head_dim, int64_t blocks, in
 }
 
 template <typename T, int HD, int NT, bool BLOCKS, int U, int WARPS, int STAGES, int MINB>
-cudaError_t launch_q4(const msgl::Q4DecodeParams& p, cudaStream_t s) {
+cudaError_t launch_q4(const msgl::Q4DecodeParams& p, cudaStream_t s, const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
   auto* kernel = msgl::q4_decode_kernel<T, HD, NT, BLOCKS, U, WARPS, STAGES, MINB>;
   constexpr int smem = msgl::q4_decode_smem(HD, WARPS, STAGES * U);
   const cudaError_t e = allow_smem(kernel, smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(p.num_shares * p.col_tiles * p.hkv)), dim3(WARPS * 32), smem, s, p);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(p.num_shares * p.col_tiles * p.hkv)), dim3(WARPS * 32), smem, s, p, tm_k, tm_v);
 }
 template <bool BLOCKS>
-cudaError_t launch_q4_any(const msgl::Q4DecodeParams& p, int head_dim, int cols, int dtype, cudaStream_t s) {
+cudaError_t launch_q4_any(const msgl::Q4DecodeParams& p, int head_dim, int cols, int dtype, cudaStream_t s,
+                          const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
   auto go = [&](auto tag) -> cudaError_t {
     using T = decltype(tag);
-    if (head_dim == 256) return launch_q4<T, 256, 1, BLOCKS, 2, 8, 2, 1>(p, s);
-    return cols == 8 ? launch_q4<T, 128, 1, BLOCKS, 4, 4, 2, 2>(p, s) : launch_q4<T, 128, 2, BLOCKS, 2, 8, 3, 1>(p, s);
+    if (head_dim == 256) return launch_q4<T, 256, 1, BLOCKS, 2, 8, 2, 1>(p, s, tm_k, tm_v);
+    return cols == 8 ? launch_q4<T, 128, 1, BLOCKS, 4, 4, 2, 2>(p, s, tm_k, tm_v) : launch_q4<T, 128, 2, BLOCKS, 2, 8, 3, 1>(p, s, tm_k, tm_v);
   };
   return dtype == MSGL_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }
@@ -100,7 +101,16 @@ int run_q4(const char* op, msgl::Q4DecodeParams& p, const Q4Plan& pl, void* work
   p.num_shares = static_cast<int>(pl.shares);
   p.min_share = kQ4MinShare;
   p.pad = kQ4Pad;
-  const cudaError_t e = launch_q4_any<BLOCKS>(p, head_dim, pl.cols, dtype, s);
+  CUtensorMap tm_k, tm_v;
+  std::memset(&tm_k, 0, sizeof(tm_k));
+  std::memset(&tm_v, 0, sizeof(tm_v));
+  const int64_t slots = p.num_blocks * msgl::kKv4Rows;
+  if (slots == 0 && p.total_pages > 0) return fail(MSGL_BAD_SHAPE, std::string(op) + ": pages of a pool without slots");
+  p.num_rows = static_cast<int>(p.num_blocks * p.hkv * (head_dim / 128));
+  if (slots > 0 && (!make_pool_map(&tm_k, PoolBox::kPacked, p.k_pool, slots, p.hkv, head_dim, dtype) ||
+                    !make_pool_map(&tm_v, PoolBox::kPacked, p.v_pool, slots, p.hkv, head_dim, dtype)))
+    return fail(MSGL_CUDA_ERROR, std::string(op) + ": cannot build the tensor maps of the K/V pool");
+  const cudaError_t e = launch_q4_any<BLOCKS>(p, head_dim, pl.cols, dtype, s, tm_k, tm_v);
   return e == cudaSuccess ? MSGL_OK : cuda_fail(op, e);
 }
 
