@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
         for (int i = 0; i < 4; ++i) top = max(top, max(qf[nt][w][i] >> 16 & 0x7fffu, qf[nt][w][i] & 0x7fffu));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float power = row_power(T{}, top), inv = 1.f / power;
+      const float power = row_power(T{}, top), inv = power_inverse(power);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         cscale[nt][j] = p.scale_log2 * 1048576.f * __shfl_sync(0xffffffffu, power, (2 * c + j) * 4);

@@ -126,6 +126,8 @@ __device__ __forceinline__ float row_power(__half, uint32_t top) {
 __device__ __forceinline__ float row_power(__nv_bfloat16, uint32_t top) {
   return __uint_as_float((max(top >> 7, 12u) - 10u) << 23);
 }
+// 1 / power, exactly (its exponent field is 2 to 245).
+__device__ __forceinline__ float power_inverse(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 
 // A pair of type T as one of another type.
 template <typename T>
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4ExpandParams p
     for (int e = 0; e < 4; ++e) top = max(top, max(w[e] >> 16 & 0x7fffu, w[e] & 0x7fffu));
 #pragma unroll
     for (int o = 1; o < CH; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-    const float power = row_power(T{}, top), inv = 1.f / power;
+    const float power = row_power(T{}, top), inv = power_inverse(power);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 f = unpack_pair(T{}, w[e]);

@@ -1122,50 +1122,51 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     const bool sc_neg = !(p.scale_log2 > 0.f);
     float row_scale = p.scale_log2;
     if constexpr (CONVERT) {
-      // Q as f16, a warp its own 32 rows, CPR lanes a row, RU rows in flight a lane.  (By the copying warps, in front of their
-      // first tile: four chunks of 300 to 512 tokens over up to 4096 132 us for 104.)
-      constexpr int RP = 32 / CPR, RU = 8;              // rows a pass; passes in flight
-      const uint32_t mask = CPR == 32 ? 0xffffffffu : (lane & 16) ? 0xffff0000u : 0x0000ffffu;
-      const int chunk = lane % CPR;
+      // Q as f16.  A warp takes every fourth row of the sub-tile, all its lanes a row, RU rows in flight: 40 rows are ten a warp,
+      // and the largest magnitude is one reduction.  (Half a warp a row, each warp its own 32 rows: the first scores of 40 rows
+      // stood 10000 cycles later.  By the copying warps, in front of their first tile: four chunks of 300 to 512 tokens over up to
+      // 4096 132 us for 104.)
+      constexpr int RU = 8;                             // rows of a warp in flight
+      using Piece = typename std::conditional<HD == 128, uint2, uint4>::type;
+      constexpr int PW = HD / 64;                       // words of a lane
       unsigned char* const q_at = smem_raw + (q_smem - smem_u32(smem_raw)) + i * kTcQTileBytes;
-      if (ntiles > 0) {
+      const int have = min(rows_valid - i * SUB, SUB);
+      const int filled = have <= 0 || ntiles == 0 ? 0 : (have + 31) / 32 * 32;     // rows of warps that have any: zeros behind the last
 #pragma unroll 1
-        for (int b = 0; b < 32; b += RP * RU) {
-          uint4 x[RU];
+      for (int b = warp & 3; b < filled; b += 4 * RU) {
+        Piece x[RU];
 #pragma unroll
-          for (int u = 0; u < RU; ++u) {
-            const int at = i * SUB + (warp & 3) * 32 + b + u * RP + lane / CPR;
-            x[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (at < rows_valid) {
-              const int t = over_group(pk0 + at), g = pk0 + at - t * G;
-              x[u] = *reinterpret_cast<const uint4*>(
-                  static_cast<const T*>(p.q) +
-                  (static_cast<int64_t>(sq.q_begin + t) * p.hq + static_cast<int64_t>(h) * G + g) * HD + chunk * 8);
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < RU; ++u) {
-            const int at = (warp & 3) * 32 + b + u * RP + lane / CPR;
-            uint32_t* const w = reinterpret_cast<uint32_t*>(&x[u]);
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, max(w[e] >> 16 & 0x7fffu, w[e] & 0x7fffu));
-#pragma unroll
-            for (int o = 1; o < CPR; o <<= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-            const float power = row_power(T{}, top), inv = 1.f / power;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack_pair(T{}, w[e]);
-              w[e] = MmaOp<M>::pack(f.x * inv, f.y * inv);
-            }
-            *reinterpret_cast<uint4*>(q_at + tc_tile_offset<128>(at, chunk)) = x[u];
-            if (chunk == 0) s_row_power[i * SUB + at] = power;
+        for (int u = 0; u < RU; ++u) {
+          const int at = b + 4 * u;
+          x[u] = Piece{};
+          if (at < have) {
+            const int n = pk0 + i * SUB + at, t = over_group(n), g = n - t * G;
+            x[u] = reinterpret_cast<const Piece*>(static_cast<const T*>(p.q) +
+                                                  (static_cast<int64_t>(sq.q_begin + t) * p.hq + static_cast<int64_t>(h) * G + g) * HD)[lane];
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        row_scale *= s_row_power[row];
+#pragma unroll
+        for (int u = 0; u < RU; ++u) {
+          const int at = b + 4 * u;
+          if (at >= filled) break;
+          uint32_t* const w = reinterpret_cast<uint32_t*>(&x[u]);
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < PW; ++e) top = max(top, max(w[e] >> 16 & 0x7fffu, w[e] & 0x7fffu));
+          const float power = row_power(T{}, __reduce_max_sync(0xffffffffu, top)), inv = power_inverse(power);
+#pragma unroll
+          for (int e = 0; e < PW; ++e) {
+            const float2 f = unpack_pair(T{}, w[e]);
+            w[e] = MmaOp<M>::pack(f.x * inv, f.y * inv);
+          }
+          const int byte = lane * (PW * 4);
+          *reinterpret_cast<Piece*>(q_at + tc_tile_offset<128>(at, byte / 16) + byte % 16) = x[u];
+          if (lane == 0) s_row_power[i * SUB + at] = power;
+        }
       }
+      fence_proxy_async_smem();
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");      // (the four warps of the sub-tile)
+      row_scale *= s_row_power[row];
       if (lane == 0) mbar_arrive(bar_q);
     }
     const float sc = sc_neg ? 1.f : row_scale;
