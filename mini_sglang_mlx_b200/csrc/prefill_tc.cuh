@@ -394,6 +394,9 @@ __device__ __noinline__ void merge_kv_splits(const MergeArgs p, int nsp, int64_t
   }
 }
 
+// The four warps of a sub-tile.
+__device__ __forceinline__ void subtile_sync(int i) { asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory"); }
+
 // The same by the CTA that arrived last, NSW of its warps: the rows of all splits are copied into shared
 // memory with everything in flight at once, then a warp reduces a row at a time.  Straight from scratch, 8
 // rows in flight per warp, 64 rows x 2 splits took 6.7 us.  `buf`: `bytes` of free shared memory, holding
@@ -486,6 +489,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   using Shape = TcShape<NSUB, HD, PAGED>;
   using M = typename std::conditional<KV4, __half, T>::type;       // type of the operands
   constexpr bool CONVERT = !std::is_same<M, T>::value;
+  constexpr bool IN_PLACE = CONVERT && NSUB == 2;      // Q lands as it is and is converted there
   constexpr int kTcQTileBytes = Shape::kQTileBytes;
   constexpr int CPR = HD / 8;                          // 16-byte chunks of a token row
   constexpr int BM = Shape::kBM, SUB = kTcSub;
@@ -507,6 +511,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   constexpr int kRaw = KV4 ? Kv4Shape<NSUB, HD>::kRawSlots : 1;
   __shared__ uint64_t s_raw_full[kRaw], s_raw_empty[kRaw];   // KV4: fetched blocks
   __shared__ int s_raw_bad[kRaw];                             // their page is not in the pool
+  __shared__ uint64_t s_q_raw;                                // IN_PLACE: Q as it is has arrived
   __shared__ float s_row_power[CONVERT ? BM : 1];             // what a row of q was divided by
   __shared__ int s_slots[KV4 ? 1 : (LA + 1) * BN];  // slot ids of the key tiles being copied / next to copy
 
@@ -530,7 +535,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   auto bar_pv = [&](int i, int sb) { return smem_u32(&bars.pv_done[i][sb]); };
   // Q arrives as TMA boxes when the caller could describe it (query heads per KV head a power
   // of two), else as 16-byte copies by the producer threads
-  const bool q_tma = (PAGED || KV4) && !CONVERT && p.q_tma != 0;
+  const bool q_tma = (PAGED || KV4) && (!CONVERT || IN_PLACE) && p.q_tma != 0;
+  const uint32_t bar_q_in = IN_PLACE ? smem_u32(&s_q_raw) : bar_q;      // (what the copies arrive at)
 
   if (warp == 1) {
     // a barrier per lane.  (PAGED: per copying warp its 32 lanes, their cp.async arrivals, and the arrival that
@@ -538,7 +544,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     auto init = [&](uint64_t* first, int n, int count) {
       if (lane < n) mbar_init(smem_u32(first + lane), count);
     };
-    init(&bars.q_full, 1, q_tma ? 1 : CONVERT ? NSUB * SUB / 32 : NPROD);
+    init(&bars.q_full, 1, CONVERT ? NSUB * SUB / 32 : q_tma ? 1 : NPROD);
+    if constexpr (IN_PLACE) init(&s_q_raw, 1, q_tma ? 1 : NPROD);
     init(&bars.idx_sync, 1, NPROD);
     init(bars.full, kTcBufs, PAGED ? (NPROD / 32) * 33 : KV4 ? BN / kKv4Rows : NPROD);
     if constexpr (KV4) {
@@ -558,6 +565,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     tmem_relinquish();
   }
 
+  if (KV4 && q_tma && warp == 2 && lane == 0) prefetch_tensormap(&tm_q);
   if (!p.early) grid_dependency_wait();
   const bool by_warp = p.batch <= kWarpBatchMax;
   if (by_warp) {
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     auto load_q = [&]() {
     if (p.early) grid_dependency_wait();
     if (NSUB == 1 && ntiles == 0) return;      // (the epilogue's zeros are staged where Q would land)
-    if constexpr (CONVERT) return;             // (Q is the softmax warps')
+    if constexpr (CONVERT && !IN_PLACE) return;      // (Q is the softmax warps')
     if (q_tma) {
       // Q: one box per sub-tile and 64-element column block.  The tensor map is
       // (head_dim, query heads, tokens) with a box of 64 x G x 128/G, so the rows land in
@@ -668,12 +676,12 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       // the batch); they are computed on and never written out.
       if (warp == kTcProducerWarp0 && lane == 0) {
         prefetch_tensormap(&tm_q);
-        mbar_arrive_expect_tx(bar_q, nsub * kTcQTileBytes);
+        mbar_arrive_expect_tx(bar_q_in, nsub * kTcQTileBytes);
         for (int i = 0; i < nsub; ++i)
 #pragma unroll
           for (int c = 0; c < HD / 64; ++c)
             tma_load_3d(q_smem + i * kTcQTileBytes + c * (SUB * 128), &tm_q, c * 64, h * G,
-                        sq.q_begin + tok_first + i * (SUB / G), bar_q);
+                        sq.q_begin + tok_first + i * (SUB / G), bar_q_in);
       }
     } else {
       // Q: rows_valid packed rows, the rest zero
@@ -689,7 +697,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
         cp_async_16(q_smem + (row >> 7) * kTcQTileBytes + tc_tile_offset<128>(row & 127, chunk),
                     reinterpret_cast<const unsigned char*>(q + off) + chunk * 16, ok ? 16 : 0);
       }
-      cp_async_mbar_arrive(bar_q);
+      cp_async_mbar_arrive(bar_q_in);
     }
     };
 
@@ -917,16 +925,23 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_raw_empty[slot]));
+            if (left < kKv4Rows) {      // rows behind the keys, or of a page that is not there: zeros
+#pragma unroll
+              for (int i = 0; i < kKv4Rows / RPP; ++i)
+                if (i * RPP + rsub >= left) {
+#pragma unroll
+                  for (int w = 0; w < 4; ++w) words[i][w] = 0u;
+#pragma unroll
+                  for (int g = 0; g < G; ++g) pairs[i][g] = 0u;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kKv4Rows / RPP; ++i) {
-              const int row = i * RPP + rsub;
-              const bool in = row < left;
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
                 const int g = w % G, r8 = piece * (4 / G) + w / G;
-                uint4 x = kv4_values<M>(words[i][w], same_pair(T{}, M{}, pairs[i][g]));
-                if (!in) x = make_uint4(0u, 0u, 0u, 0u);
-                *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(blk * kKv4Rows + row, g * 8 + r8)) = x;
+                *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(blk * kKv4Rows + i * RPP + rsub, g * 8 + r8)) =
+                    kv4_values<M>(words[i][w], same_pair(T{}, M{}, pairs[i][g]));
               }
             }
             fence_proxy_async_smem();
@@ -1122,24 +1137,33 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     const bool sc_neg = !(p.scale_log2 > 0.f);
     float row_scale = p.scale_log2;
     if constexpr (CONVERT) {
-      // Q as f16.  A warp takes every fourth row of the sub-tile, all its lanes a row, RU rows in flight: 40 rows are ten a warp,
-      // and the largest magnitude is one reduction.  (Half a warp a row, each warp its own 32 rows: the first scores of 40 rows
-      // stood 10000 cycles later.  By the copying warps, in front of their first tile: four chunks of 300 to 512 tokens over up to
-      // 4096 132 us for 104.)
-      constexpr int RU = 8;                             // rows of a warp in flight
+      // Q as f16.  A warp takes every fourth row of the sub-tile, all its lanes a row, so that 40 rows are ten a warp and the
+      // largest magnitude is one reduction.  Two sub-tiles are converted in the place where they landed, by a short loop, because
+      // code that runs once is paid for by its size (from global memory, eight rows unrolled, 4000 cycles for the first
+      // eight and 1000 for the next: four chunks of 300 to 512 tokens over up to 4096 105 us for 97.7).  One sub-tile is the short one, of few
+      // rows, and comes straight from global memory (in place: five verify tokens of 16 requests 59.8 us for 57.5).
       using Piece = typename std::conditional<HD == 128, uint2, uint4>::type;
       constexpr int PW = HD / 64;                       // words of a lane
+      constexpr int RU = IN_PLACE ? 4 : 8;              // rows of a warp in flight
+      if constexpr (IN_PLACE) alive = mbar_wait_warp(smem_u32(&s_q_raw), 0, abort_flag);
       unsigned char* const q_at = smem_raw + (q_smem - smem_u32(smem_raw)) + i * kTcQTileBytes;
       const int have = min(rows_valid - i * SUB, SUB);
-      const int filled = have <= 0 || ntiles == 0 ? 0 : (have + 31) / 32 * 32;     // rows of warps that have any: zeros behind the last
+      const int filled = have <= 0 || ntiles == 0 || !alive ? 0 : (have + 31) / 32 * 32;     // rows of warps that have any
 #pragma unroll 1
       for (int b = warp & 3; b < filled; b += 4 * RU) {
         Piece x[RU];
+        auto place = [&](int at) {
+          const int byte = lane * (PW * 4);
+          return reinterpret_cast<Piece*>(q_at + tc_tile_offset<128>(at, byte / 16) + byte % 16);
+        };
 #pragma unroll
         for (int u = 0; u < RU; ++u) {
           const int at = b + 4 * u;
           x[u] = Piece{};
-          if (at < have) {
+          if (at >= have) continue;                     // (zeros behind the last; in place a neighbour's may stand there)
+          if constexpr (IN_PLACE) {
+            x[u] = *place(at);
+          } else {
             const int n = pk0 + i * SUB + at, t = over_group(n), g = n - t * G;
             x[u] = reinterpret_cast<const Piece*>(static_cast<const T*>(p.q) +
                                                   (static_cast<int64_t>(sq.q_begin + t) * p.hq + static_cast<int64_t>(h) * G + g) * HD)[lane];
@@ -1159,13 +1183,12 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
             const float2 f = unpack_pair(T{}, w[e]);
             w[e] = MmaOp<M>::pack(f.x * inv, f.y * inv);
           }
-          const int byte = lane * (PW * 4);
-          *reinterpret_cast<Piece*>(q_at + tc_tile_offset<128>(at, byte / 16) + byte % 16) = x[u];
+          *place(at) = x[u];
           if (lane == 0) s_row_power[i * SUB + at] = power;
         }
       }
       fence_proxy_async_smem();
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");      // (the four warps of the sub-tile)
+      subtile_sync(i);
       row_scale *= s_row_power[row];
       if (lane == 0) mbar_arrive(bar_q);
     }
