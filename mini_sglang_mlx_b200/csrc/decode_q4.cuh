@@ -41,6 +41,7 @@ struct Q4DecodeParams {
   const unsigned char *k_pool, *v_pool;
   const int32_t *page_indptr, *page_indices, *kv_lens;
   const int32_t *qo_indptr, *prefix_lens;   // BLOCKS
+  int total_q;                // BLOCKS: rows of q
   int page_blocks;            // blocks of 16 tokens per page
   int total_pages;            // entries of page_indices
   void* out;
@@ -143,8 +144,8 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
     k.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(lens + b), 0)), cap));
     k.first = 0;
     if constexpr (BLOCKS) {
-      k.tok0 = __ldg(p.qo_indptr + b);
-      k.new_tok = max(__ldg(p.qo_indptr + b + 1) - k.tok0, 0);
+      k.tok0 = min(max(__ldg(p.qo_indptr + b), 0), p.total_q);
+      k.new_tok = max(min(__ldg(p.qo_indptr + b + 1), p.total_q) - k.tok0, 0);
       k.prefix = __ldg(p.prefix_lens + b);
       const int hi = p.is_cross ? k.len : static_cast<int>(min(static_cast<int64_t>(k.len), static_cast<int64_t>(k.prefix) + k.new_tok));
       const int lo = p.window > 0 ? max(0, k.prefix - p.window + 1) : 0;
@@ -160,7 +161,12 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
   int sum = 0;
   for (int j = 0; j < run; ++j) {
     const int b = lane * run + j;
-    if (b < p.batch) sum += room(keys(b).blocks);
+    if (b < p.batch) sum = min(sum + room(keys(b).blocks), 1 << 28);
+  }
+  // (All pages of a call hold less than 2^27 blocks.  Row pointers that lay more end to end are none of a batch: no positions for them.)
+  if (__reduce_add_sync(0xffffffffu, sum >> 8) > 1 << 20) {
+    if (blockIdx.x == 0 && tid == 0 && p.status) atomicOr(p.status, 2);
+    return;
   }
   int incl = sum;
 #pragma unroll

@@ -26,6 +26,9 @@ int check_pool(const char* op, int num_kv_heads, int head_dim, int64_t num_slots
   if (num_slots % msgl::kKv4Rows != 0 || num_slots >= (1ll << 31))
     return fail(MSGL_BAD_SHAPE, std::string(op) + "num_slots must be a multiple of 16 below 2^31");
   if (num_kv_heads > 65535) return fail(MSGL_BAD_SHAPE, std::string(op) + "num_kv_heads must be <= 65535");
+  // (decode addresses a pool as rows of 1152 bytes, by 32 bits: 2.4 TB)
+  if (num_slots / msgl::kKv4Rows * num_kv_heads * (head_dim / 128) >= (1ll << 31))
+    return fail(MSGL_BAD_SHAPE, std::string(op) + "the pool has too many rows");
   return MSGL_OK;
 }
 
@@ -422,6 +425,7 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     p.page_indices = page_indices;
     p.kv_lens = kv_lens;
     p.qo_indptr = qo_indptr;
+    p.total_q = total_q;
     p.prefix_lens = prefix_lens;
     p.page_blocks = page_size / msgl::kKv4Rows;
     p.total_pages = static_cast<int>(total_pages);

@@ -52,29 +52,14 @@ __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The 16-bit numbers OFF + n of nibble i of both halves of a word, and OFF.
-template <typename T>
-struct Nibble;
-template <>
-struct Nibble<__nv_bfloat16> {    // seven bits of fraction: a nibble in the lowest four counts from 128, one at bit 3 from 16
-  __host__ __device__ static constexpr float off(int i) { return i == 0 ? 128.f : 16.f; }
-  __device__ __forceinline__ static uint32_t make(uint32_t w, int i) {
-    return i == 0 ? ((w & 0x000f000fu) | 0x43004300u) : (((w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u);
-  }
-};
-template <>
-struct Nibble<__half> {           // ten bits of fraction: at bit 4, 4, 2 and 6
-  __host__ __device__ static constexpr float off(int i) { return i < 2 ? 64.f : i == 2 ? 256.f : 16.f; }
-  __device__ __forceinline__ static uint32_t make(uint32_t w, int i) {
-    return i == 0   ? (((w << 4) & 0x00f000f0u) | 0x54005400u)
-           : i == 1 ? ((w & 0x00f000f0u) | 0x54005400u)
-           : i == 2 ? (((w >> 6) & 0x003c003cu) | 0x5c005c00u)
-                    : (((w >> 6) & 0x03c003c0u) | 0x4c004c00u);
-  }
-};
-// A constant in both halves.
-template <typename T>
-__device__ __forceinline__ uint32_t both(float x) { return MmaOp<T>::pack(x, x); }
+// The f16 numbers off + n of nibble i of both halves of a word, and off.  (Ten bits of fraction: the nibble at bit 4, 4, 2 and 6.)
+__host__ __device__ constexpr float nibble_off(int i) { return i < 2 ? 64.f : i == 2 ? 256.f : 16.f; }
+__device__ __forceinline__ uint32_t nibble_f16(uint32_t w, int i) {
+  return i == 0   ? (((w << 4) & 0x00f000f0u) | 0x54005400u)
+         : i == 1 ? ((w & 0x00f000f0u) | 0x54005400u)
+         : i == 2 ? (((w >> 6) & 0x003c003cu) | 0x5c005c00u)
+                  : (((w >> 6) & 0x03c003c0u) | 0x4c004c00u);
+}
 
 // BYTES at an aligned address, four to a word.
 template <int BYTES>
@@ -95,25 +80,20 @@ __device__ __forceinline__ void read_words(uint32_t (&r)[BYTES / 4], const unsig
   }
 }
 
-// The eight elements of a word under a pair, in order: scale * code + bias, rounded once.
-__device__ __forceinline__ uint32_t fma_pair(__nv_bfloat16, uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t fma_pair(__half, uint32_t a, uint32_t b, uint32_t c) {
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-template <typename T>
+// The eight elements of a word under an f16 pair, in order: scale * code + bias in f16, rounded once (half a unit, 2^-12 of the
+// element where T is bf16, whose own unit is sixteen times that).
 __device__ __forceinline__ uint4 kv4_values(uint32_t word, uint32_t pair) {
   const uint32_t scale = __byte_perm(pair, pair, 0x1010), bias = __byte_perm(pair, pair, 0x3232);
   uint32_t v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t n = fma_pair(T{}, Nibble<T>::make(word, i), both<T>(1.f), both<T>(-Nibble<T>::off(i)));   // exact
-    v[i] = fma_pair(T{}, n, scale, bias);
+    const uint32_t one = MmaOp<__half>::pack(1.f, 1.f), off = MmaOp<__half>::pack(-nibble_off(i), -nibble_off(i));
+    v[i] = fma_f16x2(fma_f16x2(nibble_f16(word, i), one, off), scale, bias);         // (the inner one is exact)
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
@@ -129,10 +109,9 @@ __device__ __forceinline__ float row_power(__nv_bfloat16, uint32_t top) {
 // 1 / power, exactly (its exponent field is 2 to 245).
 __device__ __forceinline__ float power_inverse(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 
-// A pair of type T as one of another type.
-template <typename T>
-__device__ __forceinline__ uint32_t same_pair(T, T, uint32_t pair) { return pair; }
-__device__ __forceinline__ uint32_t same_pair(__nv_bfloat16, __half, uint32_t pair) {
+// A pair of type T in f16: exact from 2^-14 on (what the pool holds is below 2^15), below that to 2^-25.
+__device__ __forceinline__ uint32_t f16_pair(__half, uint32_t pair) { return pair; }
+__device__ __forceinline__ uint32_t f16_pair(__nv_bfloat16, uint32_t pair) {
   const float2 x = unpack_pair(__nv_bfloat16{}, pair);
   return MmaOp<__half>::pack(x.x, x.y);
 }
@@ -220,7 +199,7 @@ struct Kv4StoreParams {
   int64_t k_stride, v_stride; // elements between tokens
   int64_t num_slots;
   int n, hkv;
-  uint32_t hkv_recip;         // see row_of_token
+  uint32_t hkv_recip;         // see token_of
   int wide;                   // rows are 16-byte aligned
   int* status;
 };
@@ -376,7 +355,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4ExpandParams p
 #pragma unroll
       for (int k = 0; k < kKv4Rows / RPP; ++k)
         *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(k * RPP + rsub) * p.hkv * HD) =
-            kv4_values<__half>(word[k], same_pair(T{}, __half{}, pair[k]));
+            kv4_values(word[k], f16_pair(T{}, pair[k]));
     }
   }
   if (q == nullptr) return;

@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
               for (int w = 0; w < 4; ++w) {
                 const int g = w % G, r8 = piece * (4 / G) + w / G;
                 *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(blk * kKv4Rows + i * RPP + rsub, g * 8 + r8)) =
-                    kv4_values<M>(words[i][w], same_pair(T{}, M{}, pairs[i][g]));
+                    kv4_values(words[i][w], f16_pair(T{}, pairs[i][g]));
               }
             }
             fence_proxy_async_smem();

@@ -75,6 +75,7 @@ EVERY = ("store", "load", "project", "decode", "prefill")
     (EVERY, dict(dtype=7), 2, "unsupported dtype"),
     (EVERY, dict(slots=24), 1, "multiple of 16"),
     (EVERY, dict(slots=1 << 31), 1, "below 2^31"),
+    (EVERY, dict(slots=(1 << 31) - 16, hkv=17), 1, "too many rows"),
     (EVERY, dict(hkv=0), 1, ""),
     (EVERY, dict(n=-1), 1, ""),
     (EVERY, dict(), 5, "null tensor pointer"),
@@ -514,3 +515,29 @@ def test_a_long_prefill_without_memory_for_its_pages(monkeypatch):
         _lib.host.set_pages_maker(K._make_pages)
     # two forms, each within half a unit of the output and its operands' roundings of the other
     assert float((got.double() - want.double()).norm() / want.double().norm()) <= 2 * half_unit(BF16)
+
+
+@pytest.mark.gpu
+def test_row_pointers_that_fit_no_batch():
+    """Page pointers that lay more blocks end to end than any batch holds are reported and nothing is read; query pointers beyond
+    the rows of q end with them."""
+    gen = torch.Generator().manual_seed(12)
+    q, decode = _call("decode", gen, [300, 17])
+    before = decode()
+    batch, pages = 16384, 4096
+    kc = torch.zeros(K.kv_cache_q4_shape(4096, 1, 128), dtype=BF16, device="cuda")
+    ends = torch.tensor([0, pages] * (batch // 2) + [0]).int().cuda()
+    ids = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    K.paged_decode_attention_q4(torch.ones(batch, 1, 128, dtype=BF16, device="cuda"), kc, kc, ends, ids,
+                                torch.full((batch,), 1 << 20, dtype=torch.int32, device="cuda"), 0.1, page_size=256)
+    assert K.device_status() == 2
+    assert torch.equal(decode(), before) and K.device_status() == 0
+
+    kc, vc, indptr, order, _ = sequences(gen, [50, 40], 16, 4, 128, BF16)
+    q = torch.randn(5, 16, 128, generator=gen).to(BF16).cuda()
+
+    def attend(qo):
+        return K.paged_prefill_attention_q4(q, kc, vc, torch.tensor(qo).int().cuda(), indptr.cuda(), order.cuda(),
+                                            torch.tensor([50, 40]).int().cuda(), torch.tensor([47, 38]).int().cuda(), 0.1, 4)
+
+    assert torch.equal(attend([0, 3, 9]), attend([0, 3, 5]))
