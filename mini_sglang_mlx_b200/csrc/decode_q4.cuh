@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ uint64_t s_bar[WARPS * STAGES];
-  __shared__ int s_last;
+  __shared__ int s_last[2];
   struct Keys {
     int page0, len;      // its first page, its tokens (clamped to what the pages hold)
     int first, blocks;   // blocks with a key that some of its columns see
@@ -638,6 +638,9 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
         const int cc = e / (HD / 4), d = e % (HD / 4) * 4;
         const int col = nt * 8 + cc;
         if (col >= cs.cols) break;
+        const int64_t at = row_of(b, cs.k.tok0, col) * HD + d;
+        uint2 gate = make_uint2(0u, 0u);
+        if (whole && p.gate != nullptr) gate = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.gate) + at);
         float M = -INFINITY, den = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_ml[(w * 8 + cc) * 2]);
@@ -655,14 +658,9 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
         }
         if (whole) {
           const float inv = den == 0.f ? 0.f : 1.f / den;
-          const int64_t at = row_of(b, cs.k.tok0, col) * HD + d;
-          alignas(8) T y[4] = {MmaOp<T>::from_float(x.x * inv), MmaOp<T>::from_float(x.y * inv),
-                               MmaOp<T>::from_float(x.z * inv), MmaOp<T>::from_float(x.w * inv)};
-          if (p.gate != nullptr) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = apply_gate<T>(to_f32(y[k]), static_cast<const T*>(p.gate)[at + k]);
-          }
-          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = *reinterpret_cast<const uint2*>(y);
+          uint2 y = make_uint2(MmaOp<T>::pack(x.x * inv, x.y * inv), MmaOp<T>::pack(x.z * inv, x.w * inv));
+          if (p.gate != nullptr) y = make_uint2(apply_gate_pair<T>(y.x, gate.x), apply_gate_pair<T>(y.y, gate.y));
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = y;
         } else {
           float* to = p.part + (slot + col) * PROW;
           *reinterpret_cast<float4*>(to + d) = x;
@@ -680,14 +678,15 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
   }
 
   // ---- the CTA that arrives last at a (sequence, head) merges its pieces
+  if (tid < parts) {         // (a thread each: an arrival takes 2000 cycles)
+    const int i = tid;
+    int* ticket = p.tickets + (static_cast<int64_t>(part_b[i]) * p.hkv + h) * p.col_tiles + ct;
+    s_last[i] = atomic_add_acq_rel(ticket, 1) == part_count[i] - 1;   // (the others' rows: behind the CTA barrier above)
+    if (s_last[i]) *ticket = 0;
+  }
+  __syncthreads();
   for (int i = 0; i < parts; ++i) {
-    if (tid == 0) {
-      int* ticket = p.tickets + (static_cast<int64_t>(part_b[i]) * p.hkv + h) * p.col_tiles + ct;
-      s_last = atomic_add_acq_rel(ticket, 1) == part_count[i] - 1;   // (the others' rows: behind the CTA barrier above)
-      if (s_last) *ticket = 0;
-    }
-    __syncthreads();
-    if (s_last) {
+    if (s_last[i]) {
       const int64_t pitch = 2ll * p.hkv * p.col_tiles * COLS * PROW;          // from share to share
       const float* rows = p.part + part_first[i] * pitch + (static_cast<int64_t>(h) * p.col_tiles + ct) * COLS * PROW;
       const int n = part_count[i];
@@ -696,6 +695,10 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
       for (int e = tid; e < cols * (HD / 4); e += WARPS * 32) {
         const int col = e / (HD / 4), d = e % (HD / 4) * 4;
         const float* row = rows + col * PROW;
+        const int head = BLOCKS ? (ct * COLS + col) % p.group : ct * COLS + col;
+        const int64_t at = ((BLOCKS ? k.tok0 + (ct * COLS + col) / p.group : static_cast<int64_t>(part_b[i])) * p.hq + h * p.group + head) * HD + d;
+        uint2 gate = make_uint2(0u, 0u);
+        if (p.gate != nullptr) gate = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.gate) + at);
         auto piece = [&](int k) { return row + k * pitch + (k == 0 ? pitch / 2 : 0); };
         float M = -INFINITY, den = 0.f;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -731,18 +734,11 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
           }
         }
         const float inv = den == 0.f ? 0.f : 1.f / den;
-        const int head = BLOCKS ? (ct * COLS + col) % p.group : ct * COLS + col;
-        const int64_t at = ((BLOCKS ? k.tok0 + (ct * COLS + col) / p.group : static_cast<int64_t>(part_b[i])) * p.hq + h * p.group + head) * HD + d;
-        alignas(8) T y[4] = {MmaOp<T>::from_float(x.x * inv), MmaOp<T>::from_float(x.y * inv),
-                             MmaOp<T>::from_float(x.z * inv), MmaOp<T>::from_float(x.w * inv)};
-        if (p.gate != nullptr) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = apply_gate<T>(to_f32(y[k]), static_cast<const T*>(p.gate)[at + k]);
-        }
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = *reinterpret_cast<const uint2*>(y);
+        uint2 y = make_uint2(MmaOp<T>::pack(x.x * inv, x.y * inv), MmaOp<T>::pack(x.z * inv, x.w * inv));
+        if (p.gate != nullptr) y = make_uint2(apply_gate_pair<T>(y.x, gate.x), apply_gate_pair<T>(y.y, gate.y));
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = y;
       }
     }
-    __syncthreads();
   }
   if (!alive) {       // gave up: what is still on its way lands before the shared memory goes away; bounded
     if (p.status && lane == 0) atomicOr(p.status, 1);
