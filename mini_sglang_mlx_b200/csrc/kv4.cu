@@ -32,24 +32,30 @@ int check_pool(const char* op, int num_kv_heads, int head_dim, int64_t num_slots
   return MSGL_OK;
 }
 
-constexpr int64_t kItemsFill = 148 * 32;     // groups of lanes that keep a B200 busy
+// Groups of lanes that keep a B200 busy.
+constexpr int64_t kItemsFill = 148 * 32;
+// CTAs of 256 threads for so many threads' work, at most `per_sm` of them per SM (the kernels step through the rest).
 unsigned grid_of(int64_t threads, int per_sm) {
   int sms = sm_count_cached();
   if (sms <= 0) sms = 148;
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, static_cast<int64_t>(sms) * per_sm)));
 }
 
-// ---- decode scheduling, in blocks of 16 tokens
+// ---- decode scheduling, in blocks of 16 tokens.  A share holds at least kQ4MinShare of them (4: geometric mean of twelve decode
+// shapes, one to 61 sequences and 108 to 441093 tokens, 15.88 us, 8: 15.76, 16: 16.33), and the end of a segment counts for
+// kQ4Pad (6: 17.0 us, 12: 15.76, 20: 15.68).  Batches of so many blocks that a wave's shares would be longer than kQ4MaxShare get
+// whole waves more (2^31 tokens are then 131072 shares, and positions stay far from 32 bits).
 constexpr int kQ4MinShare = 8;
 constexpr int kQ4MaxShare = 1024;
-constexpr int kQ4Pad = 12;
+constexpr int kQ4Pad = 20;
 
 struct Q4Plan {
   int col_tiles, cols;       // CTAs side by side, columns of each
   int64_t shares;
   size_t ticket_bytes, part_bytes;
 };
-// `columns` of a sequence at most, `blocks` of all sequences at most.
+// `columns` of a sequence at most, `blocks` of all sequences at most.  Sixteen columns a CTA where a warp's registers hold
+// them (head_dim 128): the second eight cost 375 cycles a block on top of 460, and 460 in a CTA of their own.
 Q4Plan plan_q4(int batch, int columns, int hkv, int head_dim, int64_t blocks, int sms) {
   Q4Plan pl{};
   pl.cols = head_dim == 128 && columns > 8 ? 16 : 8;
@@ -72,6 +78,10 @@ cudaError_t launch_q4(const msgl::Q4DecodeParams& p, cudaStream_t s, const CUten
   if (e != cudaSuccess) return e;
   return launch_dependent(kernel, dim3(static_cast<unsigned>(p.num_shares * p.col_tiles * p.hkv)), dim3(WARPS * 32), smem, s, p, tm_k, tm_v);
 }
+// Blocks a step, warps, stages of the ring and CTAs per SM, by what fits (255 registers at eight warps an SM).  Eight columns of 128,
+// 441093 tokens: 4 blocks, 4 warps, 2 CTAs 109 us; 2, 4, 3 CTAs 115; 4, 8, one CTA 125; 2, 12, one 129.  Head_dim 256, 97061
+// tokens: 2 blocks, 8 warps, one CTA 29.3 us; 2, 4, two CTAs 32.1; 1, 12, one 33.9; 1, 4, three 38.4.  (Measured with
+// a copy for each block; 99 and 26.1 us since.)  Sixteen columns: 2 blocks and a third stage, for their sums take twice the registers.
 template <bool BLOCKS>
 cudaError_t launch_q4_any(const msgl::Q4DecodeParams& p, int head_dim, int cols, int dtype, cudaStream_t s,
                           const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
@@ -117,7 +127,9 @@ int run_q4(const char* op, msgl::Q4DecodeParams& p, const Q4Plan& pl, void* work
   return e == cudaSuccess ? MSGL_OK : cuda_fail(op, e);
 }
 
-// Query blocks of few columns per KV head run the decode kernel (decode_q4.cuh), others the one-CTA tcgen05 kernel.
+// Query blocks of few columns per KV head run the decode kernel (decode_q4.cuh), others the one-CTA tcgen05 kernel.  16 sequences of
+// 16384 tokens, 8 KV heads, decode kernel / tcgen05: 8 columns 69 us / 222, 16 columns 115 / 222; with 20 to 64 columns as CTAs of
+// 16 side by side, five verify tokens of 40 columns 81 / 63, draft blocks of 64 149 / 86 (56 and 72 since).
 constexpr int kQ4BlockColumns = 16;
 bool q4_block_form(int max_len_extend, int group) {
   return static_cast<int64_t>(max_len_extend) * group <= kQ4BlockColumns;

@@ -191,7 +191,9 @@ __device__ __forceinline__ uint32_t token_of(uint32_t row, uint32_t heads, uint3
   return t * heads > row ? t - 1 : t;
 }
 
-// Eight lanes a group, sixteen bytes of K and as many of V a lane.  What bounds it is instruction issue.
+// Eight lanes a group, sixteen bytes of K and as many of V a lane: one exchange of (max, -min) over eight lanes, and K and V of a row
+// under one look-up of its slot.  What bounds it is instruction issue (a quotient and a rounding for every element): 65536 rows of
+// 8 heads of 128, 117 us, 4.6 TB/s of 532 MB with the read back; few rows are one launch.
 struct Kv4StoreParams {
   unsigned char *k_pool, *v_pool;
   const void *k, *v;          // (n, hkv, head_dim), dense heads
@@ -253,6 +255,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreParams p) {
 }
 
 // ---------------------------------------------------------------- rows out of the pool
+// A word and its pair a lane, eight elements in order, rounded once from fp32.  Bound by memory.
 struct Kv4LoadParams {
   const unsigned char *k_pool, *v_pool;
   void *k, *v;                // (n, hkv, head_dim), contiguous
