@@ -192,8 +192,9 @@ __device__ __forceinline__ uint32_t token_of(uint32_t row, uint32_t heads, uint3
 }
 
 // Eight lanes a group, sixteen bytes of K and as many of V a lane: one exchange of (max, -min) over eight lanes, and K and V of a row
-// under one look-up of its slot.  What bounds it is instruction issue (a quotient and a rounding for every element): 65536 rows of
-// 8 heads of 128, 117 us, 4.6 TB/s of 532 MB with the read back; few rows are one launch.
+// under one look-up of its slot.  What bounds it is instruction issue (a quotient and a rounding for every element): 49152 tokens of
+// 8 heads of 128 stored and read back, two launches, 118 us, 4.5 TB/s (with an exchange for each end and one quotient at a
+// time 143); 24 tokens 8.7.
 struct Kv4StoreParams {
   unsigned char *k_pool, *v_pool;
   const void *k, *v;          // (n, hkv, head_dim), dense heads
@@ -307,7 +308,8 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
 // A long prefill reads a key once for every 256 query rows, and to expand its codes each time is what bounds the kernel that does
 // (one CTA; 4096 tokens over 16384 1425 us).  Expanded once into f16 pages, one per entry of the index list and
 // in its order, they come by TMA and pairs of CTAs share them.  q goes with them, as f16 over a power of two per row (bf16 only).
-// Bound by memory: 2.6 bytes an element of the pool, 4 of q.
+// Bound by memory: 2.6 bytes an element of the pool, 4 of q; 20480 tokens of 8 heads of 128 and 4096 queries of 32 heads 34 us, 5.2
+// TB/s, in front of an attention of 1010 (with 116 registers and two CTAs per SM 44).
 struct Kv4ExpandParams {
   const unsigned char *k_pool, *v_pool;
   const int32_t* page_indices;
@@ -322,7 +324,7 @@ struct Kv4ExpandParams {
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4ExpandParams p) {
+__global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const Kv4ExpandParams p) {
   constexpr int CH = HD / 8, G = HD / kKv4Group, RPP = 32 / CH;      // chunks of a row; rows a pass of a warp
   grid_dependency_wait();
   grid_dependency_launch();
