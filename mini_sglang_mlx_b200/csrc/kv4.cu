@@ -239,7 +239,7 @@ int msgl_load_kv_cache_q4(const void* k_cache, const void* v_cache, const int32_
                                                              : msgl::kv4_load_kernel<__half, 256>)
                                  : (dtype == MSGL_DTYPE_BF16 ? msgl::kv4_load_kernel<__nv_bfloat16, 128>
                                                              : msgl::kv4_load_kernel<__half, 128>);
-  const cudaError_t e = launch_dependent(kernel, dim3(grid_of(static_cast<int64_t>(length) * num_kv_heads * head_dim / 8, 16)),
+  const cudaError_t e = launch_dependent(kernel, dim3(grid_of(static_cast<int64_t>(length) * num_kv_heads * head_dim / 16, 16)),
                                          dim3(256), 0, static_cast<cudaStream_t>(stream), p);
   return e == cudaSuccess ? MSGL_OK : cuda_fail("load_kv_cache_q4", e);
 }

@@ -193,8 +193,8 @@ __device__ __forceinline__ uint32_t token_of(uint32_t row, uint32_t heads, uint3
 
 // Eight lanes a group, sixteen bytes of K and as many of V a lane: one exchange of (max, -min) over eight lanes, and K and V of a row
 // under one look-up of its slot.  What bounds it is instruction issue (a quotient and a rounding for every element): 49152 tokens of
-// 8 heads of 128 stored and read back, two launches, 118 us, 4.5 TB/s (with an exchange for each end and one quotient at a
-// time 143); 24 tokens 8.7.
+// 8 heads of 128 stored and read back, two launches, 113 to 115 us, 4.7 TB/s, 61 of them storing (with an exchange for each end and one
+// quotient at a time 143); 24 tokens 8.6.
 struct Kv4StoreParams {
   unsigned char *k_pool, *v_pool;
   const void *k, *v;          // (n, hkv, head_dim), dense heads
@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(Kv4StoreParams p) {
 }
 
 // ---------------------------------------------------------------- rows out of the pool
-// A word and its pair a lane, eight elements in order, rounded once from fp32.  Bound by memory.
+// A word and its pair a lane, of two rows at once, eight elements in order, rounded once from fp32.  Bound by memory: 52272 tokens of 8
+// heads of 128 53 us, 5.2 TB/s (a row at a time 57).
 struct Kv4LoadParams {
   const unsigned char *k_pool, *v_pool;
   void *k, *v;                // (n, hkv, head_dim), contiguous
@@ -275,31 +276,42 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
   const int32_t* slots = after_wait(p.slots);
   const unsigned char* pools[2] = {after_wait(p.k_pool), after_wait(p.v_pool)};
   constexpr uint32_t PER = 256 / CH;
+  constexpr int RU = 2;                             // rows in flight
   const uint32_t rows = static_cast<uint32_t>(p.n) * p.hkv;
-  const int c = threadIdx.x % CH;
-  for (uint32_t row = blockIdx.x * PER + threadIdx.x / CH; row < rows; row += gridDim.x * PER) {
-    const uint32_t t = token_of(row, p.hkv, p.hkv_recip), h = row - t * p.hkv;
-    const int slot = slots[t];
-    const bool ok = slot >= 0 && slot < p.num_slots;
-    if (!ok && p.status) atomicOr(p.status, 2);
-    const int64_t block = (static_cast<int64_t>(ok ? slot / kKv4Rows : 0) * p.hkv + h) * kv4_block_bytes(HD);
-    const int r = slot % kKv4Rows, g = c / 8;
+  const int c = threadIdx.x % CH, g = c / 8;
+  for (uint32_t row0 = blockIdx.x * PER + threadIdx.x / CH; row0 < rows; row0 += gridDim.x * PER * RU) {
+    uint32_t word[RU][2], pair[RU][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t word = 0, pair = 0;
-      if (ok) {
-        word = *reinterpret_cast<const uint32_t*>(pools[j] + block + r * (HD / 2) + ((c % 8) * G + g) * 4);
-        pair = *reinterpret_cast<const uint32_t*>(pools[j] + block + kv4_pairs_at(HD) + (r * G + g) * 4);
-      }
-      const float2 sb = unpack_pair(T{}, pair);
-      uint4 o;
+    for (int u = 0; u < RU; ++u) {
+      const uint32_t row = row0 + u * gridDim.x * PER;
+      const uint32_t t = token_of(row, p.hkv, p.hkv_recip), h = row - t * p.hkv;
+      const int slot = row < rows ? __ldg(slots + t) : 0;
+      const bool ok = row < rows && slot >= 0 && slot < p.num_slots;
+      if (!ok && row < rows && p.status) atomicOr(p.status, 2);
+      const int64_t block = (static_cast<int64_t>(slot / kKv4Rows) * p.hkv + h) * kv4_block_bytes(HD);
+      const int r = slot % kKv4Rows;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t n = word >> (4 * e);
-        reinterpret_cast<uint32_t*>(&o)[e] = MmaOp<T>::pack(fmaf(static_cast<float>(n & 15u), sb.x, sb.y),
-                                                            fmaf(static_cast<float>(n >> 16 & 15u), sb.x, sb.y));
+      for (int j = 0; j < 2; ++j) {
+        word[u][j] = ok ? __ldg(reinterpret_cast<const uint32_t*>(pools[j] + block + r * (HD / 2) + ((c % 8) * G + g) * 4)) : 0u;
+        pair[u][j] = ok ? __ldg(reinterpret_cast<const uint32_t*>(pools[j] + block + kv4_pairs_at(HD) + (r * G + g) * 4)) : 0u;
       }
-      reinterpret_cast<uint4*>(j == 0 ? p.k : p.v)[static_cast<int64_t>(row) * CH + c] = o;
+    }
+#pragma unroll
+    for (int u = 0; u < RU; ++u) {
+      const uint32_t row = row0 + u * gridDim.x * PER;
+      if (row >= rows) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 sb = unpack_pair(T{}, pair[u][j]);
+        uint4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t n = word[u][j] >> (4 * e);
+          reinterpret_cast<uint32_t*>(&o)[e] = MmaOp<T>::pack(fmaf(static_cast<float>(n & 15u), sb.x, sb.y),
+                                                              fmaf(static_cast<float>(n >> 16 & 15u), sb.x, sb.y));
+        }
+        reinterpret_cast<uint4*>(j == 0 ? p.k : p.v)[static_cast<int64_t>(row) * CH + c] = o;
+      }
     }
   }
 }
