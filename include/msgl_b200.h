@@ -541,6 +541,9 @@ int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const voi
 
 /*
  * msgl_paged_prefill_attention_p16 over this pool: masks, arguments and zeros of rows without a key as there.
+ * With more than 16 rows (new tokens times query heads) a KV head, the elements of K and V are rounded to f16, each over a power of two
+ * that follows the largest of a head's keys, or values, that are read together: eleven bits down to 2^-27 of that largest, below that 2^-38 of it.
+ * The softmax weights are rounded to f16: eleven bits down to 2^-21 of a row's largest, below that 2^-32 of it.
  * max_len_extend is the longest query block, or more (rows of a longer one may stay unwritten, and 2 is reported).
  * Long prefills expand their pages into f16 first, into `expanded`, memory of the call's own of
  * msgl_prefill_expanded_bytes_q4 bytes (0 where a call does not), which can go elsewhere once its launches are queued

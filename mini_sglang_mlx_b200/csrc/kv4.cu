@@ -161,11 +161,12 @@ bool q4_expands(int batch, int total_q, int64_t total_kv, int hq, int hkv, int h
   return attend_us > (head_dim == 256 ? kQ4ExpandWorth256 : kQ4ExpandWorth128) * copy_us;
 }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-// K rows, V rows, page ids, q rows and their powers.
-size_t q4_expanded_bytes(int total_q, int64_t total_kv, int64_t total_pages, int hq, int hkv, int head_dim, int dtype) {
+// K rows, V rows, sequences' powers, page ids, q rows and their powers.
+size_t q4_tops_bytes(int batch, int hkv) { return static_cast<size_t>(batch) * hkv * 2 * msgl::kRangeParts * sizeof(uint32_t); }
+size_t q4_expanded_bytes(int batch, int total_q, int64_t total_kv, int64_t total_pages, int hq, int hkv, int head_dim, int dtype) {
   const size_t rows = rounded(static_cast<size_t>(total_kv) * hkv * head_dim * 2);
   const size_t q_rows = static_cast<size_t>(total_q) * hq;
-  return 2 * rows + rounded(total_pages * sizeof(int32_t)) +
+  return 2 * rows + q4_tops_bytes(batch, hkv) + rounded(total_pages * sizeof(int32_t)) +
          (dtype == MSGL_DTYPE_BF16 ? rounded(q_rows * head_dim * 2) + rounded(q_rows * sizeof(float)) : 0);
 }
 
@@ -392,7 +393,7 @@ size_t msgl_prefill_expanded_bytes_q4(int batch, int total_q, int64_t total_page
   const int64_t total_kv = total_pages * page_size;
   return q4_expands(batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, max_len_extend, is_cross_attention != 0,
                     sliding_window_size, sms > 0 ? sms : 148)
-             ? q4_expanded_bytes(total_q, total_kv, total_pages, num_q_heads, num_kv_heads, head_dim, dtype)
+             ? q4_expanded_bytes(batch, total_q, total_kv, total_pages, num_q_heads, num_kv_heads, head_dim, dtype)
              : 0;
 }
 
@@ -496,7 +497,7 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
   if (expanded != nullptr && batch <= 65535 &&
       q4_expands(batch, total_q, total_kv, num_q_heads, num_kv_heads, head_dim, max_len_extend, is_cross_attention != 0,
                  sliding_window_size, sms) &&
-      expanded_bytes >= q4_expanded_bytes(total_q, total_kv, total_pages, num_q_heads, num_kv_heads, head_dim, dtype)) {
+      expanded_bytes >= q4_expanded_bytes(batch, total_q, total_kv, total_pages, num_q_heads, num_kv_heads, head_dim, dtype)) {
     const int64_t pairs =
         msgl::prefill_item_bound(batch, total_q, total_kv, p.group, 256, max_len_extend, 0) * num_kv_heads;
     if (pairs * 2 > 0x7fffffffLL) return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
@@ -508,8 +509,16 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     x.page_indices = page_indices;
     x.k_rows = reinterpret_cast<__half*>(at);
     x.v_rows = reinterpret_cast<__half*>(at + rows);
-    x.pages = reinterpret_cast<int32_t*>(at + 2 * rows);
-    at += 2 * rows + rounded(total_pages * sizeof(int32_t));
+    at += 2 * rows;
+    x.tops = reinterpret_cast<uint32_t*>(at);
+    at += q4_tops_bytes(batch, num_kv_heads);
+    x.pages = reinterpret_cast<int32_t*>(at);
+    at += rounded(total_pages * sizeof(int32_t));
+    x.page_indptr = page_indptr;
+    x.kv_lens = kv_lens;
+    x.prefix_lens = prefix_lens;
+    x.batch = batch;
+    x.window = sliding_window_size;
     x.total_pages = static_cast<int>(total_pages);
     x.page_blocks = page_size / msgl::kKv4Rows;
     x.hkv = num_kv_heads;
@@ -534,14 +543,19 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
       return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot build the tensor map of the queries");
     p.q = q16;
     p.q_power = x.q_power;
+    p.kv_tops = x.tops;
     p.k_cache = x.k_rows;
     p.v_cache = x.v_rows;
     p.page_indices = x.pages;
     p.num_slots = total_kv;
     p.kv_chunk = 0;
     p.chunk_recip = 0;
-    auto run = [&](auto expand, auto kernel, int threads, int smem) -> cudaError_t {
-      cudaError_t err = launch_dependent(expand, dim3(static_cast<unsigned>(sms * 8)), dim3(256), 0, s, x);
+    if (static_cast<int64_t>(batch) * num_kv_heads * msgl::kRangeParts > 0x7fffffffLL)
+      return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
+    auto run = [&](auto range, auto expand, auto kernel, int threads, int smem) -> cudaError_t {
+      cudaError_t err = launch_dependent(range, dim3(static_cast<unsigned>(batch * num_kv_heads * msgl::kRangeParts)), dim3(256), 0, s, x);
+      if (err != cudaSuccess) return err;
+      err = launch_dependent(expand, dim3(static_cast<unsigned>(sms * 8)), dim3(256), 0, s, x);
       if (err != cudaSuccess) return err;
       if ((err = allow_smem(kernel, smem)) != cudaSuccess) return err;
       return launch_clusters(2, kernel, dim3(static_cast<unsigned>(pairs * 2)), dim3(threads), smem, s, p, tm_k, tm_v, tg_k, tg_v,
@@ -551,9 +565,11 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
       using T = decltype(tag);
       using P128 = msgl::PairShape<128, true>;
       using P256 = msgl::PairShape<256, true>;
-      return head_dim == 128 ? run(msgl::kv4_expand_kernel<T, 128>, msgl::prefill_pair_kernel<T, 128, true, __half>,
+      return head_dim == 128 ? run(msgl::kv4_range_kernel<T, 128>, msgl::kv4_expand_kernel<T, 128>,
+                                   msgl::prefill_pair_kernel<T, 128, true, __half, true>,
                                    P128::kThreads, P128::kSmemBytes)
-                             : run(msgl::kv4_expand_kernel<T, 256>, msgl::prefill_pair_kernel<T, 256, true, __half>,
+                             : run(msgl::kv4_range_kernel<T, 256>, msgl::kv4_expand_kernel<T, 256>,
+                                   msgl::prefill_pair_kernel<T, 256, true, __half, true>,
                                    P256::kThreads, P256::kSmemBytes);
     };
     const cudaError_t e = convert ? of(__nv_bfloat16{}) : of(__half{});

@@ -85,8 +85,8 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// The eight elements of a word under an f16 pair, in order: scale * code + bias in f16, rounded once (half a unit, 2^-12 of the
-// element where T is bf16, whose own unit is sixteen times that).
+// The eight elements of a word under an f16 pair, in order: scale * code + bias in f16, rounded once (half a unit: 2^-11 of an
+// element from 2^-14 on, which is what block_power is for).
 __device__ __forceinline__ uint4 kv4_values(uint32_t word, uint32_t pair) {
   const uint32_t scale = __byte_perm(pair, pair, 0x1010), bias = __byte_perm(pair, pair, 0x3232);
   uint32_t v[4];
@@ -106,14 +106,64 @@ __device__ __forceinline__ float row_power(__half, uint32_t top) {
 __device__ __forceinline__ float row_power(__nv_bfloat16, uint32_t top) {
   return __uint_as_float((max(top >> 7, 12u) - 10u) << 23);
 }
-// 1 / power, exactly (its exponent field is 2 to 245).
+// 1 / power, exactly (its exponent field is 1 to 253).
 __device__ __forceinline__ float power_inverse(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 
-// A pair of type T in f16: exact from 2^-14 on (what the pool holds is below 2^15), below that to 2^-25.
-__device__ __forceinline__ uint32_t f16_pair(__half, uint32_t pair) { return pair; }
-__device__ __forceinline__ uint32_t f16_pair(__nv_bfloat16, uint32_t pair) {
-  const float2 x = unpack_pair(__nv_bfloat16{}, pair);
-  return MmaOp<__half>::pack(x.x, x.y);
+// Powers of two for keys and values.  Elements go to the products as f16 numbers, and the pool's (scales from 2^-100, numbers to 2^15) are
+// more than f16 has.  So the keys of a head that go into one sum are divided by a power of two, and so are the values; one comes
+// back in the scores' scale, the other with the output.  Let t be the largest of their biases' magnitudes and 16 scales: elements are below
+// 2 t, and the power brings t to [2^13, 2^14).  An element keeps f16's eleven bits down to 2^-27 of the largest one, and below that is
+// held to 2^-38 of it.  At least 2^-95, so that sums over it stay finite; 1 where there is nothing.
+// (Largest scales in the low halves and biases' magnitudes in the high ones: such bits are ordered as the numbers are.)
+__device__ __forceinline__ uint32_t pair_tops(uint32_t tops, uint32_t pair) { return __vmaxu2(tops, pair & 0x7fff7fffu); }
+// t, as the bits of a float.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(uint32_t tops) {
+  const float2 x = unpack_pair(T{}, tops);
+  return __float_as_uint(fmaxf(16.f * x.x, x.y));
+}
+__device__ __forceinline__ float range_power(uint32_t top) {
+  return top == 0u ? 1.f : __uint_as_float((min(max(top >> 23, 45u), 254u) - 13u) << 23);
+}
+// The largest t of K and of V over keys [t_lo, t_hi) of a sequence, of what this warp's threads look at (`thread` of THREADS that share the
+// range): the pairs of a block of a head are 8 G words of 16 bytes in K and V together, one a thread.  block_of: a key's block in the pool.
+template <typename T, int HD, int THREADS, typename BlockOf>
+__device__ __forceinline__ uint2 pair_range(const unsigned char* k_pool, const unsigned char* v_pool, int hkv, int h, int t_lo, int t_hi,
+                                            int64_t num_blocks, int thread, BlockOf block_of) {
+  constexpr int G = HD / kKv4Group, UNITS = 8 * G, FLY = 4;
+  constexpr int STEP = THREADS / UNITS * kKv4Rows;
+  const int part = thread % (UNITS / 2);             // of 4 / G rows
+  const bool is_v = thread % UNITS >= UNITS / 2;
+  const unsigned char* const from = (is_v ? v_pool : k_pool) + static_cast<int64_t>(h) * kv4_block_bytes(HD) + kv4_pairs_at(HD) + part * 16;
+  const int t_end = t_hi - part * 4 / G;             // its first row is a key below this
+  uint32_t tops = 0u;
+#pragma unroll 1
+  for (int t0 = t_lo + thread / UNITS * kKv4Rows; t0 < t_hi; t0 += FLY * STEP) {
+    int64_t block[FLY];
+    uint4 x[FLY];
+#pragma unroll
+    for (int f = 0; f < FLY; ++f) block[f] = t0 + f * STEP < t_end ? block_of(t0 + f * STEP) : -1;
+#pragma unroll
+    for (int f = 0; f < FLY; ++f)
+      x[f] = block[f] >= 0 && block[f] < num_blocks ? __ldg(reinterpret_cast<const uint4*>(from + block[f] * hkv * kv4_block_bytes(HD)))
+                                                     : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int f = 0; f < FLY; ++f) {
+      if (G == 2 && t0 + f * STEP + 1 >= t_end) x[f].z = x[f].w = 0u;      // (its second row)
+      tops = pair_tops(pair_tops(pair_tops(pair_tops(tops, x[f].x), x[f].y), x[f].z), x[f].w);
+    }
+  }
+  const uint32_t top = largest<T>(tops);
+  return make_uint2(__reduce_max_sync(0xffffffffu, is_v ? 0u : top), __reduce_max_sync(0xffffffffu, is_v ? top : 0u));
+}
+// The largest weight of a row is put 2^7 above 1 (f16 ends at 2^16, and it may grow by 2^8 before it is put there again): a weight then has
+// all its bits down to 2^-21 of the largest, where the value under it may be that much larger than the others.
+constexpr float kWeightRoom = 7.f;
+// A pair in f16, times a power of two.
+template <typename T>
+__device__ __forceinline__ uint32_t f16_pair(T, uint32_t pair, float by) {
+  const float2 x = unpack_pair(T{}, pair);
+  return MmaOp<__half>::pack(x.x * by, x.y * by);
 }
 
 // Codes of the 2 W elements that a lane holds of a group of 64, LANES = 32 / W lanes of `mask` together, and the group's pair
@@ -319,7 +369,8 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
 // ---------------------------------------------------------------- pages laid out for the pairs of CTAs
 // A long prefill reads a key once for every 256 query rows, and to expand its codes each time is what bounds the kernel that does
 // (one CTA; 4096 tokens over 16384 1425 us).  Expanded once into f16 pages, one per entry of the index list and
-// in its order, they come by TMA and pairs of CTAs share them.  q goes with them, as f16 over a power of two per row (bf16 only).
+// in its order, they come by TMA and pairs of CTAs share them.  A sequence's keys and values of a head are divided by powers of two
+// (range_power), which a kernel in front finds.  q goes with them, as f16 over a power of two per row (bf16 only).
 // Bound by memory: 2.6 bytes an element of the pool, 4 of q; 20480 tokens of 8 heads of 128 and 4096 queries of 32 heads 34 us, 5.2
 // TB/s, in front of an attention of 1010 (with 116 registers and two CTAs per SM 44).
 struct Kv4ExpandParams {
@@ -327,6 +378,9 @@ struct Kv4ExpandParams {
   const int32_t* page_indices;
   __half *k_rows, *v_rows;      // (total_pages * page_size, hkv, head_dim)
   int32_t* pages;               // (total_pages): 0, 1, ...
+  uint32_t* tops;               // (batch, hkv, 2, kRangeParts): the largest t of K and of V in parts of a sequence
+  const int32_t *page_indptr, *kv_lens, *prefix_lens;
+  int batch, window;
   const void* q;                // (q_rows, head_dim), or null
   __half* q_rows;
   float* q_power;
@@ -335,12 +389,69 @@ struct Kv4ExpandParams {
   int* status;
 };
 
+constexpr int kRangeParts = 32;
+// What a sequence's keys (is_v: values) of a head are divided by, for a warp.
+__device__ __forceinline__ float sequence_power(const uint32_t* tops, int b, int hkv, int h, int is_v, int lane) {
+  return range_power(__reduce_max_sync(0xffffffffu, __ldg(tops + ((static_cast<int64_t>(b) * hkv + h) * 2 + is_v) * kRangeParts + lane)));
+}
+
+// A CTA for each part of each sequence and head: the keys from the first that a row's window can reach (and the tile of 128 that it is
+// in) to the last.  A ninth of the pool is read.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv4_range_kernel(const Kv4ExpandParams p) {
+  __shared__ uint2 s_top[8];
+  grid_dependency_wait();
+  grid_dependency_launch();
+  const int32_t* const ids = after_wait(p.page_indices);
+  const int32_t* const indptr = after_wait(p.page_indptr);
+  const int32_t* const lens = after_wait(p.kv_lens);
+  const int32_t* const prefixes = after_wait(p.prefix_lens);
+  const int part = blockIdx.x % kRangeParts, h = blockIdx.x / kRangeParts % p.hkv, b = blockIdx.x / kRangeParts / p.hkv;
+  const int page_size = p.page_blocks * kKv4Rows;
+  const int begin = __ldg(indptr + b);
+  const int64_t cap = static_cast<int64_t>(max(__ldg(indptr + b + 1) - begin, 0)) * page_size;
+  const int len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(lens + b), 0)), cap));
+  const int lo = p.window > 0 ? max(0, __ldg(prefixes + b) - p.window + 1) / 128 * 128 : 0;
+  const int per = (max(len - lo, 0) / kKv4Rows / kRangeParts + 1) * kKv4Rows;        // keys of a part
+  const int64_t from = lo + static_cast<int64_t>(part) * per;
+  uint2 top = make_uint2(0u, 0u);
+  if (from < len)
+    top = pair_range<T, HD, 256>(after_wait(p.k_pool), after_wait(p.v_pool), p.hkv, h, static_cast<int>(from),
+                                 static_cast<int>(min(from + per, static_cast<int64_t>(len))), p.num_blocks, threadIdx.x, [&](int t) -> int64_t {
+                                   const int page = t / page_size;
+                                   return static_cast<int64_t>(__ldg(ids + begin + page)) * p.page_blocks + (t - page * page_size) / kKv4Rows;
+                                 });
+  if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    uint32_t most = 0u;
+    for (int w = 0; w < 8; ++w) most = max(most, threadIdx.x == 0 ? s_top[w].x : s_top[w].y);
+    p.tops[((static_cast<int64_t>(b) * p.hkv + h) * 2 + threadIdx.x) * kRangeParts + part] = most;
+  }
+}
+
+// The sequence that `page` (an entry of the index list) belongs to: a search by the warp in the row pointers, for the last that is
+// at most `page`.
+__device__ __forceinline__ int sequence_of_page(const int32_t* indptr, int batch, int page, int lane) {
+  int first = 0, n = batch;
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lane * step;
+    const uint32_t in = __ballot_sync(0xffffffffu, at < n && __ldg(indptr + first + min(at, n - 1)) <= page);
+    const int k = in == 0u ? 0 : 31 - __clz(in);
+    first += k * step;
+    n = min(step, n - k * step);
+  }
+  return first;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const Kv4ExpandParams p) {
   constexpr int CH = HD / 8, G = HD / kKv4Group, RPP = 32 / CH;      // chunks of a row; rows a pass of a warp
   grid_dependency_wait();
   grid_dependency_launch();
   const int32_t* ids = after_wait(p.page_indices);
+  const int32_t* const indptr = after_wait(p.page_indptr);
+  const uint32_t* const tops = after_wait(p.tops);
   const unsigned char* pools[2] = {after_wait(p.k_pool), after_wait(p.v_pool)};
   const T* q = after_wait(static_cast<const T*>(p.q));
   const int lane = threadIdx.x & 31;
@@ -358,9 +469,13 @@ __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const Kv4ExpandParam
     const bool ok = block >= 0 && block < p.num_blocks;
     if (!ok && p.status && lane == 0) atomicOr(p.status, 2);
     const int64_t at = ((ok ? block : 0) * p.hkv + h) * kv4_block_bytes(HD);
-#pragma unroll
+    const int seq = sequence_of_page(indptr, p.batch, page, lane);
+    const float inverse[2] = {power_inverse(sequence_power(tops, seq, p.hkv, h, 0, lane)),
+                              power_inverse(sequence_power(tops, seq, p.hkv, h, 1, lane))};
+#pragma unroll (HD == 128 ? 2 : 1)
     for (int j = 0; j < 2; ++j) {
-      const unsigned char* src = pools[j] + at;
+      const unsigned char* src = (j == 0 ? pools[0] : pools[1]) + at;
+      const float by = j == 0 ? inverse[0] : inverse[1];
       uint32_t word[kKv4Rows / RPP], pair[kKv4Rows / RPP];
 #pragma unroll
       for (int k = 0; k < kKv4Rows / RPP; ++k) {
@@ -372,7 +487,7 @@ __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const Kv4ExpandParam
 #pragma unroll
       for (int k = 0; k < kKv4Rows / RPP; ++k)
         *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(k * RPP + rsub) * p.hkv * HD) =
-            kv4_values(word[k], f16_pair(T{}, pair[k]));
+            kv4_values(word[k], f16_pair(T{}, pair[k], by));
     }
   }
   if (q == nullptr) return;

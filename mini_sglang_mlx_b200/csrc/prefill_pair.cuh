@@ -189,8 +189,9 @@ struct PairBarriers {
 };
 
 // M: type of the operands.  Where it is not T, q has been converted (p.q_power: what each row was divided by), and the pool's
-// rows are of type M.
-template <typename T, int HD, bool PAGED, typename M = T>
+// rows are of type M.  EXPANDED: the pages are kv4_expand_kernel's, a sequence's keys and values of a head divided by a power of two
+// each (p.kv_tops), which come back in the scores' scale and with the output.
+template <typename T, int HD, bool PAGED, typename M = T, bool EXPANDED = false>
 __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
     prefill_pair_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tg_k,
@@ -663,6 +664,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
     const int vhi = p.is_cross ? sq.L - 1 : min(pos, sq.L - 1);
     const int vlo = p.window > 0 ? pos - p.window + 1 : 0;
     float m_ref = -INFINITY, l = 0.f;
+    constexpr float kRoom = EXPANDED ? kWeightRoom : 0.f;
     bool alive = true;
     const bool sc_neg = !(p.scale_log2 > 0.f);
     float row_scale = p.scale_log2;
@@ -670,6 +672,13 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
       const int pk = pk0 + rank * ROWS + r;
       if (r < rows_valid)
         row_scale *= p.q_power[static_cast<int64_t>(sq.q_begin + tl) * p.hq + static_cast<int64_t>(h) * G + (pk - tl * G)];
+    }
+    float v_power = 1.f;
+    if constexpr (EXPANDED) {
+      row_scale *= sequence_power(p.kv_tops, it.b, p.hkv, h, 0, lane);
+      // (above zero also where the powers leave nothing: a masked score is -inf)
+      if (!sc_neg) row_scale = fmaxf(row_scale, 1.17549435e-38f);
+      v_power = sequence_power(p.kv_tops, it.b, p.hkv, h, 1, lane);
     }
     const float sc = sc_neg ? 1.f : row_scale;
 
@@ -757,7 +766,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
           m_old = __uint_as_float(got.x);
         }
       }
-      const float m_new = mt > m_old + 8.f ? mt : m_old;
+      const float m_new = mt > m_old + (8.f + kRoom) ? mt - kRoom : m_old;
       if constexpr (NG == 2) {
         st_shared_tagged(smem_u32(&s_mref[(j & 1) * ROWS + r]), __float_as_uint(m_new), j);
       }
@@ -831,6 +840,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
                       (peer.x == -INFINITY ? 0.f : peer.y * fast_exp2(peer.x - M));
       inv = L > 0.f ? 1.f / L : 0.f;
     }
+    inv *= v_power;
 #pragma unroll 1
     for (int c = grp * (HD / 32 / NG); c < (grp + 1) * (HD / 32 / NG); ++c) {   // a group's share of the columns
       uint32_t v[32];

@@ -97,8 +97,10 @@ struct TcShape {
 };
 
 // The same over a pool held in 4 bits (kv4.cuh).  The first copying warp fetches blocks (16 tokens of the head, one bulk copy)
-// into a ring of their own; the others, a block each in turn, write its elements into the tiles, scale * code + bias
-// rounded once (K to T, V to f16, see below); the tiles' ring is shorter for it.
+// into a ring of their own; the others, a block each in turn, write its elements into the tiles, scale * code + bias over the item's power of
+// two (range_power) rounded once to f16; the tiles' ring is shorter for it.  They find the powers first, from the pairs of the item's keys,
+// a ninth of what it reads, while the first blocks are on their way.  (Measured otherwise, five verify tokens 56.2 us without any powers,
+// 59 with these, 66 with a power for each block of sixteen keys, which the softmax warps then have to apply.)
 template <int NSUB, int HD>
 struct Kv4Shape {
   // (three buffers and twice the blocks: 512 tokens of four over 4096 115 us for 104, short blocks the same)
@@ -476,8 +478,9 @@ __device__ __noinline__ void merge_kv_splits_cta(const MergeArgs p, int nsp, int
 
 // KV4: the pool is held in 4 bits and addressed by pages (Kv4Shape).  Every operand is f16 there whatever T is: three bits of
 // fraction more than bf16 where elements of K and V and the weights are rounded (in bf16, results are 0.0035 off 64 bits as a
-// norm; the rounding of the output alone is 0.0017; with f16 outputs 0.00035, of which 0.00021).  What the pool holds lies within +-2^15, so f16 takes it (below 2^-14 to
-// 2^-25); a row of q is divided by a power of two, which comes back in the row's scale.  Five verify tokens of 16 requests over
+// norm; the rounding of the output alone is 0.0017; with f16 outputs 0.00035, of which 0.00021).  The range that f16 lacks is in powers of two: a
+// row of q and the item's keys are divided by one, which comes back in the row's scale, and its values by another, which comes
+// back with the output.  Five verify tokens of 16 requests over
 // 1024 to 16384 56 us, 16 draft tokens of 16 under a window of 4096 72, four chunks of 300 to 512 over up to 4096 99 (over 16-bit pages
 // 53, 62, 82).  No part bounds it alone: 64 keys take an SM with two CTAs 1100 cycles, in which a quarter of the instructions expand
 // codes and a seventh are the softmax, the rest copies, waits and bookkeeping of twelve warps; each waits for the others in turn.  Without
@@ -517,6 +520,9 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   __shared__ int s_raw_bad[kRaw];                             // their page is not in the pool
   __shared__ uint64_t s_q_raw;                                // IN_PLACE: Q as it is has arrived
   __shared__ float s_row_power[CONVERT ? BM : 1];             // what a row of q was divided by
+  constexpr int kWriters = Shape::kWarps - kTcProducerWarp0 - 1;     // KV4: warps that write tiles
+  __shared__ uint32_t s_tops[2][KV4 ? kWriters : 1];          // largest of K's and V's pairs that each of them found
+  __shared__ uint64_t s_tops_full;
   __shared__ int s_slots[KV4 ? 1 : (LA + 1) * BN];  // slot ids of the key tiles being copied / next to copy
 
   const int tid = threadIdx.x;
@@ -555,6 +561,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     if constexpr (KV4) {
       init(s_raw_full, kRaw, 1);
       init(s_raw_empty, kRaw, 1);
+      init(&s_tops_full, 1, kWriters);
     }
     init(bars.empty, kTcBufs, 1);
     init(bars.stage, NSUB, SUB / 32);                  // one arrival per warp of the group
@@ -641,6 +648,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
 
   const uint32_t tmem = s_tmem_base;
   volatile int* abort_flag = &s_abort;
+  // KV4: what the item's K (0) or V (1) is divided by, once s_tops_full is complete (and the item has tiles)
+  auto item_power = [&](int j) -> float { return range_power(__reduce_max_sync(0xffffffffu, lane < kWriters ? s_tops[KV4 ? j : 0][lane] : 0u)); };
 #ifdef MSGL_TRACE
   if (tid == 0) {
     MSGL_TR(3, clock64());          // set-up done
@@ -835,7 +844,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     } else if constexpr (KV4) {
       constexpr int PPT = BN / kKv4Rows;               // blocks of a tile
       constexpr int BLK = kv4_block_bytes(HD), G = HD / kKv4Group;
-      constexpr int DW = Shape::kWarps - kTcProducerWarp0 - 1;     // warps that write tiles
+      constexpr int DW = kWriters;
       const uint32_t raw = ring + kTcBufs * kTcKvTileBytes;
       unsigned char* const raw_at = smem_raw + (raw - smem_u32(smem_raw));
       load_q();
@@ -907,6 +916,21 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
         constexpr int PPR = HD / 32, RPP = 32 / PPR;   // rows a pass
         const int dw = warp - kTcProducerWarp0 - 1;
         const int piece = lane % PPR, rsub = lane / PPR;
+        if (ntiles > 0) {
+          const int page_blocks = p.page_size / kKv4Rows;
+          const uint2 tops = pair_range<T, HD, DW * 32>(
+              after_wait(kbase), after_wait(vbase), p.hkv, h, kv_lo, kv_hi_load, p.num_slots / kKv4Rows, dw * 32 + lane, [&](int t) -> int64_t {
+                const int page = divide_by(t, p.page_recip);
+                return static_cast<int64_t>(__ldg(p.page_indices + sq.kv_begin + page)) * page_blocks + (t - page * p.page_size) / kKv4Rows;
+              });
+          if (lane == 0) {
+            s_tops[0][dw] = tops.x;
+            s_tops[1][dw] = tops.y;
+            mbar_arrive(smem_u32(&s_tops_full));
+          }
+          alive = mbar_wait_warp(smem_u32(&s_tops_full), 0, abort_flag);
+        }
+        const float k_inverse = power_inverse(item_power(0)), v_inverse = power_inverse(item_power(1));
         each_tile([&](int seq, bool is_v, int tile, int at) {
           const int bf = seq % kTcBufs;
           int blk = (dw - at % DW + DW) % DW;
@@ -942,10 +966,12 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
 #pragma unroll
             for (int i = 0; i < kKv4Rows / RPP; ++i) {
 #pragma unroll
+              for (int g = 0; g < G; ++g) pairs[i][g] = f16_pair(T{}, pairs[i][g], is_v ? v_inverse : k_inverse);
+#pragma unroll
               for (int w = 0; w < 4; ++w) {
                 const int g = w % G, r8 = piece * (4 / G) + w / G;
                 *reinterpret_cast<uint4*>(dst + tc_tile_offset<BN>(blk * kKv4Rows + i * RPP + rsub, g * 8 + r8)) =
-                    kv4_values(words[i][w], f16_pair(T{}, pairs[i][g]));
+                    kv4_values(words[i][w], pairs[i][g]);
               }
             }
             fence_proxy_async_smem();
@@ -1137,6 +1163,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     const int vlo = max(p.window > 0 ? pos - p.window + 1 : 0, s_lo);
     const int my_tiles = ntiles_sub[i];
     float m_ref = -INFINITY, l = 0.f;
+    constexpr float kRoom = KV4 ? kWeightRoom : 0.f;
     bool alive = true;
     const bool sc_neg = !(p.scale_log2 > 0.f);
     float row_scale = p.scale_log2;
@@ -1196,6 +1223,16 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       row_scale *= s_row_power[row];
       if (lane == 0) mbar_arrive(bar_q);
     }
+    float v_power = 1.f;
+    if constexpr (KV4) {
+      if (my_tiles > 0) {
+        alive = mbar_wait_warp(smem_u32(&s_tops_full), 0, abort_flag) && alive;
+        v_power = item_power(1);
+        row_scale *= item_power(0);
+        // (above zero also where the powers leave nothing: a masked score is -inf)
+        if (!sc_neg) row_scale = fmaxf(row_scale, 1.17549435e-38f);
+      }
+    }
     const float sc = sc_neg ? 1.f : row_scale;
 
 #pragma unroll 1
@@ -1248,12 +1285,13 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       // ---- lazy rescale of the accumulator
       float alpha = 1.f;
       bool resc = false;
-      if (mt > m_ref + 8.f) {
+      if (mt > m_ref + (8.f + kRoom)) {
+        const float m_new = mt - kRoom;
         if (m_ref != -INFINITY) {
-          alpha = fast_exp2(m_ref - mt);
+          alpha = fast_exp2(m_ref - m_new);
           resc = true;
         }
-        m_ref = mt;
+        m_ref = m_new;
       }
       if (j > 0 && __any_sync(0xffffffffu, resc)) {
         alive = mbar_wait_warp(bar_pv(i, (j - 1) % LA), ((j - 1) / LA) & 1, abort_flag);
@@ -1319,7 +1357,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       if (alive) tc_fence_after();
     }
     if (alive) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l > 0.f ? 1.f / l * v_power : 0.f;
       if (p.kv_chunk == 0 || sq.nsplit == 1) {
         // Each warp stages its 32 output rows (HD*2 bytes each) in the Q sub-tile's shared memory,
         // free once the last S MMA has completed, then writes them out as whole rows (two per
@@ -1416,6 +1454,10 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
               } else {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = 0u;
+              }
+              if constexpr (KV4) {       // (a split has powers of its own)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * v_power);
               }
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {

@@ -53,6 +53,7 @@ struct PrefillParams {
   int kv_chunk;  // tokens per kv split; 0 = never split
   uint64_t group_recip, page_recip, chunk_recip;   // of group, page_size and kv_chunk: see divide_by
   const float* q_power;  // (total_q, hq): what the rows of a converted q were divided by (else unused)
+  const uint32_t* kv_tops;   // of expanded pages: see sequence_power (else unused)
   int early;     // the kernel in front is this call's own K/V store: the index arrays are complete
 };
 
