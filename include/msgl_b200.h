@@ -530,8 +530,10 @@ size_t msgl_decode_workspace_bytes_q4(int batch, int num_q_heads, int num_kv_hea
 
 /*
  * msgl_paged_decode_attention_p16 over this pool: arguments, clamps, gate and zeros of empty sequences as there.
- * Codes go to the tensor cores as they are, scales and biases are applied in fp32; the softmax weight times the
- * value's scale is rounded to the data type.
+ * Codes go to the tensor cores as they are, scales and biases are applied in fp32.  The softmax weight times the value's
+ * scale is rounded to f16, whatever the data type: eleven bits down to 2^-13 of the largest such product of a query head and a group of
+ * 64 elements, below that 2^-24 of it.  q is rounded to f16 over a power of two of its row: eleven bits (all of bf16's) down to 2^-24 of the
+ * row's largest, below that 2^-35 of it.
  */
 int msgl_paged_decode_attention_q4(const void* q, const void* k_cache, const void* v_cache,
                                    const int32_t* page_indptr, const int32_t* page_indices, const int32_t* kv_lens,

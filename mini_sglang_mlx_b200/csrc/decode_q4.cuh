@@ -21,15 +21,16 @@
 //                 s = sum_g scale_g (sum_d n q) + bias_g sum_d q, in fp32.  q is an f16 number times a power of two of its row
 //                 (exactly, but for what is below 2^-24 of the row's largest).
 //   O^T = V^T P^T: rows are head_dim, the 16 tokens the k dimension.  A group's scale belongs to the token, so it is multiplied
-//                 into the weight: P_g = f16(p scale_g 2^-e), 2^e a power of two over all scales so far;
-//                 sum(p bias_g) is kept in fp32.  That rounding of P_g, half a unit of f16, is the only one in front of the
-//                 output's.
+//                 into the weight: P_g = f16(p scale_g f), and sum(p bias_g) is kept in fp32.  That rounding of P_g, half a unit
+//                 of f16, is the only one in front of the output's.  f is a power of two of the column and the group that puts
+//                 the largest p scale_g so far to 1/2 .. 2^15: groups of any size, and tokens of any size whose weight is small, leave
+//                 each other their bits (eleven down to 2^-13 of the largest, below that 2^-24 of it).
 // (Columns as rows and tokens as columns, the usual way round, leaves half of each product's rows empty at eight columns; to
 // scale the codes to 16-bit values first takes twice the integer instructions, and rounds every element.  The byte n is the e4m3 number
 // n 2^-9 and would take half the masks, but a product of e4m3 with an fp32 sum is made of two of f16, conversions and additions
 // here: 171 us for 32 requests of 4096 to 32768 tokens.)
-// The weights' reference maximum moves only when a score passes it by more than 2^8, so that the rows' maxima need not
-// be reduced in every step.
+// The weights' reference maximum, a whole number, moves only when a score passes it by more than 2^8, and f when p scale_g could pass
+// 2^15 / f by the largest of both in a lane, so that maxima need not be reduced in every step.
 //
 // What bounds it: integer instructions that take the codes apart, next to the memory.  32 requests of 4096 to 32768 tokens, 8 KV heads
 // of 128, four query heads each: 108 us behind a write of the whole L2, 99 without, 4.7 and 5.1 TB/s (the same over 16-bit pages:
@@ -96,7 +97,8 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
   constexpr bool CENTRED = std::is_same<T, __half>::value;
   constexpr float kSlack = 8.f;
   constexpr float kNoScore = -1.5e38f;       // reference maximum of a column without a key (its sums are zero)
-  constexpr int kLeastExponent = -80;        // of the scales, as the reference counts it (sums stay below 2^128 then)
+  constexpr float kMostFactor = 110.f;       // log2 of f at most
+  constexpr float kNoFactor = 8.077935669463161e-28f;      // 2^-90: f of a column without a key
   using Mma = MmaOp<__half>;
 
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -392,15 +394,15 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
     const int all_lo = BLOCKS && p.window > 0 ? cs.k.prefix + cs.k.new_tok - p.window : 0;
     const int all_hi = BLOCKS && !p.is_cross ? min(t_hi, cs.k.prefix + 1) : t_hi;
     const int steps = (cs.ng + U - 1) / U, prefix = cs.k.prefix;
-    float vlim = 0.f;                             // the power of two over the scales so far (0: there was none)
-    float limit = kSlack - kLeastExponent;        // exponent over the reference that is not let pass
     float o[NT][G][4][4];        // [group][nibble]: elements 64 g + 8 r + 2 i, + 1 of columns 2 c, 2 c + 1
     float pbias[NT][G][2];       // sums of p bias_g over this lane's tokens
     float m[NT][2], l[NT][2];
+    float f[NT][G][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
+        f[nt][g][0] = f[nt][g][1] = kNoFactor;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -482,12 +484,16 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
             }
           }
         }
-        float smax = 0.f;
+        float most = 0.f;          // p scale f is below this times 2^8
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+        for (int g = 0; g < G; ++g) {
+          float smax = 0.f, fmax = 0.f;
 #pragma unroll
-          for (int g = 0; g < G; ++g)
-            smax = max3(smax, unpack_pair(T{}, vpair[u][0][g]).x, unpack_pair(T{}, vpair[u][1][g]).x);
+          for (int u = 0; u < N; ++u) smax = max3(smax, unpack_pair(T{}, vpair[u][0][g]).x, unpack_pair(T{}, vpair[u][1][g]).x);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) fmax = max3(fmax, f[nt][g][0], f[nt][g][1]);
+          most = fmaxf(most, smax * fmax);
+        }
         // ---- exponents over the reference (one that is not there yet is far below every score)
         float x[N][NT][4], over = -INFINITY;
         auto seen = [&](int u, int nt, int j) -> bool {
@@ -520,14 +526,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
             for (int j = 0; j < 4; ++j) x[u][nt][j] = s[u][nt][j] - m[nt][j & 1];
             over = max3(max3(over, x[u][nt][0], x[u][nt][1]), x[u][nt][2], x[u][nt][3]);
           }
-        if (__any_sync(0xffffffffu, over > limit || smax > vlim)) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
-          if (smax > vlim) {
-            const uint32_t e = (__float_as_uint(smax) >> 23) + 1;
-            vlim = __uint_as_float(e << 23);
-            limit = kSlack - max(static_cast<int>(e) - 127, kLeastExponent);
-          }
+        if (__any_sync(0xffffffffu, over > kSlack || most > 128.f)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -537,23 +536,36 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
               for (int u = 0; u < N; ++u) mx = max3(mx, s[u][nt][j], s[u][nt][2 + j]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              mx = fmaxf(mx + (kSlack - limit), m[nt][j]);
-              const float a = fast_exp2(m[nt][j] - mx);
+              mx = fmaxf(ceilf(mx), m[nt][j]);
+              const float up = m[nt][j] - mx, a = fast_exp2(up);
               m[nt][j] = mx;
               l[nt][j] *= a;
-#pragma unroll
-              for (int g = 0; g < G; ++g) {
-                pbias[nt][g][j] *= a;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  o[nt][g][i][j] *= a;
-                  o[nt][g][i][2 + j] *= a;
-                }
-              }
 #pragma unroll
               for (int u = 0; u < N; ++u) {
                 x[u][nt][j] = s[u][nt][j] - mx;
                 x[u][nt][2 + j] = s[u][nt][2 + j] - mx;
+              }
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                pbias[nt][g][j] *= a;
+                // the largest p scale of the step, and log2 of what the sums are in units of, as the new reference counts it
+                float top = 0.f;
+#pragma unroll
+                for (int u = 0; u < N; ++u)
+                  top = max3(top, fast_exp2(x[u][nt][j]) * unpack_pair(T{}, vpair[u][0][g]).x,
+                             fast_exp2(x[u][nt][2 + j]) * unpack_pair(T{}, vpair[u][1][g]).x);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float e = static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 126);     // top < 2^e
+                const float unit = 127.f - static_cast<float>(__float_as_uint(f[nt][g][j]) >> 23) + up;
+                const float to = fmaxf(e > unit + 7.f ? e : unit, -kMostFactor);
+                const float b = fast_exp2(unit - to);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  o[nt][g][i][j] *= b;
+                  o[nt][g][i][2 + j] *= b;
+                }
+                f[nt][g][j] = mx == kNoScore ? kNoFactor : __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(to)) << 23);
               }
             }
           }
@@ -570,14 +582,15 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               float2 p0 = unpack_pair(T{}, vpair[u][0][g]), p1 = unpack_pair(T{}, vpair[u][1][g]);
-              const uint32_t w0 = Mma::pack(x[u][nt][0] * p0.x, x[u][nt][1] * p0.x);
-              const uint32_t w1 = Mma::pack(x[u][nt][2] * p1.x, x[u][nt][3] * p1.x);
+              const uint32_t w0 = Mma::pack(x[u][nt][0] * f[nt][g][0] * p0.x, x[u][nt][1] * f[nt][g][1] * p0.x);
+              const uint32_t w1 = Mma::pack(x[u][nt][2] * f[nt][g][0] * p1.x, x[u][nt][3] * f[nt][g][1] * p1.x);
               if constexpr (CENTRED) {
                 p0.y = fmaf(7.5f, p0.x, p0.y);
                 p1.y = fmaf(7.5f, p1.x, p1.y);
                 const float2 r0 = unpack_pair(T{}, w0), r1 = unpack_pair(T{}, w1);
-                pbias[nt][g][0] = fmaf(-7.5f, r0.x, fmaf(-7.5f, r1.x, pbias[nt][g][0]));
-                pbias[nt][g][1] = fmaf(-7.5f, r0.y, fmaf(-7.5f, r1.y, pbias[nt][g][1]));
+                const float c0 = -7.5f * power_inverse(f[nt][g][0]), c1 = -7.5f * power_inverse(f[nt][g][1]);
+                pbias[nt][g][0] = fmaf(c0, r0.x, fmaf(c0, r1.x, pbias[nt][g][0]));
+                pbias[nt][g][1] = fmaf(c1, r0.y, fmaf(c1, r1.y, pbias[nt][g][1]));
               }
               pbias[nt][g][0] = fmaf(x[u][nt][0], p0.y, fmaf(x[u][nt][2], p1.y, pbias[nt][g][0]));
               pbias[nt][g][1] = fmaf(x[u][nt][1], p0.y, fmaf(x[u][nt][3], p1.y, pbias[nt][g][1]));
@@ -640,9 +653,10 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) bj += __shfl_xor_sync(0xffffffffu, bj, x);
           float x[8];
+          const float inv = power_inverse(f[nt][g][j]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float unit = i & 1 ? 1048576.f : 16777216.f;
+            const float unit = (i & 1 ? 1048576.f : 16777216.f) * inv;
             x[2 * i] = fmaf(o[nt][g][i][j], unit, bj);
             x[2 * i + 1] = fmaf(o[nt][g][i][2 + j], unit, bj);
           }

@@ -12,8 +12,12 @@ from tests.test_kv4_gpu import BF16, F16, half_unit, mask_of, pools
 
 pytestmark = pytest.mark.gpu
 
-# hq, hkv, d, cached, new: one CTA of 128 and of 256 rows, its key range split, pages expanded first
+# hq, hkv, d, cached, new: the decode kernel (one token; a block), one CTA of 128 and of 256 rows, its key range split, pages expanded first
 FORMS = {
+    "decode": (16, 4, 128, [300, 45, 1000], [1, 1, 1]),
+    "decode_16_heads": (16, 1, 128, [300, 45, 1000], [1, 1, 1]),
+    "decode_256": (16, 2, 256, [300, 45, 700], [1, 1, 1]),
+    "block": (8, 4, 128, [300, 45], [5, 5]),
     "one_cta": (16, 4, 128, [300, 45], [30, 22]),
     "one_cta_256": (16, 4, 256, [300, 45], [30, 22]),
     "one_cta_two_tiles": (16, 4, 128, [200, 45], [90, 150]),
