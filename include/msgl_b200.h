@@ -162,8 +162,9 @@ int msgl_paged_decode_attention_static(
  * msgl_paged_decode_attention_static on the current device): waits for the work
  * queued on `stream`, copies the word to the host, clears it on the device if
  * `clear` is non-zero.  Returns MSGL_OK if it was 0, else MSGL_DEVICE_STATUS with
- * a message that names the condition; *status_out (may be NULL) receives the raw
- * word.  The only entry point that waits for the device.  No counterpart in the
+ * a message that names the conditions; *status_out (may be NULL) receives the raw
+ * word, to which each adds its bit (1: a bounded wait ran out; 2: a slot, page id or length outside the pool; 4: a number that a
+ * 4-bit pool does not hold).  The only entry point that waits for the device.  No counterpart in the
  * reference (its kernels do not check slot ids).
  */
 int msgl_read_status(void* workspace, int clear, int* status_out, void* stream);

@@ -326,7 +326,7 @@ __global__ void bounded_wait_selftest_kernel(int* status, long long limit_cycles
   const bool all_out = __all_sync(0xffffffffu, !ok);
   __syncthreads();
   if (threadIdx.x == 0) msgl::mbar_inval(msgl::smem_u32(&bar));
-  if (all_out && (threadIdx.x & 31) == 0) atomicExch(status, 1);
+  if (all_out && (threadIdx.x & 31) == 0) atomicOr(status, 1);
 }
 
 // ---- small data-movement kernels
@@ -349,7 +349,7 @@ __global__ void store_kv_kernel(unsigned char* __restrict__ kc, unsigned char* _
     const int c = static_cast<int>(i - static_cast<int64_t>(r) * vec_per_row);
     const int slot = indices[r];
     if (slot < 0 || slot >= num_slots) {
-      if (status) atomicExch(status, 2);
+      if (status) atomicOr(status, 2);
       continue;
     }
     const int64_t src = r * input_row_bytes + static_cast<int64_t>(c) * VEC_BYTES;
@@ -375,10 +375,10 @@ __global__ void gather_kv_indices_kernel(const int32_t* __restrict__ page_table,
   bool bad = begin < 0 || len < 0 || r < 0 || r >= num_rows;
   if (!bad && (len > num_cols || begin + len > total_kv)) {
     len = max(static_cast<int64_t>(0), min(num_cols, total_kv - begin));
-    if (status && threadIdx.x == 0 && blockIdx.x == 0) atomicExch(status, 2);
+    if (status && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(status, 2);
   }
   if (bad) {
-    if (status && threadIdx.x == 0 && blockIdx.x == 0) atomicExch(status, 2);
+    if (status && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(status, 2);
     return;
   }
   const int32_t* row = page_table + r * row_stride;
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(256) build_metadata_kernel(const MetadataParam
     p.prefix_lens[b] = k - e;
     const int chunk = p.split_chunk > 0 ? p.split_chunk : 128;
     p.num_kv_splits[b] = min(p.max_kv_splits, max(1, (k + chunk - 1) / chunk));
-    if (bad && p.status) atomicExch(p.status, 2);
+    if (bad && p.status) atomicOr(p.status, 2);
   }
   if (bad) return;
   const int32_t* row = p.page_table + r * p.row_stride;
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(256) build_metadata_kernel(const MetadataParam
     if (p.kv_indices) p.kv_indices[k0 + t] = slot;
     if (p.page_indices && t % p.page_size == 0) {
       if (slot < 0 || slot % p.page_size != 0) {
-        if (p.status) atomicExch(p.status, 2);     // a sequence that does not start its pages on page boundaries
+        if (p.status) atomicOr(p.status, 2);     // a sequence that does not start its pages on page boundaries
         p.page_indices[g0 + t / p.page_size] = -1;
       } else {
         p.page_indices[g0 + t / p.page_size] = slot / p.page_size;
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(256)
     kv_lens[b] = m.kv;
     const int chunk = p.split_chunk > 0 ? p.split_chunk : 128;
     p.num_kv_splits[b] = min(p.max_kv_splits, max(1, (k + chunk - 1) / chunk));
-    if (bad && p.status) atomicExch(p.status, 2);
+    if (bad && p.status) atomicOr(p.status, 2);
   }
   if (bad) return;
   const int32_t* row = p.page_table + static_cast<int64_t>(m.row) * p.row_stride;
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(256)
     for (int g = first; g < npg; g += stride) {
       const int32_t slot = row[static_cast<int64_t>(g) * p.page_size];
       const bool off = slot < 0 || slot % p.page_size != 0;   // pages must start on page boundaries
-      if (off && p.status) atomicExch(p.status, 2);
+      if (off && p.status) atomicOr(p.status, 2);
       p.page_indices[m.g0 + g] = off ? -1 : slot / p.page_size;
     }
   }
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(1024) page_lens_scan_kernel(const int32_t* __r
       len = kv_lens[i];
       const int64_t cap = static_cast<int64_t>(page_indptr[i + 1] - page_indptr[i]) * page_size;
       if (len < 0 || len > cap) {
-        if (status) atomicExch(status, 2);
+        if (status) atomicOr(status, 2);
         len = len < 0 ? 0 : static_cast<int>(cap < 0 ? 0 : cap);
       }
     }
@@ -586,7 +586,7 @@ __global__ void expand_page_indices_kernel(const int32_t* __restrict__ page_indp
   const int len = kv_indptr[b + 1] - begin;
   const int64_t first = page_indptr[b];
   if (first < 0 || first > total_pages) {
-    if (status && threadIdx.x == 0 && blockIdx.x == 0) atomicExch(status, 2);
+    if (status && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(status, 2);
     for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < len; t += gridDim.x * blockDim.x)
       kv_indices[begin + t] = -1;
     return;
@@ -597,7 +597,7 @@ __global__ void expand_page_indices_kernel(const int32_t* __restrict__ page_indp
     int64_t slot = -1;
     if (first + pg < total_pages) slot = static_cast<int64_t>(pages[pg]) * page_size + (t - pg * page_size);
     if (slot < 0 || slot >= num_slots) {
-      if (status) atomicExch(status, 2);
+      if (status) atomicOr(status, 2);
       slot = -1;
     }
     kv_indices[begin + t] = static_cast<int32_t>(slot);
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const GatherRowsParams
         row = static_cast<int>(to);
         slot = __ldg(ids + t0 + lane);
         if (slot < -1 || slot >= p.num_slots) {
-          if (p.status) atomicExch(p.status, 2);
+          if (p.status) atomicOr(p.status, 2);
           slot = -1;
         }
       }
@@ -1015,12 +1015,15 @@ int msgl_read_status(void* workspace, int clear, int* status_out, void* stream) 
   if (e != cudaSuccess) return cuda_fail("read_status", e);
   if (status_out) *status_out = value;
   if (value == 0) return MSGL_OK;
-  return fail(MSGL_DEVICE_STATUS,
-              value == 1 ? "read_status: a bounded wait inside a kernel ran out (results are not valid)"
-              : value == 2
-                  ? "read_status: a slot or page id outside the pool, or a length beyond a sequence's "
-                    "pages, was met (those rows were read as zeros)"
-                  : "read_status: unknown device status " + std::to_string(value));
+  std::string what;
+  auto add = [&](int bit, const char* text) {
+    if (value & bit) what += (what.empty() ? "" : "; ") + std::string(text);
+  };
+  add(1, "a bounded wait inside a kernel ran out (results are not valid)");
+  add(2, "a slot or page id outside the pool, or a length beyond a sequence's pages, was met (those rows were read as zeros)");
+  add(4, "a number that is not finite, or above 2^15, was stored into a 4-bit pool (as 0 or 2^15)");
+  if (value & ~7) what += (what.empty() ? "" : "; ") + ("unknown device status " + std::to_string(value));
+  return fail(MSGL_DEVICE_STATUS, "read_status: " + what);
 }
 
 int msgl_selftest_bounded_wait(void* workspace, int limit_us, void* stream) {

@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(NWARPS * 32, HD == 256 ? 1 : 2)
       if (id >= 0 && row + rows <= p.num_slots) w.y = static_cast<int>(row);
       else {                                        // page or slot outside the pool: zeros
         if (PAGED) w.y = static_cast<int>(p.num_slots);
-        if (p.status) atomicExch(p.status, 2);
+        if (p.status) atomicOr(p.status, 2);
       }
     }
     if constexpr (!PAGED) {
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(NWARPS * 32, HD == 256 ? 1 : 2)
   Segment cs;
   for (int b = b0; segment(cw, b, cs); ++b) {
     if (PAGED && h == 0 && threadIdx.x == 0 && cs.beg >= r0 && p.status && __ldg(kv_lens + b) != cs.len)
-      atomicExch(p.status, 2);   // a length that is negative or beyond the sequence's pages: clamped, reported
+      atomicOr(p.status, 2);   // a length that is negative or beyond the sequence's pages: clamped, reported
     if (cs.ng == 0 && cs.end > cs.beg) continue;   // (only its padding is in this share)
     // Q: fragments in registers (rows = query heads of this KV head, rows >= G are zero); at head_dim
     // 256, where they would spill, a swizzled tile in shared memory
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(NWARPS * 32, HD == 256 ? 1 : 2)
       write_decode_row<T, VPL>(out, gate, oi, num);
     }
   }
-  if (!alive && p.status && lane == 0) atomicExch(p.status, 1);   // a wait ran out
+  if (!alive && p.status && lane == 0) atomicOr(p.status, 1);   // a wait ran out
 }
 
 }  // namespace msgl

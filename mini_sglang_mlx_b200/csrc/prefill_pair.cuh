@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
     // a length that is negative or exceeds the sequence's pages was clamped: report it
     const int64_t cap = static_cast<int64_t>(p.page_indptr[it.b + 1] - p.page_indptr[it.b]) * p.page_size;
     const int len = p.kv_lens[it.b];
-    if (len < 0 || len > cap) atomicExch(p.status, 2);
+    if (len < 0 || len > cap) atomicOr(p.status, 2);
   }
 
   // ---- geometry: the pair's key range, this CTA's rows
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
               const int64_t row0 = static_cast<int64_t>(pg) * p.page_size + (t - page * p.page_size);
               const int nv = min(kTmaBoxRows, sq.L - t);
               if (pg < 0 || row0 + nv > p.num_slots) {
-                if (p.status) atomicExch(p.status, 2);     // page outside the pool: rows read as zeros
+                if (p.status) atomicOr(p.status, 2);     // page outside the pool: rows read as zeros
               } else {
                 d.a[0] = static_cast<int>(row0);
                 d.n = nv;
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
               int slot = -1;
               if (lane * 4 < RT && tile < ntiles && t < kv_hi) {
                 slot = __ldg(ids + t);
-                if ((slot < -1 || static_cast<int64_t>(slot) >= p.num_slots) && p.status) atomicExch(p.status, 2);
+                if ((slot < -1 || static_cast<int64_t>(slot) >= p.num_slots) && p.status) atomicOr(p.status, 2);
               }
               d.a[e] = slot < 0 || static_cast<int64_t>(slot) >= p.num_slots ? absent : slot;
             }
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
           const int t = kv_lo + tile * BN + row0 + lane;
           int slot = tile < ntiles && t < kv_hi ? __ldg(ids + t) : -1;
           if (slot < -1 || static_cast<int64_t>(slot) >= p.num_slots) {
-            if (p.status) atomicExch(p.status, 2);
+            if (p.status) atomicOr(p.status, 2);
             slot = -1;
           }
           return slot;
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
         cp_async_wait_all();
       }
       if (!alive) {
-        if (p.status && lane == 0) atomicExch(p.status, 1);
+        if (p.status && lane == 0) atomicOr(p.status, 1);
         // gave up: let the copies still in flight land before the shared memory goes away
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) {
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
         }
         __syncwarp();
       }
-      if (!alive && p.status && lane == 0) atomicExch(p.status, 1);
+      if (!alive && p.status && lane == 0) atomicOr(p.status, 1);
     } else if (!PAGED && warp == Shape::kMmaWarp) {
       // =========================================================== relay of the peer's V copies
       // The release at cluster scope that ordinary writes need in front of the leader's MMAs.  A warp without
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
         fence_proxy_async_smem();
         if (alive && lane == 0) mbar_arrive_release_cluster(full0 + ring_seq_v<LA>(t) % NB * 8, 2 * NKW);
       }
-      if (!alive && p.status && lane == 0) atomicExch(p.status, 1);
+      if (!alive && p.status && lane == 0) atomicOr(p.status, 1);
     }
     __syncwarp();
     first_gates();
@@ -864,7 +864,7 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
       }
     }
     write_rows();
-    if (!alive && p.status && r == 0) atomicExch(p.status, 1);
+    if (!alive && p.status && r == 0) atomicOr(p.status, 1);
   }
 
   // ---- teardown: both CTAs are past their last MMA, TMEM access and remote arrival

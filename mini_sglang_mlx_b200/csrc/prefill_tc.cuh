@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     // a length that is negative or exceeds the sequence's pages was clamped: report it
     const int64_t cap = static_cast<int64_t>(p.page_indptr[it.b + 1] - p.page_indptr[it.b]) * p.page_size;
     const int len = p.kv_lens[it.b];
-    if (len < 0 || len > cap) atomicExch(p.status, 2);
+    if (len < 0 || len > cap) atomicOr(p.status, 2);
   }
 
   // ---- geometry of the CTA's rows and of each sub-tile
@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
             const int64_t row0 = static_cast<int64_t>(pg) * p.page_size + (t0 - page * p.page_size);
             const int nv = min(kTmaBoxRows, sq.L - t0);
             if (pg < 0 || row0 + nv > p.num_slots) {
-              if (p.status) atomicExch(p.status, 2);   // page outside the pool: rows read as zeros
+              if (p.status) atomicOr(p.status, 2);   // page outside the pool: rows read as zeros
             } else {
               y = static_cast<int>(row0);
               n = nv;
@@ -993,7 +993,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       auto stage_slot = [&](int tile, int slot) {
         if (ptid < BN) {
           if (slot < -1 || static_cast<int64_t>(slot) >= p.num_slots) {
-            if (p.status) atomicExch(p.status, 2);
+            if (p.status) atomicOr(p.status, 2);
             slot = -1;
           }
           s_slots[(tile % (LA + 1)) * BN + ptid] = slot;
@@ -1046,7 +1046,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       }
     }
     cp_async_wait<0>();
-    if (!alive && p.status && ptid == 0) atomicExch(p.status, 1);
+    if (!alive && p.status && ptid == 0) atomicOr(p.status, 1);
   } else if (warp == kMmaWarp) {
     // =========================================================== MMA issuer
     {
@@ -1141,7 +1141,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
       }
       __syncwarp();
     }
-    if (!alive && p.status && lane == 0) atomicExch(p.status, 1);
+    if (!alive && p.status && lane == 0) atomicOr(p.status, 1);
     }
   }
   } else {
@@ -1490,7 +1490,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
 #endif
       }
     }
-    if (!alive && p.status && r == 0) atomicExch(p.status, 1);
+    if (!alive && p.status && r == 0) atomicOr(p.status, 1);
 #ifdef MSGL_TRACE
     if (tid == 0) MSGL_TR(7, clock64());               // output written
 #endif
