@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
   const int32_t* const indptr = after_wait(p.page_indptr);
   const int32_t* const pages = after_wait(p.page_indices);
   const int32_t* const lens = after_wait(p.kv_lens);
+  const int32_t* const new_tokens = BLOCKS ? after_wait(p.qo_indptr) : nullptr;
+  const int32_t* const prefixes = BLOCKS ? after_wait(p.prefix_lens) : nullptr;
   const T* const q = after_wait(static_cast<const T*>(p.q));
   const unsigned char* const kp = after_wait(p.k_pool);
   const unsigned char* const vp = after_wait(p.v_pool);
@@ -156,9 +158,9 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
     k.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(lens + b), 0)), cap));
     k.first = 0;
     if constexpr (BLOCKS) {
-      k.tok0 = min(max(__ldg(p.qo_indptr + b), 0), p.total_q);
-      k.new_tok = max(min(__ldg(p.qo_indptr + b + 1), p.total_q) - k.tok0, 0);
-      k.prefix = __ldg(p.prefix_lens + b);
+      k.tok0 = min(max(__ldg(new_tokens + b), 0), p.total_q);
+      k.new_tok = max(min(__ldg(new_tokens + b + 1), p.total_q) - k.tok0, 0);
+      k.prefix = __ldg(prefixes + b);
       const int hi = p.is_cross ? k.len : static_cast<int>(min(static_cast<int64_t>(k.len), static_cast<int64_t>(k.prefix) + k.new_tok));
       const int lo = p.window > 0 ? max(0, k.prefix - p.window + 1) : 0;
       k.first = lo / kKv4Rows;

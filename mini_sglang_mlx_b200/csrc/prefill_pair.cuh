@@ -675,10 +675,11 @@ __global__ void __launch_bounds__(PairShape<HD, PAGED>::kThreads, 1)
     }
     float v_power = 1.f;
     if constexpr (EXPANDED) {
-      row_scale *= sequence_power(p.kv_tops, it.b, p.hkv, h, 0, lane);
+      const uint32_t* const tops = after_wait(p.kv_tops);
+      row_scale *= sequence_power(tops, it.b, p.hkv, h, 0, lane);
       // (above zero also where the powers leave nothing: a masked score is -inf)
       if (!sc_neg) row_scale = fmaxf(row_scale, 1.17549435e-38f);
-      v_power = sequence_power(p.kv_tops, it.b, p.hkv, h, 1, lane);
+      v_power = sequence_power(tops, it.b, p.hkv, h, 1, lane);
     }
     const float sc = sc_neg ? 1.f : row_scale;
 
