@@ -518,7 +518,9 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     x.kv_lens = kv_lens;
     x.prefix_lens = prefix_lens;
     x.batch = batch;
+    x.qo_indptr = qo_indptr;
     x.window = sliding_window_size;
+    x.is_cross = is_cross_attention ? 1 : 0;
     x.total_pages = static_cast<int>(total_pages);
     x.page_blocks = page_size / msgl::kKv4Rows;
     x.hkv = num_kv_heads;

@@ -379,8 +379,8 @@ struct Kv4ExpandParams {
   __half *k_rows, *v_rows;      // (total_pages * page_size, hkv, head_dim)
   int32_t* pages;               // (total_pages): 0, 1, ...
   uint32_t* tops;               // (batch, hkv, 2, kRangeParts): the largest t of K and of V in parts of a sequence
-  const int32_t *page_indptr, *kv_lens, *prefix_lens;
-  int batch, window;
+  const int32_t *page_indptr, *kv_lens, *prefix_lens, *qo_indptr;
+  int batch, window, is_cross;
   const void* q;                // (q_rows, head_dim), or null
   __half* q_rows;
   float* q_power;
@@ -451,6 +451,9 @@ __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const Kv4ExpandParam
   grid_dependency_launch();
   const int32_t* ids = after_wait(p.page_indices);
   const int32_t* const indptr = after_wait(p.page_indptr);
+  const int32_t* const lens = after_wait(p.kv_lens);
+  const int32_t* const prefixes = after_wait(p.prefix_lens);
+  const int32_t* const new_tokens = after_wait(p.qo_indptr);
   const uint32_t* const tops = after_wait(p.tops);
   const unsigned char* pools[2] = {after_wait(p.k_pool), after_wait(p.v_pool)};
   const T* q = after_wait(static_cast<const T*>(p.q));
@@ -467,9 +470,16 @@ __global__ void __launch_bounds__(256, 4) kv4_expand_kernel(const Kv4ExpandParam
     const int page = p.page_blocks == 1 ? static_cast<int>(b) : static_cast<int>(b / p.page_blocks);
     const int64_t block = static_cast<int64_t>(__ldg(ids + page)) * p.page_blocks + (b - static_cast<int64_t>(page) * p.page_blocks);
     const bool ok = block >= 0 && block < p.num_blocks;
-    if (!ok && p.status && lane == 0) atomicOr(p.status, 2);
-    const int64_t at = ((ok ? block : 0) * p.hkv + h) * kv4_block_bytes(HD);
     const int seq = sequence_of_page(indptr, p.batch, page, lane);
+    const int64_t t = b * kKv4Rows - static_cast<int64_t>(__ldg(indptr + seq)) * p.page_blocks * kKv4Rows;     // its first token
+    const int len = __ldg(lens + seq);
+    if (t < 0 || t >= len) continue;              // an entry that no sequence has a token in: not read, and not reported
+    if (!ok && lane == 0 && p.status) {           // reported where a row sees it
+      const int prefix = __ldg(prefixes + seq), fresh = __ldg(new_tokens + seq + 1) - __ldg(new_tokens + seq);
+      if ((p.is_cross || t < static_cast<int64_t>(prefix) + fresh) && (p.window == 0 || t + kKv4Rows > static_cast<int64_t>(prefix) - p.window + 1))
+        atomicOr(p.status, 2);
+    }
+    const int64_t at = ((ok ? block : 0) * p.hkv + h) * kv4_block_bytes(HD);
     const float inverse[2] = {power_inverse(sequence_power(tops, seq, p.hkv, h, 0, lane)),
                               power_inverse(sequence_power(tops, seq, p.hkv, h, 1, lane))};
 #pragma unroll (HD == 128 ? 2 : 1)
