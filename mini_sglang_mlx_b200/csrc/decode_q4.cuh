@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
   float* const sm_o = reinterpret_cast<float*>(smem_raw + WARPS * STAGES * U * 2 * BLK);   // [WARPS][8][MROW]
   float* const sm_ml = sm_o + WARPS * 8 * MROW;                                       // [WARPS][8][2]
   if (lane < STAGES) mbar_init(smem_u32(&s_bar[warp * STAGES + lane]), 1);
-  if (GATHER && tid == 0) {
+  if (GATHER && tid == 0 && p.num_rows > 0) {       // (no maps over a pool without slots)
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
   }

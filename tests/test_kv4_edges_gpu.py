@@ -1,0 +1,32 @@
+"""Calls at the edges of what the 4-bit pool's operators take."""
+import math
+
+import pytest
+import torch
+
+from mini_sglang_mlx_b200 import _lib
+from mini_sglang_mlx_b200 import kernel as K
+from oracle import kv4_oracle as Q
+from tests.test_kv4_gpu import BF16, F16, assert_within, mask_of, pools, rows, sequences
+
+
+def ints(x):
+    return torch.as_tensor(x).int().cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(8, 4, 128), (8, 4, 256), (16, 1, 128)])
+def test_a_pool_without_slots(hq, hkv, d):
+    """Through the C ABI: no slots, no pages, nothing but empty sequences: rows of zeros."""
+    lib = _lib.lib()
+    q = torch.ones(3, hq, d, dtype=BF16, device="cuda")
+    some = torch.zeros(64, dtype=BF16, device="cuda")           # (a pointer that nothing is read through)
+    stream = torch.cuda.current_stream().cuda_stream
+    nbytes = lib.msgl_decode_workspace_bytes_q4(3, hq, hkv, d, 0, 16)
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, math.nan)
+    zeros = torch.zeros(4, dtype=torch.int32, device="cuda")
+    assert lib.msgl_paged_decode_attention_q4(q.data_ptr(), some.data_ptr(), some.data_ptr(), zeros.data_ptr(), None, zeros.data_ptr(),
+                                              None, out.data_ptr(), ws.data_ptr(), nbytes, 3, hq, hkv, d, 0, 0, 0.1, 16, 0, stream) == 0
+    torch.cuda.synchronize()
+    assert (out == 0).all()
