@@ -177,9 +177,13 @@ __global__ void __launch_bounds__(WARPS * 32, MINB)
     const int b = lane * run + j;
     if (b < p.batch) sum = min(sum + room(keys(b).blocks), 1 << 28);
   }
-  // (All pages of a call hold less than 2^27 blocks.  Row pointers that lay more end to end are none of a batch: no positions for them.)
+  // (All pages of a call hold less than 2^27 blocks.  Row pointers that lay more end to end are none of a batch: no positions for
+  // them, and zeros for the rows.)
   if (__reduce_add_sync(0xffffffffu, sum >> 8) > 1 << 20) {
     if (blockIdx.x == 0 && tid == 0 && p.status) atomicOr(p.status, 2);
+    const int64_t pieces = static_cast<int64_t>(BLOCKS ? p.total_q : p.batch) * p.hq * (HD / 8);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (WARPS * 32) + tid; i < pieces; i += static_cast<int64_t>(gridDim.x) * (WARPS * 32))
+      static_cast<uint4*>(p.out)[i] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
   int incl = sum;

@@ -30,3 +30,24 @@ def test_a_pool_without_slots(hq, hkv, d):
                                               None, out.data_ptr(), ws.data_ptr(), nbytes, 3, hq, hkv, d, 0, 0, 0.1, 16, 0, stream) == 0
     torch.cuda.synchronize()
     assert (out == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 2])
+def test_row_pointers_that_fit_no_batch_give_zeros(new):
+    """(One call's workspace is the next one's: what is right afterwards shows that nothing was left in it.)"""
+    batch, pages = 16384, 4096
+    kc, vc = pools(pages * 16, 1, 128, BF16, fill=0x3c)
+    ends = ints([0, pages] * (batch // 2) + [0])
+    ids = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    lens = torch.full((batch,), 1 << 20, dtype=torch.int32, device="cuda")
+    q = torch.ones(batch * new, 1, 128, dtype=BF16, device="cuda")
+    for _ in range(2):
+        dirt = torch.full_like(q, math.nan)          # (what the result's memory held)
+        del dirt
+        if new == 1:
+            out = K.paged_decode_attention_q4(q, kc, vc, ends, ids, lens, 0.1, page_size=256)
+        else:
+            out = K.paged_prefill_attention_q4(q, kc, vc, torch.arange(0, batch * new + 1, new).int().cuda(), ends, ids, lens,
+                                               lens - new, 0.1, new, page_size=256)
+        assert K.device_status() == 2 and (out == 0).all()
