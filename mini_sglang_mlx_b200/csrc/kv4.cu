@@ -131,8 +131,8 @@ int run_q4(const char* op, msgl::Q4DecodeParams& p, const Q4Plan& pl, void* work
 // 16384 tokens, 8 KV heads, decode kernel / tcgen05: 8 columns 69 us / 222, 16 columns 115 / 222; with 20 to 64 columns as CTAs of
 // 16 side by side, five verify tokens of 40 columns 81 / 63, draft blocks of 64 149 / 86 (56 and 72 since).
 constexpr int kQ4BlockColumns = 16;
-bool q4_block_form(int max_len_extend, int group) {
-  return static_cast<int64_t>(max_len_extend) * group <= kQ4BlockColumns;
+bool q4_block_form(int batch, int max_len_extend, int group) {
+  return batch <= 65535 && static_cast<int64_t>(max_len_extend) * group <= kQ4BlockColumns;
 }
 // Blocks of a call at most: what the pages hold, or what a window leaves.
 int64_t q4_block_bound(int batch, int64_t total_pages, int page_size, int max_len_extend, int window) {
@@ -155,7 +155,7 @@ bool q4_expands(int batch, int total_q, int64_t total_kv, int hq, int hkv, int h
   if (!prefill_pairs(batch, total_q, total_kv, hq / hkv, hkv, head_dim, max_len_extend, cross, window, pl.kv_chunk, true, sms))
     return false;
   double keys = std::max(1., static_cast<double>(total_kv) / batch - (cross ? 0. : 0.5 * total_q / batch));
-  if (window > 0) keys = std::min<double>(keys, window + max_len_extend);
+  if (window > 0) keys = std::min<double>(keys, static_cast<double>(window) + max_len_extend);
   const double attend_us = 4. * head_dim * hq * static_cast<double>(total_q) * keys / 1e9;             // at 1 PFLOP/s
   const double copy_us = 5. + (static_cast<double>(total_kv) * hkv * 5.2 + static_cast<double>(total_q) * hq * 4.) * head_dim / 4e6;
   return attend_us > (head_dim == 256 ? kQ4ExpandWorth256 : kQ4ExpandWorth128) * copy_us;
@@ -373,7 +373,7 @@ size_t msgl_prefill_workspace_bytes_q4(int batch, int total_q, int64_t total_pag
     return kStatusBytes;
   max_len_extend = std::max(1, max_len_extend);
   const int group = std::max(1, num_q_heads / num_kv_heads);
-  if (!q4_block_form(max_len_extend, group))
+  if (!q4_block_form(batch, max_len_extend, group))
     return msgl_prefill_workspace_bytes(batch, total_q, total_pages * page_size, num_q_heads, num_kv_heads, head_dim,
                                         max_len_extend, sliding_window_size);
   const int sms = sm_count_cached();
@@ -427,7 +427,7 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     return fail(MSGL_BAD_ARG, std::string(op) + "q, the pools, out, gate and the workspace must be 16-byte aligned");
   const int sms = sm_count_cached();
   if (sms <= 0) return fail(MSGL_CUDA_ERROR, std::string(op) + "cannot query the device");
-  if (batch <= 65535 && q4_block_form(max_len_extend, num_q_heads / num_kv_heads)) {
+  if (q4_block_form(batch, max_len_extend, num_q_heads / num_kv_heads)) {
     const Q4Plan blocks = plan_q4(batch, max_len_extend * (num_q_heads / num_kv_heads), num_kv_heads, head_dim,
                                   q4_block_bound(batch, total_pages, page_size, max_len_extend, sliding_window_size), sms);
     msgl::Q4DecodeParams p{};

@@ -51,3 +51,26 @@ def test_row_pointers_that_fit_no_batch_give_zeros(new):
             out = K.paged_prefill_attention_q4(q, kc, vc, torch.arange(0, batch * new + 1, new).int().cuda(), ends, ids, lens,
                                                lens - new, 0.1, new, page_size=256)
         assert K.device_status() == 2 and (out == 0).all()
+
+
+def test_workspace_of_a_batch_beyond_the_decode_kernels():
+    """More sequences than a grid of the decode kernel numbers go to the tile kernel: its workspace, whatever the block's columns."""
+    lib = _lib.lib()
+    for batch in (65535, 65536, 70000):
+        got = lib.msgl_prefill_workspace_bytes_q4(batch, batch, batch, 16, 16, 2, 128, 1, 0)
+        tiles = lib.msgl_prefill_workspace_bytes(batch, batch, batch * 16, 16, 2, 128, 1, 0)
+        assert (got == tiles) == (batch > 65535)
+
+
+@pytest.mark.gpu
+def test_prefill_of_more_sequences_than_the_decode_kernel_numbers():
+    gen = torch.Generator().manual_seed(41)
+    batch = 66000
+    lens = [1 + i % 5 for i in range(batch)]
+    kc, vc, indptr, order, slots = sequences(gen, lens, 16, 1, 128, BF16)
+    q = torch.randn(batch, 2, 128, generator=gen).to(BF16)
+    out = K.paged_prefill_attention_q4(q.cuda(), kc, vc, torch.arange(batch + 1).int().cuda(), ints(indptr), ints(order), ints(lens),
+                                       ints(lens) - 1, 0.09, 1)
+    for b in (0, 1, 65534, 65535, 65536, batch - 1):
+        assert_within(out[b:b + 1], *Q.attention(q[b:b + 1], kc, vc, slots[b], torch.ones(1, lens[b], dtype=torch.bool), 0.09), BF16)
+    assert K.device_status() == 0
