@@ -74,3 +74,90 @@ def test_prefill_of_more_sequences_than_the_decode_kernel_numbers():
     for b in (0, 1, 65534, 65535, 65536, batch - 1):
         assert_within(out[b:b + 1], *Q.attention(q[b:b + 1], kc, vc, slots[b], torch.ones(1, lens[b], dtype=torch.bool), 0.09), BF16)
     assert K.device_status() == 0
+
+
+BLOCKS = [
+    # hq, hkv, d, dtype, page_size, cached, new
+    (8, 8, 128, BF16, 16, [700, 33], [5, 16]),
+    (16, 4, 128, F16, 16, [0, 1000, 17], [1, 4, 3]),
+    (32, 8, 128, BF16, 32, [2000, 300], [4, 4]),
+    (8, 4, 256, BF16, 16, [500, 3], [2, 8]),
+    (16, 2, 256, F16, 64, [90, 4000], [2, 2]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,dtype,page_size,cached,new", BLOCKS)
+@pytest.mark.parametrize("cross,window", [(False, 1), (False, 3), (False, 40), (False, 5000), (True, 0), (True, 40), (True, 2)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_masks_of_short_blocks(hq, hkv, d, dtype, page_size, cached, new, cross, window, gated):
+    """Up to sixteen rows a KV head run the decode kernel: sliding windows and bidirectional masks against 64 bits."""
+    assert max(new) * hq // hkv <= 16
+    gen = torch.Generator().manual_seed(hq + d + window)
+    lens = [a + b for a, b in zip(cached, new)]
+    kc, vc, indptr, order, slots = sequences(gen, lens, page_size, hkv, d, dtype)
+    q = torch.randn(sum(new), hq, d, generator=gen).to(dtype)
+    gate = torch.randn(q.shape, generator=gen).to(dtype) if gated else None
+    qo = torch.tensor([0] + new).cumsum(0).int()
+
+    def call(gate):
+        return K.paged_prefill_attention_q4(q.cuda(), kc, vc, ints(qo), ints(indptr), ints(order), ints(lens), ints(cached), 0.09, max(new),
+                                            page_size=page_size, is_cross_attention=cross, sliding_window_size=window, gate=gate)
+
+    plain = call(None)
+    parts = [Q.attention(q[qo[b]:qo[b + 1]], kc, vc, s, mask_of(cached[b], new[b], cross, window), 0.09) for b, s in enumerate(slots)]
+    ref, weighted, size = (torch.cat(x) for x in zip(*parts))
+    assert_within(plain, ref, weighted, size, dtype)
+    if gated:      # (the output, the sigmoid and the product are rounded: three half units; one is in `plain`)
+        g, u = torch.sigmoid(gate.double()), torch.finfo(dtype).eps / 2
+        err = (call(gate.cuda()).double().cpu() - ref * g).abs()
+        assert (err <= (plain.double().cpu() - ref).abs() * g * (1 + 4 * u) + 2.1 * u * (ref * g).abs() + 1e-6).all()
+    assert K.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,page_size", [(128, 16), (256, 32)])
+def test_a_cached_prefix_over_4_bit_pages(d, page_size):
+    """Prompts that share prefixes, through the radix cache: a request's new tokens attend to pages that another one filled."""
+    from types import SimpleNamespace
+
+    import numpy as np
+
+    from mini_sglang_mlx_b200.attention import AttnBackend
+    from mini_sglang_mlx_b200.core import Batch, BatchPhase, Req
+    from mini_sglang_mlx_b200.kvcache import MHAKVCacheQ4
+    from mini_sglang_mlx_b200.scheduler import CacheManager, TableManager
+
+    gen = torch.Generator().manual_seed(43)
+    hq, hkv, vocab, pages = 8, 2, 300, 80
+    emb_q, emb_k, emb_v = (rows(gen, vocab, h, d, BF16) for h in (hq, hkv, hkv))
+    pool = MHAKVCacheQ4(hkv, 1, d, pages * page_size, BF16)
+    table = torch.zeros((5, 640), dtype=torch.int32, device="cuda")
+    tm, cm = TableManager(4, table), CacheManager("cuda", pages, page_size=page_size)
+    backend = AttnBackend(SimpleNamespace(head_dim=d, num_kv_heads=hkv), pool, table, page_size=page_size)
+    rng = np.random.default_rng(3)
+    shared = rng.integers(0, vocab, size=300).tolist()
+    prompts = [shared[:200] + rng.integers(0, vocab, size=17).tolist(), shared[:150] + rng.integers(0, vocab, size=60).tolist(),
+               shared[:200] + rng.integers(0, vocab, size=1).tolist(), shared[:150] + rng.integers(0, vocab, size=333).tolist()]
+    reused = 0
+    for tokens in prompts:
+        n, t = len(tokens), torch.tensor(tokens)
+        handle, cached = cm.match_req(SimpleNamespace(input_ids=np.asarray(tokens, dtype=np.int32), input_len=n))
+        have = handle.cached_len
+        reused += have
+        cm.lock(handle)
+        row = tm.allocate()
+        table[row, :have] = cached
+        fresh = cm.allocate(n - have, start=have)
+        table[row, have:n] = fresh
+        batch = Batch(reqs=[Req(table_idx=row, cached_len=have, device_len=n)], phase=BatchPhase.PREFILL, out_loc=fresh)
+        backend.prepare_metadata(batch)
+        out = backend.forward(*(e[t[have:]].cuda() for e in (emb_q, emb_k, emb_v)), 0, batch)
+        own = [torch.zeros(K.kv_cache_q4_shape(n, hkv, d), dtype=BF16) for _ in range(2)]      # the whole prompt, in a pool of its own
+        for p, e in zip(own, (emb_k, emb_v)):
+            Q.write(p, e[t], range(n))
+        assert_within(out, *Q.attention(emb_q[t[have:]], *own, torch.arange(n), mask_of(have, n - have, False, 0), backend.sm_scale), BF16)
+        cm.free_and_cache_finished_req(handle, np.asarray(tokens, np.int32), table[row, :n])
+        tm.free(row)
+        cm.check_integrity()
+    assert reused >= 400 and K.device_status() == 0
