@@ -418,8 +418,9 @@ __global__ void __launch_bounds__(256) kv4_range_kernel(const Kv4ExpandParams p)
   if (from < len)
     top = pair_range<T, HD, 256>(after_wait(p.k_pool), after_wait(p.v_pool), p.hkv, h, static_cast<int>(from),
                                  static_cast<int>(min(from + per, static_cast<int64_t>(len))), p.num_blocks, threadIdx.x, [&](int t) -> int64_t {
-                                   const int page = t / page_size;
-                                   return static_cast<int64_t>(__ldg(ids + begin + page)) * p.page_blocks + (t - page * page_size) / kKv4Rows;
+                                   const int page = t / page_size, at = begin + page;
+                                   if (at < 0 || at >= p.total_pages) return -1;
+                                   return static_cast<int64_t>(__ldg(ids + at)) * p.page_blocks + (t - page * page_size) / kKv4Rows;
                                  });
   if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
   __syncthreads();
