@@ -516,7 +516,7 @@ int msgl_load_kv_cache_q4(const void* k_cache, const void* v_cache, const int32_
 /*
  * msgl_qk_norm_rope_store for this pool: the rotated, rounded keys and the values are quantised into it.  q is
  * read (any token stride) and its result goes to q_out (n_tokens, num_q_heads, head_dim), contiguous.  Positions
- * below 2^24; the angle is good to 1e-6 turns whatever the position.
+ * below 2^24; sines and cosines are taken in 64 bits and rounded to fp32, products and sums are separate fp32 operations.
  */
 int msgl_qk_norm_rope_store_q4(const void* q, const void* k, const void* v, const void* q_weight,
                                const void* k_weight, const int32_t* positions, const int32_t* out_loc, void* q_out,

@@ -299,6 +299,7 @@ int msgl_qk_norm_rope_store_q4(const void* q, const void* k, const void* v, cons
   p.num_slots = num_slots;
   p.log2_base = std::log2(rope_base);
   p.eps = eps;
+  p.minus_zero = -0.f;
   p.status = static_cast<int*>(status_word);
   auto* kernel = head_dim == 256 ? (dtype == MSGL_DTYPE_BF16 ? msgl::kv4_project_kernel<__nv_bfloat16, 256>
                                                              : msgl::kv4_project_kernel<__half, 256>)

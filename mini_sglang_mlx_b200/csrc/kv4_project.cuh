@@ -4,9 +4,10 @@
 // y = x * rsqrt(mean(x^2) + eps) * w in fp32, rounded to the 16-bit type (the array that the layer's norm gives); pairs
 // (i, i + rd/2) rotated by position * base^(-2i/rd), rounded once more; what is quantised is that rounded key, the one a
 // 16-bit pool would hold.  Where a rounding falls the other way a code can, and an element is off by a whole step of its
-// group, so the chain in front of the roundings is that of separate fp32 operations (no product is fused with a sum), and sine and cosine are good to a unit
-// in the last place: the angle is kept in turns, position times a frequency of two floats, exact to 2^-33 turns at 10^5
-// tokens (one float of frequency leaves an angle of 10^5 radians 6e-3 off).
+// group, so the chain in front of the roundings is that of separate fp32 operations, over sines and
+// cosines that are those of 64 bits rounded once: the angle is kept in quarter turns, position times frequency in 64 bits, exact to 2^-37 of one
+// at 10^5 tokens, and what is left of it within an eighth of a turn goes into Taylor's polynomials to the 13th power.  (Products fused with the sum
+// behind them turn one rounding in 10^5 the other way.)
 //
 // A work item is a few rows of one token and one kind (q, k or v), one after the other, the next on its way: angles and
 // weights are the item's, and the code is short (with four rows unrolled the kernel waited for instructions as much as for
@@ -34,9 +35,32 @@ struct Kv4ProjectParams {
   int64_t num_slots;
   double log2_base;
   float eps;
+  float minus_zero;          // -0, which the compiler does not know: see product
   int* status;
 };
 __host__ __device__ constexpr int kv4_project_lanes(int hd) { return hd / 8; }
+
+// Sine and cosine of pos * freq quarter turns (below 2^51 of them).
+__device__ __forceinline__ void sine_cosine(double pos, double freq, float& sine, float& cosine) {
+  const double magic = 6755399441055744.;                  // 1.5 * 2^52: the sum's lowest bits are the rounded number
+  const double whole = fma(pos, freq, magic);
+  const double z = fma(pos, freq, magic - whole) * 1.5707963267948966, y = z * z;      // |z| <= pi / 4
+  double s = fma(y, 1. / 6227020800., -1. / 39916800.), c = fma(y, 1. / 479001600., -1. / 3628800.);
+  s = fma(y, s, 1. / 362880.);
+  c = fma(y, c, 1. / 40320.);
+  s = fma(y, s, -1. / 5040.);
+  c = fma(y, c, -1. / 720.);
+  s = fma(y, s, 1. / 120.);
+  c = fma(y, c, 1. / 24.);
+  s = fma(y, s, -1. / 6.);
+  c = fma(y, c, -1. / 2.);
+  const float s1 = static_cast<float>(fma(y * z, s, z)), c1 = static_cast<float>(fma(y, c, 1.));
+  const int k = __double2loint(whole);                     // quarter turns, modulo 4
+  sine = k & 1 ? c1 : s1;
+  cosine = k & 1 ? s1 : c1;
+  if (k & 2) sine = -sine;
+  if ((k + 1) & 2) cosine = -cosine;
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectParams p) {
@@ -46,6 +70,9 @@ __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectPar
   __shared__ __align__(16) float s_weight[2][HD];
   const int lane = threadIdx.x & 31;
   const int hl = lane & (LANES - 1);
+  // A product that stays one: mul.rn.f32x2 and the add behind it come out of the compiler as one operation.
+  const uint64_t nothing = pack_f32x2(p.minus_zero, p.minus_zero);
+  auto product = [&](uint64_t a, uint64_t b) -> uint64_t { return fma_f32x2(a, b, nothing); };
   const uint32_t hmask = LANES == 32 ? 0xffffffffu : (lane & 16) ? 0xffff0000u : 0x0000ffffu;
   const uint32_t gmask = (lane & 16) ? 0xffff0000u : 0x0000ffffu;     // the sixteen lanes of a group
   const int half = p.rotary_dim >> 1;
@@ -53,13 +80,9 @@ __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectPar
   const int xm = in_lane ? 0 : half / 4;             // pairs inside the lower half of the row: the partner is lane ^ xm
   const bool rot_lane = in_lane || hl < 2 * xm;
   const int f0 = in_lane ? 4 * hl : 4 * (hl & (xm - 1));
-  float f_hi[4], f_lo[4];                            // turns per token
+  double freq[4];                                    // quarter turns per token
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const double f = exp2(-p.log2_base * static_cast<double>(f0 + e) / half) * 0.15915494309189535;
-    f_hi[e] = static_cast<float>(f);
-    f_lo[e] = static_cast<float>(f - f_hi[e]);
-  }
+  for (int e = 0; e < 4; ++e) freq[e] = exp2(-p.log2_base * static_cast<double>(f0 + e) / half) * 0.63661977236758134;
   grid_dependency_wait();
   grid_dependency_launch();
   const T* const q = after_wait(static_cast<const T*>(p.q));
@@ -95,19 +118,10 @@ __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectPar
     const float* weight = s_weight[is_q ? 0 : 1];
     uint2 lo = reinterpret_cast<const uint2*>(src)[hl], hi = reinterpret_cast<const uint2*>(src)[LANES + hl];
     if (!is_v) {
-      const float pos = static_cast<float>(positions[tok]);
+      const double pos = static_cast<double>(positions[tok]);
       float c4[4], s4[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float t = pos * f_hi[e];
-        const float rest = fmaf(pos, f_lo[e], fmaf(pos, f_hi[e], -t));
-        const float part = t - rintf(t), x = part + rest;              // turns, in [-1/2, 1/2]
-        const float off = 6.2831854820251465f * (rest - (x - part));   // what the sum lost, in radians
-        float s0, c0;
-        sincospif(2.f * x, &s0, &c0);
-        s4[e] = fmaf(off, c0, s0);
-        c4[e] = fmaf(-off, s0, c0);
-      }
+      for (int e = 0; e < 4; ++e) sine_cosine(pos, freq[e], s4[e], c4[e]);
       const float sign = in_lane || hl < xm ? -1.f : 1.f;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -143,8 +157,8 @@ __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectPar
           if constexpr (LANES == 32) {
             float* part = s_part + (threadIdx.x >> 5) * 128;
             float4 u;
-            unpack_f32x2(add_f32x2(mul_f32x2(a[0], a[0]), mul_f32x2(b[0], b[0])), u.x, u.y);
-            unpack_f32x2(add_f32x2(mul_f32x2(a[1], a[1]), mul_f32x2(b[1], b[1])), u.z, u.w);
+            unpack_f32x2(add_f32x2(product(a[0], a[0]), product(b[0], b[0])), u.x, u.y);
+            unpack_f32x2(add_f32x2(product(a[1], a[1]), product(b[1], b[1])), u.z, u.w);
             __syncwarp();
             reinterpret_cast<float4*>(part)[hl] = u;
             __syncwarp();
@@ -183,14 +197,14 @@ __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectPar
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint64_t x = a[w];
-            a[w] = add_f32x2(mul_f32x2(x, cs[w]), mul_f32x2(b[w], sm[w]));
-            b[w] = add_f32x2(mul_f32x2(b[w], cs[w]), mul_f32x2(x, sn[w]));
+            a[w] = add_f32x2(product(x, cs[w]), product(b[w], sm[w]));
+            b[w] = add_f32x2(product(b[w], cs[w]), product(x, sn[w]));
           }
         } else {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint64_t other = __shfl_xor_sync(hmask, static_cast<unsigned long long>(a[w]), xm);
-            if (rot_lane) a[w] = add_f32x2(mul_f32x2(a[w], cs[w]), mul_f32x2(other, sm[w]));
+            if (rot_lane) a[w] = add_f32x2(product(a[w], cs[w]), product(other, sm[w]));
           }
         }
         lo = make_uint2(close(a[0]), close(a[1]));
