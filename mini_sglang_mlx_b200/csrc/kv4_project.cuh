@@ -16,7 +16,7 @@
 // one lane, and a group of 64 is in sixteen lanes.
 //
 // What bounds it is instruction issue, some 250 instructions a row that is quantised: 6000 tokens of 16 + 2 x 4 heads of 256, and the
-// read back behind it, 53 us, 3.1 TB/s (one element at a time, squares summed by shuffles and four rows an item unrolled: 74).
+// read back behind it, 51.6 us, 3.2 TB/s (one element at a time and four rows an item unrolled: 74; squares through shared memory 53).
 #pragma once
 
 #include "kv4.cuh"
@@ -66,7 +66,6 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectParams p) {
   constexpr int LANES = kv4_project_lanes(HD), G = HD / kKv4Group;
   const int R = p.item_rows;
-  __shared__ __align__(16) float s_part[HD == 256 ? 256 * 4 : 256 * 8];   // squares on their way to the lanes that sum them
   __shared__ __align__(16) float s_weight[2][HD];
   const int lane = threadIdx.x & 31;
   const int hl = lane & (LANES - 1);
@@ -149,42 +148,24 @@ __global__ void __launch_bounds__(256, 4) kv4_project_kernel(const Kv4ProjectPar
         };
         uint64_t a[2] = {open(lo.x), open(lo.y)}, b[2] = {open(hi.x), open(hi.y)};
         if (norm) {
-          // Sum of the squares, of elements 32 apart first and then of neighbours.  Lane l = 8 i + m holds elements 4 m .. 4 m + 3
-          // of the row's i-th 32 in its lower half, and of the i-th 32 of its upper half; through shared memory it gets all that
-          // is at 4 m + i (head_dim 256, four lanes), or at 4 m + 2 i and 4 m + 2 i + 1 (128, two).
-          const int m = hl & 7, i = hl >> 3;
+          // sum of the squares: this lane's eight elements, then the lanes'
           float ss;
           if constexpr (LANES == 32) {
-            float* part = s_part + (threadIdx.x >> 5) * 128;
-            float4 u;
-            unpack_f32x2(add_f32x2(product(a[0], a[0]), product(b[0], b[0])), u.x, u.y);
-            unpack_f32x2(add_f32x2(product(a[1], a[1]), product(b[1], b[1])), u.z, u.w);
-            __syncwarp();
-            reinterpret_cast<float4*>(part)[hl] = u;
-            __syncwarp();
-            const float* at = part + 4 * m + i;
-            ss = __fadd_rn(__fadd_rn(__fadd_rn(at[0], at[32]), at[64]), at[96]);
-            ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, 8));
-            ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, 16));
+            float x0, x1, x2, x3;
+            unpack_f32x2(add_f32x2(product(a[0], a[0]), product(b[0], b[0])), x0, x1);
+            unpack_f32x2(add_f32x2(product(a[1], a[1]), product(b[1], b[1])), x2, x3);
+            ss = __fadd_rn(__fadd_rn(__fadd_rn(x0, x1), x2), x3);
           } else {
-            float* part = s_part + (threadIdx.x >> 4) * 128;
-            float4 u, v;
-            unpack_f32x2(mul_f32x2(a[0], a[0]), u.x, u.y);
-            unpack_f32x2(mul_f32x2(a[1], a[1]), u.z, u.w);
-            unpack_f32x2(mul_f32x2(b[0], b[0]), v.x, v.y);
-            unpack_f32x2(mul_f32x2(b[1], b[1]), v.z, v.w);
-            __syncwarp(hmask);
-            reinterpret_cast<float4*>(part)[hl] = u;
-            reinterpret_cast<float4*>(part)[16 + hl] = v;
-            __syncwarp(hmask);
-            const uint64_t* at = reinterpret_cast<const uint64_t*>(part + 4 * m + 2 * i);
-            float t0, t1;
-            unpack_f32x2(add_f32x2(add_f32x2(add_f32x2(at[0], at[16]), at[32]), at[48]), t0, t1);
-            ss = __fadd_rn(t0, t1);
-            ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, 8));
+            auto four = [&](const uint64_t (&x)[2]) -> float {
+              float x0, x1, x2, x3;
+              unpack_f32x2(product(x[0], x[0]), x0, x1);
+              unpack_f32x2(product(x[1], x[1]), x2, x3);
+              return __fadd_rn(__fadd_rn(__fadd_rn(x0, x1), x2), x3);
+            };
+            ss = __fadd_rn(four(a), four(b));
           }
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, o));
+          for (int o = LANES / 2; o > 0; o >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(hmask, ss, o));
           const float inv = rsqrtf(ss * (1.f / HD) + p.eps);
           const uint64_t inv2 = pack_f32x2(inv, inv);
           const ulonglong2 wl = reinterpret_cast<const ulonglong2*>(weight)[hl], wh = reinterpret_cast<const ulonglong2*>(weight)[LANES + hl];
