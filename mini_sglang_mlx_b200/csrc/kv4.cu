@@ -160,9 +160,36 @@ bool q4_expands(int batch, int total_q, int64_t total_kv, int hq, int hkv, int h
   const double copy_us = 5. + (static_cast<double>(total_kv) * hkv * 5.2 + static_cast<double>(total_q) * hq * 4.) * head_dim / 4e6;
   return attend_us > (head_dim == 256 ? kQ4ExpandWorth256 : kQ4ExpandWorth128) * copy_us;
 }
+// The largest numbers of every sequence and head (kv4_range_kernel), for long ones.
+size_t q4_tops_bytes(int batch, int hkv) { return static_cast<size_t>(batch) * hkv * 2 * msgl::kRangeParts * sizeof(uint32_t); }
+// CTAs of a sequence and head: about eight per SM in all.  (Thirty-two of each: 16 sequences of 8 heads under a window of 4096, 4 us more.)
+int q4_range_parts(int batch, int hkv) {
+  int parts = msgl::kRangeParts;
+  while (parts > 1 && static_cast<int64_t>(batch) * hkv * parts > 148 * 8) parts /= 2;
+  return parts;
+}
+msgl::Kv4ExpandParams q4_range_params(const void* k_cache, const void* v_cache, const int32_t* page_indices, const int32_t* page_indptr,
+                                      const int32_t* kv_lens, const int32_t* prefix_lens, uint32_t* tops, int batch, int hkv,
+                                      int64_t num_slots, int page_size, int64_t total_pages, int window) {
+  msgl::Kv4ExpandParams x{};
+  x.k_pool = static_cast<const unsigned char*>(k_cache);
+  x.v_pool = static_cast<const unsigned char*>(v_cache);
+  x.page_indices = page_indices;
+  x.page_indptr = page_indptr;
+  x.kv_lens = kv_lens;
+  x.prefix_lens = prefix_lens;
+  x.tops = tops;
+  x.batch = batch;
+  x.hkv = hkv;
+  x.num_blocks = static_cast<int>(num_slots / msgl::kKv4Rows);
+  x.page_blocks = page_size / msgl::kKv4Rows;
+  x.total_pages = static_cast<int>(total_pages);
+  x.window = window;
+  x.parts = q4_range_parts(batch, hkv);
+  return x;
+}
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // K rows, V rows, sequences' powers, page ids, q rows and their powers.
-size_t q4_tops_bytes(int batch, int hkv) { return static_cast<size_t>(batch) * hkv * 2 * msgl::kRangeParts * sizeof(uint32_t); }
 size_t q4_expanded_bytes(int batch, int total_q, int64_t total_kv, int64_t total_pages, int hq, int hkv, int head_dim, int dtype) {
   const size_t rows = rounded(static_cast<size_t>(total_kv) * hkv * head_dim * 2);
   const size_t q_rows = static_cast<size_t>(total_q) * hq;
@@ -375,8 +402,9 @@ size_t msgl_prefill_workspace_bytes_q4(int batch, int total_q, int64_t total_pag
   max_len_extend = std::max(1, max_len_extend);
   const int group = std::max(1, num_q_heads / num_kv_heads);
   if (!q4_block_form(batch, max_len_extend, group))
-    return msgl_prefill_workspace_bytes(batch, total_q, total_pages * page_size, num_q_heads, num_kv_heads, head_dim,
-                                        max_len_extend, sliding_window_size);
+    return rounded(msgl_prefill_workspace_bytes(batch, total_q, total_pages * page_size, num_q_heads, num_kv_heads, head_dim,
+                                                max_len_extend, sliding_window_size)) +
+           q4_tops_bytes(batch, num_kv_heads);
   const int sms = sm_count_cached();
   const Q4Plan pl = plan_q4(batch, max_len_extend * group, num_kv_heads, head_dim,
                             q4_block_bound(batch, total_pages, page_size, max_len_extend, sliding_window_size), sms > 0 ? sms : 148);
@@ -457,8 +485,12 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
   }
   const PrefillPlan pl = plan_prefill(batch, total_q, total_pages * page_size, num_q_heads, num_kv_heads, head_dim,
                                       max_len_extend, sliding_window_size, sms);
-  if (!workspace || workspace_bytes < kStatusBytes + pl.plan_bytes + pl.part_ml_bytes + pl.part_o_bytes)
+  const size_t used = rounded(kStatusBytes + pl.plan_bytes + pl.part_ml_bytes + pl.part_o_bytes);
+  if (!workspace || workspace_bytes < used + q4_tops_bytes(batch, num_kv_heads))
     return fail(MSGL_BAD_ARG, std::string(op) + "workspace too small");
+  if (static_cast<int64_t>(batch) * num_kv_heads > 0x7fffffffLL)
+    return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
+  const dim3 range_grid(static_cast<unsigned>(batch * num_kv_heads * q4_range_parts(batch, num_kv_heads)));
   if (pl.items * num_kv_heads > 0x7fffffffLL)
     return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
   unsigned char* ws = static_cast<unsigned char*>(workspace);
@@ -504,28 +536,17 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     if (pairs * 2 > 0x7fffffffLL) return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
     const size_t rows = rounded(static_cast<size_t>(total_kv) * num_kv_heads * head_dim * 2);
     unsigned char* at = static_cast<unsigned char*>(expanded);
-    msgl::Kv4ExpandParams x{};
-    x.k_pool = static_cast<const unsigned char*>(k_cache);
-    x.v_pool = static_cast<const unsigned char*>(v_cache);
-    x.page_indices = page_indices;
+    msgl::Kv4ExpandParams x = q4_range_params(k_cache, v_cache, page_indices, page_indptr, kv_lens, prefix_lens,
+                                              reinterpret_cast<uint32_t*>(at + 2 * rows), batch, num_kv_heads, num_slots, page_size,
+                                              total_pages, sliding_window_size);
     x.k_rows = reinterpret_cast<__half*>(at);
     x.v_rows = reinterpret_cast<__half*>(at + rows);
     at += 2 * rows;
-    x.tops = reinterpret_cast<uint32_t*>(at);
     at += q4_tops_bytes(batch, num_kv_heads);
     x.pages = reinterpret_cast<int32_t*>(at);
     at += rounded(total_pages * sizeof(int32_t));
-    x.page_indptr = page_indptr;
-    x.kv_lens = kv_lens;
-    x.prefix_lens = prefix_lens;
-    x.batch = batch;
     x.qo_indptr = qo_indptr;
-    x.window = sliding_window_size;
     x.is_cross = is_cross_attention ? 1 : 0;
-    x.total_pages = static_cast<int>(total_pages);
-    x.page_blocks = page_size / msgl::kKv4Rows;
-    x.hkv = num_kv_heads;
-    x.num_blocks = static_cast<int>(num_slots / msgl::kKv4Rows);
     x.status = p.status;
     const bool convert = dtype == MSGL_DTYPE_BF16;
     if (convert) {
@@ -553,10 +574,8 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     p.num_slots = total_kv;
     p.kv_chunk = 0;
     p.chunk_recip = 0;
-    if (static_cast<int64_t>(batch) * num_kv_heads * msgl::kRangeParts > 0x7fffffffLL)
-      return fail(MSGL_BAD_SHAPE, std::string(op) + "problem too large for one launch");
     auto run = [&](auto range, auto expand, auto kernel, int threads, int smem) -> cudaError_t {
-      cudaError_t err = launch_dependent(range, dim3(static_cast<unsigned>(batch * num_kv_heads * msgl::kRangeParts)), dim3(256), 0, s, x);
+      cudaError_t err = launch_dependent(range, range_grid, dim3(256), 0, s, x);
       if (err != cudaSuccess) return err;
       err = launch_dependent(expand, dim3(static_cast<unsigned>(sms * 8)), dim3(256), 0, s, x);
       if (err != cudaSuccess) return err;
@@ -583,8 +602,19 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
   std::memset(&tm_q, 0, sizeof(tm_q));
   p.q_tma = make_query_tensor_map(&tm_q, q, total_q, num_q_heads, p.group, head_dim, dtype) ? 1 : 0;
   const dim3 grid(static_cast<unsigned>(pl.items * num_kv_heads));
-  auto launch = [&](auto kernel, auto merge, int threads, int smem) -> cudaError_t {
+  uint32_t* const tops = reinterpret_cast<uint32_t*>(ws + used);
+  const bool range_first = head_dim == 128 && !prefill_short_q(max_len_extend, p.group, head_dim);      // (prefill_tc_kernel's OWN_RANGE)
+  if (range_first) {
+    p.kv_tops = tops;
+    p.early = 1;          // what is older than the kernel in front is complete: the pool, q and the index arrays
+  }
+  auto launch = [&](auto range, auto kernel, auto merge, int threads, int smem) -> cudaError_t {
     cudaError_t err = allow_smem(kernel, smem);
+    if (err != cudaSuccess) return err;
+    if (range_first)
+      err = launch_dependent(range, range_grid, dim3(256), 0, s,
+                             q4_range_params(k_cache, v_cache, page_indices, page_indptr, kv_lens, prefix_lens, tops, batch, num_kv_heads,
+                                             num_slots, page_size, total_pages, sliding_window_size));
     if (err != cudaSuccess) return err;
     err = launch_dependent(kernel, grid, dim3(threads), smem, s, p, none, none, tm_q);
     if (err != cudaSuccess) return err;
@@ -598,12 +628,12 @@ int msgl_paged_prefill_attention_q4(const void* q, const void* k_cache, const vo
     using S2 = msgl::TcShape<2>;
     using S1w = msgl::TcShape<1, 256>;
     if (head_dim == 256)
-      return launch(msgl::prefill_tc_kernel<T, 64, 1, 256, false, true>, msgl::prefill_merge_kernel<T, 256, S1w::kBM>,
+      return launch(msgl::kv4_range_kernel<T, 256>, msgl::prefill_tc_kernel<T, 64, 1, 256, false, true>, msgl::prefill_merge_kernel<T, 256, S1w::kBM>,
                     S1w::kThreads, msgl::Kv4Shape<1, 256>::kSmemBytes);
     if (prefill_short_q(max_len_extend, p.group, head_dim))
-      return launch(msgl::prefill_tc_kernel<T, 64, 1, 128, false, true>, msgl::prefill_merge_kernel<T, 128, S1::kBM>,
+      return launch(msgl::kv4_range_kernel<T, 128>, msgl::prefill_tc_kernel<T, 64, 1, 128, false, true>, msgl::prefill_merge_kernel<T, 128, S1::kBM>,
                     S1::kThreads, msgl::Kv4Shape<1, 128>::kSmemBytes);
-    return launch(msgl::prefill_tc_kernel<T, 128, 2, 128, false, true>, msgl::prefill_merge_kernel<T, 128, S2::kBM>,
+    return launch(msgl::kv4_range_kernel<T, 128>, msgl::prefill_tc_kernel<T, 128, 2, 128, false, true>, msgl::prefill_merge_kernel<T, 128, S2::kBM>,
                   S2::kThreads, msgl::Kv4Shape<2, 128>::kSmemBytes);
   };
   const cudaError_t e = dtype == MSGL_DTYPE_BF16 ? dispatch(__nv_bfloat16{}) : dispatch(__half{});

@@ -381,6 +381,7 @@ struct Kv4ExpandParams {
   uint32_t* tops;               // (batch, hkv, 2, kRangeParts): the largest t of K and of V in parts of a sequence
   const int32_t *page_indptr, *kv_lens, *prefix_lens, *qo_indptr;
   int batch, window, is_cross;
+  int parts;                    // CTAs of a sequence and head in kv4_range_kernel: a power of two up to kRangeParts
   const void* q;                // (q_rows, head_dim), or null
   __half* q_rows;
   float* q_power;
@@ -406,13 +407,13 @@ __global__ void __launch_bounds__(256) kv4_range_kernel(const Kv4ExpandParams p)
   const int32_t* const indptr = after_wait(p.page_indptr);
   const int32_t* const lens = after_wait(p.kv_lens);
   const int32_t* const prefixes = after_wait(p.prefix_lens);
-  const int part = blockIdx.x % kRangeParts, h = blockIdx.x / kRangeParts % p.hkv, b = blockIdx.x / kRangeParts / p.hkv;
+  const int part = blockIdx.x % p.parts, h = blockIdx.x / p.parts % p.hkv, b = blockIdx.x / p.parts / p.hkv;
   const int page_size = p.page_blocks * kKv4Rows;
   const int begin = __ldg(indptr + b);
   const int64_t cap = static_cast<int64_t>(max(__ldg(indptr + b + 1) - begin, 0)) * page_size;
   const int len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(lens + b), 0)), cap));
   const int lo = p.window > 0 ? max(0, __ldg(prefixes + b) - p.window + 1) / 128 * 128 : 0;
-  const int per = (max(len - lo, 0) / kKv4Rows / kRangeParts + 1) * kKv4Rows;        // keys of a part
+  const int per = (max(len - lo, 0) / kKv4Rows / p.parts + 1) * kKv4Rows;        // keys of a part
   const int64_t from = lo + static_cast<int64_t>(part) * per;
   uint2 top = make_uint2(0u, 0u);
   if (from < len)
@@ -424,10 +425,13 @@ __global__ void __launch_bounds__(256) kv4_range_kernel(const Kv4ExpandParams p)
                                  });
   if (threadIdx.x % 32 == 0) s_top[threadIdx.x / 32] = top;
   __syncthreads();
-  if (threadIdx.x < 2) {
+  // (with fewer CTAs than places, all its places hold the same)
+  const int is_v = threadIdx.x / kRangeParts, place = threadIdx.x % kRangeParts;
+  if (is_v < 2 && place % p.parts == part) {
     uint32_t most = 0u;
-    for (int w = 0; w < 8; ++w) most = max(most, threadIdx.x == 0 ? s_top[w].x : s_top[w].y);
-    p.tops[((static_cast<int64_t>(b) * p.hkv + h) * 2 + threadIdx.x) * kRangeParts + part] = most;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) most = max(most, is_v == 0 ? s_top[w].x : s_top[w].y);
+    p.tops[((static_cast<int64_t>(b) * p.hkv + h) * 2 + is_v) * kRangeParts + place] = most;
   }
 }
 

@@ -97,10 +97,12 @@ struct TcShape {
 };
 
 // The same over a pool held in 4 bits (kv4.cuh).  The first copying warp fetches blocks (16 tokens of the head, one bulk copy)
-// into a ring of their own; the others, a block each in turn, write its elements into the tiles, scale * code + bias over the item's power of
-// two (range_power) rounded once to f16; the tiles' ring is shorter for it.  They find the powers first, from the pairs of the item's keys,
-// a ninth of what it reads, while the first blocks are on their way.  (Measured otherwise, five verify tokens 56.2 us without any powers,
-// 59 with these, 66 with a power for each block of sixteen keys, which the softmax warps then have to apply.)
+// into a ring of their own; the others, a block each in turn, write its elements into the tiles, scale * code + bias over a power of
+// two rounded once to f16; the tiles' ring is shorter for it.  With one sub-tile the power is of the item's keys, and the writing warps find it
+// first, from the pairs, a ninth of what the item reads, while the first blocks are on their way; with two, where items share long
+// ranges, it is of the sequence's, and a kernel in front finds it (kv4_range_kernel), while items are found and blocks fetched.
+// The first / the second way: five verify tokens 60 / 62.5 us, draft blocks 78.6 / 80.5, four times 512 tokens over 16000 644 / 594, 2048 over
+// 70000 2664 / 2451.  (Without powers 56, 72, 574, 2380; with one for each block of sixteen keys, applied by the softmax warps, 66, 88.)
 template <int NSUB, int HD>
 struct Kv4Shape {
   // (three buffers and twice the blocks: 512 tokens of four over 4096 115 us for 104, short blocks the same)
@@ -479,7 +481,7 @@ __device__ __noinline__ void merge_kv_splits_cta(const MergeArgs p, int nsp, int
 // KV4: the pool is held in 4 bits and addressed by pages (Kv4Shape).  Every operand is f16 there whatever T is: three bits of
 // fraction more than bf16 where elements of K and V and the weights are rounded (in bf16, results are 0.0035 off 64 bits as a
 // norm; the rounding of the output alone is 0.0017; with f16 outputs 0.00035, of which 0.00021).  The range that f16 lacks is in powers of two: a
-// row of q and the item's keys are divided by one, which comes back in the row's scale, and its values by another, which comes
+// row of q and the keys are divided by one each, which come back in the row's scale, and the values by another, which comes
 // back with the output.  Five verify tokens of 16 requests over
 // 1024 to 16384 56 us, 16 draft tokens of 16 under a window of 4096 72, four chunks of 300 to 512 over up to 4096 99 (over 16-bit pages
 // 53, 62, 82).  No part bounds it alone: 64 keys take an SM with two CTAs 1100 cycles, in which a quarter of the instructions expand
@@ -521,7 +523,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
   __shared__ uint64_t s_q_raw;                                // IN_PLACE: Q as it is has arrived
   __shared__ float s_row_power[CONVERT ? BM : 1];             // what a row of q was divided by
   constexpr int kWriters = Shape::kWarps - kTcProducerWarp0 - 1;     // KV4: warps that write tiles
-  __shared__ uint32_t s_tops[2][KV4 ? kWriters : 1];          // largest of K's and V's pairs that each of them found
+  constexpr bool OWN_RANGE = KV4 && NSUB == 1;
+  __shared__ uint32_t s_tops[2][OWN_RANGE ? kWriters : 1];    // largest of K's and V's pairs that each of them found
   __shared__ uint64_t s_tops_full;
   __shared__ int s_slots[KV4 ? 1 : (LA + 1) * BN];  // slot ids of the key tiles being copied / next to copy
 
@@ -561,7 +564,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     if constexpr (KV4) {
       init(s_raw_full, kRaw, 1);
       init(s_raw_empty, kRaw, 1);
-      init(&s_tops_full, 1, kWriters);
+      if constexpr (OWN_RANGE) init(&s_tops_full, 1, kWriters);
     }
     init(bars.empty, kTcBufs, 1);
     init(bars.stage, NSUB, SUB / 32);                  // one arrival per warp of the group
@@ -648,8 +651,11 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
 
   const uint32_t tmem = s_tmem_base;
   volatile int* abort_flag = &s_abort;
-  // KV4: what the item's K (0) or V (1) is divided by, once s_tops_full is complete (and the item has tiles)
-  auto item_power = [&](int j) -> float { return range_power(__reduce_max_sync(0xffffffffu, lane < kWriters ? s_tops[KV4 ? j : 0][lane] : 0u)); };
+  // KV4: what K (0) or V (1) is divided by, behind s_tops_full (of an item with tiles), or behind the wait
+  auto item_power = [&](int j) -> float {
+    if constexpr (OWN_RANGE) return range_power(__reduce_max_sync(0xffffffffu, lane < kWriters ? s_tops[j][lane] : 0u));
+    else return sequence_power(after_wait(p.kv_tops), it.b, p.hkv, h, j, lane);
+  };
 #ifdef MSGL_TRACE
   if (tid == 0) {
     MSGL_TR(3, clock64());          // set-up done
@@ -678,7 +684,8 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     // over 32768 286 / 274, 128 over 2048 39.6 / 37.9, twelve prompts of 500 398 / 394).
     constexpr bool kQFirst = NSUB == 2 && PAGED;
     auto load_q = [&]() {
-    if (p.early) grid_dependency_wait();
+    // (KV4: the kernel in front, kv4_range_kernel, writes nothing that the fetching warp reads)
+    if (p.early && !(KV4 && warp == kTcProducerWarp0)) grid_dependency_wait();
     if (NSUB == 1 && ntiles == 0) return;      // (the epilogue's zeros are staged where Q would land)
     if constexpr (CONVERT && !IN_PLACE) return;      // (Q is the softmax warps')
     if (q_tma) {
@@ -916,19 +923,21 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
         constexpr int PPR = HD / 32, RPP = 32 / PPR;   // rows a pass
         const int dw = warp - kTcProducerWarp0 - 1;
         const int piece = lane % PPR, rsub = lane / PPR;
-        if (ntiles > 0) {
-          const int page_blocks = p.page_size / kKv4Rows;
-          const uint2 tops = pair_range<T, HD, DW * 32>(
-              after_wait(kbase), after_wait(vbase), p.hkv, h, kv_lo, kv_hi_load, p.num_slots / kKv4Rows, dw * 32 + lane, [&](int t) -> int64_t {
-                const int page = divide_by(t, p.page_recip);
-                return static_cast<int64_t>(__ldg(p.page_indices + sq.kv_begin + page)) * page_blocks + (t - page * p.page_size) / kKv4Rows;
-              });
-          if (lane == 0) {
-            s_tops[0][dw] = tops.x;
-            s_tops[1][dw] = tops.y;
-            mbar_arrive(smem_u32(&s_tops_full));
+        if constexpr (OWN_RANGE) {
+          if (ntiles > 0) {
+            const int page_blocks = p.page_size / kKv4Rows;
+            const uint2 tops = pair_range<T, HD, DW * 32>(
+                after_wait(kbase), after_wait(vbase), p.hkv, h, kv_lo, kv_hi_load, p.num_slots / kKv4Rows, dw * 32 + lane, [&](int t) -> int64_t {
+                  const int page = divide_by(t, p.page_recip);
+                  return static_cast<int64_t>(__ldg(p.page_indices + sq.kv_begin + page)) * page_blocks + (t - page * p.page_size) / kKv4Rows;
+                });
+            if (lane == 0) {
+              s_tops[0][dw] = tops.x;
+              s_tops[1][dw] = tops.y;
+              mbar_arrive(smem_u32(&s_tops_full));
+            }
+            alive = mbar_wait_warp(smem_u32(&s_tops_full), 0, abort_flag);
           }
-          alive = mbar_wait_warp(smem_u32(&s_tops_full), 0, abort_flag);
         }
         const float k_inverse = power_inverse(item_power(0)), v_inverse = power_inverse(item_power(1));
         each_tile([&](int seq, bool is_v, int tile, int at) {
@@ -1226,7 +1235,7 @@ __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
     float v_power = 1.f;
     if constexpr (KV4) {
       if (my_tiles > 0) {
-        alive = mbar_wait_warp(smem_u32(&s_tops_full), 0, abort_flag) && alive;
+        if constexpr (OWN_RANGE) alive = mbar_wait_warp(smem_u32(&s_tops_full), 0, abort_flag) && alive;
         v_power = item_power(1);
         row_scale *= item_power(0);
         // (above zero also where the powers leave nothing: a masked score is -inf)

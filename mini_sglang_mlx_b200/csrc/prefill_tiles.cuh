@@ -53,8 +53,8 @@ struct PrefillParams {
   int kv_chunk;  // tokens per kv split; 0 = never split
   uint64_t group_recip, page_recip, chunk_recip;   // of group, page_size and kv_chunk: see divide_by
   const float* q_power;  // (total_q, hq): what the rows of a converted q were divided by (else unused)
-  const uint32_t* kv_tops;   // of expanded pages: see sequence_power (else unused)
-  int early;     // the kernel in front is this call's own K/V store: the index arrays are complete
+  const uint32_t* kv_tops;   // of a 4-bit pool, see sequence_power (else unused)
+  int early;     // the kernel in front is this call's own K/V store (or kv4_range_kernel): the index arrays are complete
 };
 
 // x / d for 0 <= x < 2^31 without a division: recip = ceil(2^64 / d), 0 for d = 1 (the excess over 2^64 / d,

@@ -59,7 +59,8 @@ def test_workspace_of_a_batch_beyond_the_decode_kernels():
     for batch in (65535, 65536, 70000):
         got = lib.msgl_prefill_workspace_bytes_q4(batch, batch, batch, 16, 16, 2, 128, 1, 0)
         tiles = lib.msgl_prefill_workspace_bytes(batch, batch, batch * 16, 16, 2, 128, 1, 0)
-        assert (got == tiles) == (batch > 65535)
+        tops = batch * 2 * 64 * 4                      # (the largest numbers of every sequence and head, behind what the tile kernel takes)
+        assert (0 <= got - tiles - tops < 256) == (batch > 65535)
 
 
 @pytest.mark.gpu
