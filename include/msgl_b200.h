@@ -489,7 +489,7 @@ int msgl_prefill_layer_pages(const msgl_new_rows* rows, void* q, void* k_cache, 
  * 9 * head_dim / 2) elements of the 16-bit data type, contiguous and 16-byte aligned: per block and KV head the
  * codes of its sixteen rows, head_dim / 2 bytes each, then sixteen rows of (scale, bias) pairs, one pair for every
  * 64 elements of a row.  An element is scale * code + bias; in a group of 64, bias = min,
- * scale = T((max - min) / 15) (0 where that is below 2^-100) and code = min(15, rint((x - bias) / scale)).  The
+ * scale = T((max - min) / 15) (0 where that is below 2^-100) and code = min(15, rint((x - bias) / scale)), x - bias in fp32.  The
  * 32-bit word r * (head_dim / 64) + g of a row holds elements 64 g + 8 r to 64 g + 8 r + 7, element e of them in
  * nibble e / 2 + 4 * (e % 2).  A pool of zero bytes reads as zeros.  Magnitudes above 2^15 and
  * infinities are stored as 2^15, NaN as 0, and reported: a status word gets 4 added.  Slots and page ids outside the pool get 2 added.

@@ -32,11 +32,11 @@
 // The weights' reference maximum, a whole number, moves only when a score passes it by more than 2^8, and f when p scale_g could pass
 // 2^15 / f by the largest of both in a lane, so that maxima need not be reduced in every step.
 //
-// What bounds it: integer instructions that take the codes apart, next to the memory.  32 requests of 4096 to 32768 tokens, 8 KV heads
-// of 128, four query heads each: 108 us behind a write of the whole L2, 99 without, 4.7 and 5.1 TB/s (the same over 16-bit pages:
-// 290); 460 cycles of an SM quarter a block, 16 products of 8 cycles and 210 cycles of the integer pipe.  At head_dim 256 a
-// warp's sums leave two warps a quarter: 19 requests of 512 to 16384 tokens, two KV heads, 27 us, 20 of them start, ends and merges
-// around a loop of six steps; at few tokens the launch (700 tokens 7.9 us, the 16-bit operator 8.3).
+// What bounds it: no one pipe; integer instructions that take the codes apart (52 % of that pipe, as of the issue slots), by eight warps an SM, next
+// to the memory.  32 requests of 4096 to 32768 tokens, 8 KV heads of 128, four query heads each: 111 to 116 us behind a write of the whole
+// L2, 109 without, 4.4 to 4.7 TB/s (the same over 16-bit pages: 290; with one power of two for all scales 108 and 99).  At head_dim 256 a
+// warp's sums leave two warps a quarter: 19 requests of 512 to 16384 tokens, two KV heads, 30 us, 20 of them start, ends and merges
+// around a loop of six steps; at few tokens the launch (700 tokens 8.4 us, the 16-bit operator 8.3).
 #pragma once
 
 #include "kv4.cuh"

@@ -81,7 +81,7 @@ cudaError_t launch_q4(const msgl::Q4DecodeParams& p, cudaStream_t s, const CUten
 // Blocks a step, warps, stages of the ring and CTAs per SM, by what fits (255 registers at eight warps an SM).  Eight columns of 128,
 // 441093 tokens: 4 blocks, 4 warps, 2 CTAs 109 us; 2, 4, 3 CTAs 115; 4, 8, one CTA 125; 2, 12, one 129.  Head_dim 256, 97061
 // tokens: 2 blocks, 8 warps, one CTA 29.3 us; 2, 4, two CTAs 32.1; 1, 12, one 33.9; 1, 4, three 38.4.  (Measured with
-// a copy for each block; 99 and 26.1 us since.)  Sixteen columns: 2 blocks and a third stage, for their sums take twice the registers.
+// a copy for each block, and one power of two for all scales; 109 and 27.4 us since.)  Sixteen columns: 2 blocks and a third stage, for their sums take twice the registers.
 template <bool BLOCKS>
 cudaError_t launch_q4_any(const msgl::Q4DecodeParams& p, int head_dim, int cols, int dtype, cudaStream_t s,
                           const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
@@ -129,7 +129,7 @@ int run_q4(const char* op, msgl::Q4DecodeParams& p, const Q4Plan& pl, void* work
 
 // Query blocks of few columns per KV head run the decode kernel (decode_q4.cuh), others the one-CTA tcgen05 kernel.  16 sequences of
 // 16384 tokens, 8 KV heads, decode kernel / tcgen05: 8 columns 69 us / 222, 16 columns 115 / 222; with 20 to 64 columns as CTAs of
-// 16 side by side, five verify tokens of 40 columns 81 / 63, draft blocks of 64 149 / 86 (56 and 72 since).
+// 16 side by side, five verify tokens of 40 columns 81 / 63, draft blocks of 64 149 / 86 (60 and 78 since).
 constexpr int kQ4BlockColumns = 16;
 bool q4_block_form(int batch, int max_len_extend, int group) {
   return batch <= 65535 && static_cast<int64_t>(max_len_extend) * group <= kQ4BlockColumns;

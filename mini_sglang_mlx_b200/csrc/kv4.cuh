@@ -5,7 +5,7 @@
 // elements of a row.  So all that one KV head of a 16-token page takes is contiguous (1152 or 2304 bytes): one bulk copy.
 // An element is scale * code + bias with, in a group of 64,
 //
-//   bias = min,   scale = T((max - min) / 15)   (0 below 2^-100),   code = min(15, rint((x - bias) / scale)),
+//   bias = min,   scale = T((max - min) / 15)   (0 below 2^-100),   code = min(15, rint((x - bias) / scale)),   x - bias in fp32,
 //
 // so min itself is held exactly, and an element is off by half a scale, and by 15 half units in the last place of the scale.
 // Word r * (head_dim / 64) + g of a row holds elements 64 g + 8 r .. + 7: a lane that takes consecutive words gets the same
@@ -169,8 +169,8 @@ __device__ __forceinline__ uint32_t f16_pair(T, uint32_t pair, float by) {
 // Codes of the 2 W elements that a lane holds of a group of 64, LANES = 32 / W lanes of `mask` together, and the group's pair
 // (scale in the low half).  Element e comes back in nibble e / 2 + 4 (e % 2) of the result (W = 2: of its four lowest
 // nibbles of each half, to be shifted by 8 for the upper half of a word).
-// The quotient is that of an IEEE division (an approximate one, then its exact remainder): x - bias and scale are short
-// numbers whose quotient is often half-way between two codes, where a unit in the last place decides.
+// The quotient is an approximate one, corrected once by its exact remainder (Markstein), which makes it right at halves: x - bias and
+// scale are short numbers whose quotient is often half-way between two codes, where a unit in the last place decides.
 template <typename T, int W>
 __device__ __forceinline__ uint32_t kv4_quantise(uint32_t (&x)[W], uint32_t mask, uint32_t& pair, int* status) {
   constexpr int LANES = 32 / W;
@@ -368,11 +368,11 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(Kv4LoadParams p) {
 
 // ---------------------------------------------------------------- pages laid out for the pairs of CTAs
 // A long prefill reads a key once for every 256 query rows, and to expand its codes each time is what bounds the kernel that does
-// (one CTA; 4096 tokens over 16384 1425 us).  Expanded once into f16 pages, one per entry of the index list and
+// (one CTA; 4096 tokens over 16384 1425 us when that was measured).  Expanded once into f16 pages, one per entry of the index list and
 // in its order, they come by TMA and pairs of CTAs share them.  A sequence's keys and values of a head are divided by powers of two
 // (range_power), which a kernel in front finds.  q goes with them, as f16 over a power of two per row (bf16 only).
 // Bound by memory: 2.6 bytes an element of the pool, 4 of q; 20480 tokens of 8 heads of 128 and 4096 queries of 32 heads 34 us, 5.2
-// TB/s, in front of an attention of 1010 (with 116 registers and two CTAs per SM 44).
+// TB/s, in front of an attention of 990 (with 116 registers and two CTAs per SM 44).
 struct Kv4ExpandParams {
   const unsigned char *k_pool, *v_pool;
   const int32_t* page_indices;
@@ -397,7 +397,7 @@ __device__ __forceinline__ float sequence_power(const uint32_t* tops, int b, int
 }
 
 // A CTA for each part of each sequence and head: the keys from the first that a row's window can reach (and the tile of 128 that it is
-// in) to the last.  A ninth of the pool is read.
+// in) to the last.  A ninth of the pool is read; 20480 tokens of 8 heads 6 us.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) kv4_range_kernel(const Kv4ExpandParams p) {
   __shared__ uint2 s_top[8];

@@ -483,10 +483,10 @@ __device__ __noinline__ void merge_kv_splits_cta(const MergeArgs p, int nsp, int
 // norm; the rounding of the output alone is 0.0017; with f16 outputs 0.00035, of which 0.00021).  The range that f16 lacks is in powers of two: a
 // row of q and the keys are divided by one each, which come back in the row's scale, and the values by another, which comes
 // back with the output.  Five verify tokens of 16 requests over
-// 1024 to 16384 56 us, 16 draft tokens of 16 under a window of 4096 72, four chunks of 300 to 512 over up to 4096 99 (over 16-bit pages
+// 1024 to 16384 60 us, 16 draft tokens of 16 under a window of 4096 78, four chunks of 300 to 512 over up to 4096 103 (over 16-bit pages
 // 53, 62, 82).  No part bounds it alone: 64 keys take an SM with two CTAs 1100 cycles, in which a quarter of the instructions expand
 // codes and a seventh are the softmax, the rest copies, waits and bookkeeping of twelve warps; each waits for the others in turn.  Without
-// the expansion verify blocks take as long, without the softmax 7 % less, with 64 rows spread over 128 lanes (half a key tile each) 60 us.
+// the expansion verify blocks take as long, without the softmax 7 % less, with 64 rows spread over 128 lanes (half a key tile each) 60 us for 56.
 template <typename T, int BN, int NSUB, int HD = 128, bool PAGED = false, bool KV4 = false>
 __global__ void __launch_bounds__(TcShape<NSUB, HD, PAGED>::kThreads,
                                   TcShape<NSUB, HD, PAGED>::kMinCtasForRegs)

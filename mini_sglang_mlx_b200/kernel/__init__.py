@@ -531,7 +531,10 @@ def _check_attention_q4(op: str, q, k_cache, v_cache, gate) -> None:
 def paged_decode_attention_q4(q, k_cache, v_cache, page_indptr, page_indices, kv_lens, sm_scale: float, *,
                               page_size: int = 16, gate=None, stream=None) -> torch.Tensor:
     """``paged_decode_attention_p16`` over 4-bit pools.  ``page_size``: a multiple of 16 (slot = page * page_size +
-    offset).  Without the split hints of that operator, which it does not read either: the batch is cut into equal shares."""
+    offset).  Without the split hints of that operator, which it does not read either: the batch is cut into equal shares.
+
+    The weight times the value's scale is rounded to f16 over a power of two of the query head and the group of 64 elements: eleven
+    bits down to 2**-13 of the largest such product, below that 2**-24 of it."""
     args = (q, k_cache, v_cache, page_indptr, page_indices, kv_lens, sm_scale, page_size, gate,
             None if stream is None else _handle(stream))
     out = _ops.decode_q4(*args)
@@ -549,7 +552,10 @@ def paged_prefill_attention_q4(q, k_cache, v_cache, qo_indptr, page_indptr, page
                                is_cross_attention: bool = False, sliding_window_size: int = 0, gate=None,
                                stream=None) -> torch.Tensor:
     """``paged_prefill_attention_p16`` over 4-bit pools: ragged query blocks over prefix and new tokens, causal,
-    bidirectional or under a sliding window; rows without a visible key give zeros.  ``page_size``: a multiple of 16."""
+    bidirectional or under a sliding window; rows without a visible key give zeros.  ``page_size``: a multiple of 16.
+
+    With more than 16 rows (new tokens times query heads) a KV head, keys and values are rounded to f16 over a power of two: eleven
+    bits down to 2**-27 of a head's largest, below that 2**-38 of it; and weights, down to 2**-21 of a row's largest."""
     args = (q, k_cache, v_cache, qo_indptr, page_indptr, page_indices, kv_lens, prefix_lens, sm_scale, max_len_extend,
             page_size, is_cross_attention, sliding_window_size, gate, None if stream is None else _handle(stream))
     out = _ops.prefill_q4(*args)
